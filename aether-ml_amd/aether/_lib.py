@@ -52,6 +52,10 @@ SIGNATURES = {
     "aeth_bn_fwd_train_f32": [_p, _p, _p, _p, _p, _p, _p, _p, _i, _i, _f, _f],
     "aeth_bn_fwd_infer_f32": [_p, _p, _p, _p, _p, _p, _i, _i, _f],
     "aeth_bn_bwd_f32": [_p, _p, _p, _p, _p, _p, _p, _p, _i, _i],
+    "aeth_ln_fwd_f32": [_p] * 6 + [_i, _i, _f],
+    "aeth_ln_fwd_twin_f32": [_p] * 7 + [_i, _i, _f],
+    "aeth_ln_bwd_f32": [_p] * 8 + [_i, _i],
+    "aeth_ln_bwd_twin_f32": [_p] * 9 + [_i, _i],
     "aeth_relu_fwd_f32": [_p, _p, _f, _i64],
     "aeth_relu_bwd_f32": [_p, _p, _p, _f, _i64],
     "aeth_relu_fwd_twin_f32": [_p, _p, _p, _f, _i64],

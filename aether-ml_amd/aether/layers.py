@@ -595,6 +595,87 @@ class Batch_Norm:
 
 
 # ----------------------------------------------------------------------------------
+# Layer_Norm  (no counterpart in the reference: stands where a Batch_Norm would, for batches
+# too small for batch statistics; every sample, or pixel, is normalised over its features)
+# ----------------------------------------------------------------------------------
+class Layer_Norm:
+    """y = (x - mean) / sqrt(var + epsilon) * gamma + beta with mean and (biased) variance over the last axis.  gamma and
+    beta are `weights` and `biases`, trained like a Batch_Norm's; nothing is accumulated over steps, so training and
+    inference give the same output (`training` only decides whether the row statistics are kept for `backward`)."""
+
+    def __init__(self, epsilon=1e-5, n_features=None):
+        if not epsilon >= 0:
+            raise ValueError(f"Expected epsilon >= 0, got {epsilon}.")
+        self.epsilon = epsilon
+        if n_features is not None:
+            self.gamma = DeviceTensor.full(n_features, 1.0)
+            self.beta = DeviceTensor.zeros(n_features)
+        else:
+            self.gamma = None
+            self.beta = None
+        self.weights = self.gamma
+        self.biases = self.beta
+        self.row_mean = None
+        self.row_invstd = None
+        self.weight_regularizer_l1 = 0
+        self.weight_regularizer_l2 = 0
+        self.bias_regularizer_l1 = 0
+        self.bias_regularizer_l2 = 0
+
+    def forward(self, inputs, training):
+        inputs = as_device(inputs, _F32)
+        if inputs.ndim < 2:
+            raise ValueError(f"Expected a tensor of rows, got {inputs.ndim} dimension(s).")
+        C = inputs.shape[-1]
+        if self.gamma is None:
+            self.set_parameters(DeviceTensor.full(C, 1.0), DeviceTensor.zeros(C))
+        if self.gamma.size != C or self.beta.size != C:
+            raise ValueError(f"Expected {self.gamma.size} features, got {C}.")
+        rows = 1
+        for n in inputs.shape[:-1]:
+            rows *= n
+        self.inputs = inputs
+        self.output = DeviceTensor(inputs.shape, _F32)
+        self.row_mean = DeviceTensor(rows, _F32) if training else None
+        self.row_invstd = DeviceTensor(rows, _F32) if training else None
+        head = (inputs.ptr, self.gamma.ptr, self.beta.ptr, self.row_mean.ptr if training else None,
+                self.row_invstd.ptr if training else None, self.output.ptr)
+        if _wants_bf16(getattr(self, "next", None)):
+            _ck(_L().aeth_ln_fwd_twin_f32(*head, _twin(self.output).ptr, rows, C, self.epsilon))
+        else:
+            _ck(_L().aeth_ln_fwd_f32(*head, rows, C, self.epsilon))
+        return self.output
+
+    def backward(self, dvalues):
+        if self.row_mean is None:
+            raise ValueError("Layer_Norm.backward needs the row statistics of a forward pass with training=True")
+        dvalues = as_device(dvalues, _F32)
+        if dvalues.size != self.inputs.size:
+            raise ValueError(f"gradient shape {dvalues.shape} does not match output shape {self.inputs.shape}")
+        C = self.inputs.shape[-1]
+        rows = self.row_mean.size
+        self.dinputs = DeviceTensor(self.inputs.shape, _F32)
+        self.dweights = DeviceTensor(C, _F32)
+        self.dbiases = DeviceTensor(C, _F32)
+        head = (self.inputs.ptr, dvalues.ptr, self.gamma.ptr, self.row_mean.ptr, self.row_invstd.ptr, self.dinputs.ptr)
+        tail = (self.dweights.ptr, self.dbiases.ptr, rows, C)
+        if _wants_bf16(getattr(self, "prev", None)):
+            _ck(_L().aeth_ln_bwd_twin_f32(*head, _twin(self.dinputs).ptr, *tail))
+        else:
+            _ck(_L().aeth_ln_bwd_f32(*head, *tail))
+        return self.dinputs
+
+    def get_parameters(self):
+        return self.gamma, self.beta
+
+    def set_parameters(self, gamma, beta):
+        self.gamma = as_device(gamma, _F32).reshape(-1)
+        self.beta = as_device(beta, _F32).reshape(-1)
+        self.weights = self.gamma
+        self.biases = self.beta
+
+
+# ----------------------------------------------------------------------------------
 # Flatten / SoftMax  (CNN_classes_cupy.py:528-563)
 # ----------------------------------------------------------------------------------
 class Flatten:

@@ -196,6 +196,27 @@ int aeth_bn_fwd_infer_f32(const float* x, const float* gamma, const float* beta,
 int aeth_bn_bwd_f32(const float* x, const float* dy, const float* gamma,
                     const float* save_mean, const float* save_invstd,
                     float* dx, float* dgamma, float* dbeta, int rows, int C);
+/* Layer norm over the last axis (no counterpart in the reference; it stands where a batch norm would, for batches too small
+ * for batch statistics): rows = product of the leading axes, each row normalised on its own.
+ * ln_fwd : mean = sum_c x / C, invstd = 1 / sqrt(sum_c (x - mean)^2 / C + eps), y = (x - mean) invstd gamma + beta; the row
+ *          statistics [rows] go to save_mean / save_invstd for the backward pass, or nowhere if both are NULL (inference).
+ * ln_bwd : with xhat = (x - mean) invstd and g = dy gamma: dx = invstd (g - sum_c g / C - xhat sum_c g xhat / C),
+ *          dgamma = sum_rows dy xhat, dbeta = sum_rows dy, each element written.  Deterministic.
+ * rows may be 0 (dgamma = dbeta = 0).  A NaN or an infinity stays in its row (and, backward, in its columns' dgamma /
+ * dbeta).  Outputs may not overlap inputs.  The _twin_ forms also leave a bfloat16 copy of y / dx, as the other producers do
+ * (aeth_relu_fwd_twin_f32 below). */
+int aeth_ln_fwd_f32(const float* x, const float* gamma, const float* beta,
+                    float* save_mean /* may be NULL */, float* save_invstd /* NULL with save_mean */, float* y,
+                    int rows, int C, float eps);
+int aeth_ln_fwd_twin_f32(const float* x, const float* gamma, const float* beta,
+                         float* save_mean /* may be NULL */, float* save_invstd /* NULL with save_mean */,
+                         float* y, uint16_t* y_bf16, int rows, int C, float eps);
+int aeth_ln_bwd_f32(const float* x, const float* dy, const float* gamma,
+                    const float* save_mean, const float* save_invstd,
+                    float* dx, float* dgamma, float* dbeta, int rows, int C);
+int aeth_ln_bwd_twin_f32(const float* x, const float* dy, const float* gamma,
+                         const float* save_mean, const float* save_invstd,
+                         float* dx, uint16_t* dx_bf16, float* dgamma, float* dbeta, int rows, int C);
 /* ReLU (alpha = 0) :406-415 and Leaky_ReLU :417-428.
  * fwd: y = x > 0 ? x : alpha*x ;  bwd: dx = x < 0 ? alpha*dy : dy  (strict <). */
 int aeth_relu_fwd_f32(const float* x, float* y, float alpha, int64_t n);

@@ -1,0 +1,276 @@
+"""Layer_Norm and the aeth_ln_* entry points against the formulas in 64 bits (tests/norm_reference.py derives the
+tolerances), against differences, at the sizes, alignments and values where they can go wrong."""
+import ctypes as C
+
+import numpy as np
+import pytest
+
+from oracle import oracle as O
+from tests import norm_reference as R
+
+pytestmark = pytest.mark.gpu
+
+
+def _dev(a):
+    from aether import DeviceTensor
+    return DeviceTensor.from_numpy(a, np.float32)
+
+
+def _nan(shape, dtype=np.float32):
+    from aether import DeviceTensor
+    t = DeviceTensor(shape, dtype)
+    return t.set(np.full(shape, np.nan if dtype == np.float32 else 0x7fff, dtype))
+
+
+def _lib():
+    from aether import _lib
+    return _lib.lib(), _lib.check
+
+
+def _forward(x, gamma, beta, eps=1e-5, saves=True, twin=False):
+    lib, check = _lib()
+    rows, c = x.shape
+    y, m, s = _nan((rows, c)), _nan(rows), _nan(rows)
+    xd, gd, bd = _dev(x), _dev(gamma), _dev(beta)
+    head = (xd.ptr, gd.ptr, bd.ptr, m.ptr if saves else None, s.ptr if saves else None, y.ptr)
+    y16 = _nan((rows, c), np.uint16) if twin else None
+    if twin:
+        check(lib.aeth_ln_fwd_twin_f32(*head, y16.ptr, rows, c, eps))
+    else:
+        check(lib.aeth_ln_fwd_f32(*head, rows, c, eps))
+    return y.get(), m.get(), s.get(), y16.get() if twin else None
+
+
+def _backward(x, dy, gamma, mean, invstd, twin=False):
+    lib, check = _lib()
+    rows, c = x.shape
+    dx, dg, db = _nan((rows, c)), _nan(c), _nan(c)
+    t = [_dev(a) for a in (x, dy, gamma, mean, invstd)]
+    head = tuple(a.ptr for a in t) + (dx.ptr,)
+    dx16 = _nan((rows, c), np.uint16) if twin else None
+    if twin:
+        check(lib.aeth_ln_bwd_twin_f32(*head, dx16.ptr, dg.ptr, db.ptr, rows, c))
+    else:
+        check(lib.aeth_ln_bwd_f32(*head, dg.ptr, db.ptr, rows, c))
+    return dx.get(), dg.get(), db.get(), dx16.get() if twin else None
+
+
+def _inputs(rows, c, seed=0):
+    r = np.random.RandomState(seed + 7 * rows + c)
+    x = (r.randn(rows, c) * (0.5 + r.rand(c)) + r.randn(c)).astype(np.float32)
+    return x, (1 + 0.2 * r.randn(c)).astype(np.float32), r.randn(c).astype(np.float32), r.randn(rows, c).astype(np.float32)
+
+
+# rows x features: one of each, row lengths on both sides of every power of two that a kernel could switch at, rows that
+# no vector divides, rows longer than a workgroup's registers, many short rows
+SIZES = [(1, 1), (1, 4), (5, 1), (3, 2), (7, 3), (1, 256), (128, 256), (2, 15), (2, 16), (9, 17), (33, 31), (64, 32), (65, 33),
+         (31, 60), (130, 63), (257, 64), (17, 65), (19, 100), (5, 127), (66, 128), (5, 129), (12, 252), (3, 255), (3, 257),
+         (7, 260), (4, 511), (6, 512), (3, 513), (5, 1000), (2, 1023), (9, 1024), (3, 1025), (2, 1537), (6, 2048), (3, 2049),
+         (2, 4095), (5, 4096), (2, 4100), (2, 5001), (3, 8192), (2, 8193), (2, 8196), (2, 16384), (1, 16385), (3, 20000),
+         (1, 32768), (2, 32769), (1, 40004), (1, 70001), (3, 100000), (1000, 8), (2000, 5), (1500, 64), (1030, 100), (700, 1024)]
+
+
+@pytest.mark.parametrize("rows,c", SIZES)
+def test_forward_and_backward(rows, c):
+    x, gamma, beta, dy = _inputs(rows, c)
+    (y, mean, inv), (e_y, e_mean, e_inv) = R.forward(x, gamma, beta, 1e-5)
+    got = _forward(x, gamma, beta)
+    assert R.worst(got[0], y, e_y) <= 1 and R.worst(got[1], mean, e_mean) <= 1 and R.worst(got[2], inv, e_inv) <= 1
+    # without statistics the output has the same bits
+    assert np.array_equal(_forward(x, gamma, beta, saves=False)[0], got[0])
+    want, bounds = R.backward(x, dy, gamma, got[1], got[2])
+    back = _backward(x, dy, gamma, got[1], got[2])
+    for g, w, b, name in zip(back, want, bounds, ("dx", "dgamma", "dbeta")):
+        assert R.worst(g, w, b) <= 1, name
+    # the same call again gives the same bits
+    again = _backward(x, dy, gamma, got[1], got[2])
+    assert all(np.array_equal(a, b) for a, b in zip(again[:3], back[:3]))
+
+
+@pytest.mark.parametrize("rows,c", [(1, 1), (5, 3), (129, 64), (7, 100), (3, 1025), (40, 1024), (2, 20000), (1, 40001)])
+def test_twins_are_the_rounded_outputs(rows, c):
+    x, gamma, beta, dy = _inputs(rows, c, seed=1)
+    plain, twin = _forward(x, gamma, beta), _forward(x, gamma, beta, twin=True)
+    assert np.array_equal(plain[0], twin[0]) and np.array_equal(twin[3], O.bf16_bits(twin[0]))
+    a, b = _backward(x, dy, gamma, plain[1], plain[2]), _backward(x, dy, gamma, plain[1], plain[2], twin=True)
+    assert all(np.array_equal(p, q) for p, q in zip(a[:3], b[:3])) and np.array_equal(b[3], O.bf16_bits(b[0]))
+
+
+@pytest.mark.parametrize("rows,c,skip", [(6, 64, 1), (6, 100, 2), (5, 1024, 3), (3, 4096, 1), (2, 20000, 3)])
+def test_pointers_that_are_only_four_byte_aligned(rows, c, skip):
+    """Views that start `skip` floats into a block: no 16-byte load is aligned, the results are those of aligned ones within
+    the tolerance, and the floats in front of and behind the outputs stay."""
+    lib, check = _lib()
+    x, gamma, beta, dy = _inputs(rows, c, seed=2)
+
+    def shifted(a):
+        whole = np.full(a.size + 8, 123.0, np.float32)
+        whole[skip:skip + a.size] = a.reshape(-1)
+        return _dev(whole)
+
+    t = {k: shifted(v) for k, v in (("x", x), ("gamma", gamma), ("beta", beta), ("dy", dy))}
+    out = {k: shifted(np.zeros(n, np.float32)) for k, n in (("y", rows * c), ("dx", rows * c), ("m", rows), ("s", rows),
+                                                             ("dg", c), ("db", c))}
+    at = lambda d, *names: [d[k].ptr + 4 * skip for k in names]  # noqa: E731
+    check(lib.aeth_ln_fwd_f32(*at(t, "x", "gamma", "beta"), *at(out, "m", "s", "y"), rows, c, 1e-5))
+    check(lib.aeth_ln_bwd_f32(*at(t, "x", "dy", "gamma"), *at(out, "m", "s", "dx", "dg", "db"), rows, c))
+    got = {k: v.get() for k, v in out.items()}
+    for k, v in got.items():
+        n = v.size - 8
+        assert np.all(v[:skip] == 123.0) and np.all(v[skip + n:] == 123.0), k
+        got[k] = v[skip:skip + n]
+    (y, mean, inv), (e_y, e_mean, e_inv) = R.forward(x, gamma, beta, 1e-5)
+    assert R.worst(got["y"], y, e_y) <= 1 and R.worst(got["m"], mean, e_mean) <= 1 and R.worst(got["s"], inv, e_inv) <= 1
+    want, bounds = R.backward(x, dy, gamma, got["m"], got["s"])
+    for k, w, b in zip(("dx", "dg", "db"), want, bounds):
+        assert R.worst(got[k], w, b) <= 1, k
+
+
+@pytest.mark.parametrize("c", [48, 1000, 40000])
+def test_rows_far_from_zero_and_constant_rows(c):
+    """A mean a thousand times the spread costs what the inputs' own rounding costs and no more; a constant row has
+    variance 0 and gives beta."""
+    r = np.random.RandomState(c)
+    x = (1000 + r.randn(4, c)).astype(np.float32)
+    x[2] = 0.1
+    x[3] = 0.0
+    gamma, beta = np.ones(c, np.float32), r.randn(c).astype(np.float32)
+    (y, _, _), (e_y, _, _) = R.forward(x, gamma, beta, 1e-5)
+    got = _forward(x, gamma, beta)[0]
+    assert R.worst(got[:2], y[:2], e_y[:2]) <= 1 and R.worst(got[2], y[2], e_y[2]) <= 1
+    assert np.array_equal(got[3], beta)
+
+
+@pytest.mark.parametrize("c", [3, 64, 1024, 33000])
+def test_bad_values_stay_in_their_row(c):
+    x, gamma, beta, dy = _inputs(6, c, seed=3)
+    clean = _forward(x, gamma, beta)
+    x[1, c // 2], x[4, 0] = np.nan, np.inf
+    got = _forward(x, gamma, beta)
+    keep = [0, 2, 3, 5]
+    assert np.array_equal(got[0][keep], clean[0][keep])
+    assert np.all(np.isnan(got[0][[1, 4]]))
+    dx, dg, db, _ = _backward(x, dy, gamma, got[1], got[2])
+    x0, _, _, _ = _inputs(6, c, seed=3)
+    want = _backward(x0, dy, gamma, clean[1], clean[2])
+    assert np.array_equal(dx[keep], want[0][keep]) and np.all(np.isnan(dx[[1, 4]]))
+    assert np.all(np.isnan(dg)) and np.array_equal(db, want[2])
+
+
+def test_no_rows():
+    x, gamma, beta, _ = _inputs(1, 12)
+    empty = np.zeros((0, 12), np.float32)
+    assert _forward(empty, gamma, beta)[0].shape == (0, 12)
+    _, dg, db, _ = _backward(empty, empty, gamma, np.zeros(0, np.float32), np.zeros(0, np.float32))
+    assert np.all(dg == 0) and np.all(db == 0)
+
+
+@pytest.mark.parametrize("rows,c", [(3, 5), (2, 70)])
+def test_gradients_against_differences(rows, c):
+    """Central differences of sum(dy * y) in 64 bits of the float64 formula, at the point the kernel was given."""
+    x, gamma, beta, dy = _inputs(rows, c, seed=4)
+    fwd = _forward(x, gamma, beta)
+    dx, dg, db, _ = _backward(x, dy, gamma, fwd[1], fwd[2])
+    f = lambda a, g, b: float((R.forward_value(a, g, b, 1e-5) * dy).sum())  # noqa: E731
+    h = 1e-5
+
+    def slope(which):
+        base = [np.asarray(a, np.float64) for a in (x, gamma, beta)]
+        out = np.zeros(base[which].shape)
+        for i in np.ndindex(out.shape):
+            lo, hi = [a.copy() for a in base], [a.copy() for a in base]
+            lo[which][i] -= h
+            hi[which][i] += h
+            out[i] = (f(*hi) - f(*lo)) / (2 * h)
+        return out
+
+    # differences: h^2 / 6 times the third derivative (of order 10 here: invstd up to 2) and rounding 1e-16 / h: below 1e-8;
+    # the kernel: a few hundred roundings of 2^-24 of terms of order 10
+    for got, which in ((dx, 0), (dg, 1), (db, 2)):
+        assert np.allclose(got, slope(which), rtol=1e-4, atol=1e-4)
+
+
+def test_layer_class():
+    import aether
+    r = np.random.RandomState(5)
+    layer = aether.Layer_Norm()
+    assert layer.weights is None and layer.epsilon == 1e-5
+    x = r.randn(2, 3, 4, 20).astype(np.float32)
+    dy = r.randn(2, 3, 4, 20).astype(np.float32)
+    out = layer.forward(x, training=True)
+    assert out is layer.output and out.shape == x.shape
+    assert layer.weights is layer.gamma and layer.biases is layer.beta and layer.gamma.shape == (20,)
+    gamma, beta = r.randn(20).astype(np.float32), r.randn(20).astype(np.float32)
+    layer.set_parameters(gamma, beta.reshape(1, 20))
+    assert layer.weights is layer.gamma and np.array_equal(layer.get_parameters()[1].get(), beta)
+    y = layer.forward(x, training=True).get()
+    (want, mean, inv), (e_y, _, _) = R.forward(x, gamma, beta, 1e-5)
+    assert R.worst(y, want, e_y) <= 1
+    assert layer.backward(dy) is layer.dinputs and layer.dinputs.shape == x.shape
+    want, bounds = R.backward(x, dy, gamma, layer.row_mean.get(), layer.row_invstd.get())
+    for got, w, b in zip((layer.dinputs, layer.dweights, layer.dbiases), want, bounds):
+        assert R.worst(got.get(), w, b) <= 1
+    assert np.array_equal(layer.forward(x, training=False).get(), y)
+    with pytest.raises(ValueError, match="training=True"):
+        layer.backward(dy)
+    layer.forward(x, training=True)
+    with pytest.raises(ValueError, match="gradient shape"):
+        layer.backward(dy[:1])
+    with pytest.raises(ValueError, match="features"):
+        layer.forward(x[..., :19], training=True)
+    with pytest.raises(ValueError, match="rows"):
+        layer.forward(x[0, 0, 0], training=True)
+    assert aether.Layer_Norm(n_features=7).gamma.shape == (7,)
+
+
+def test_twin_for_a_bf16_convolution_and_behind_one():
+    """Between two bf16 convolutions the norm leaves the bfloat16 copies they take (output forward, input gradient
+    backward)."""
+    import aether
+    r = np.random.RandomState(6)
+    first, last = aether.Conv_Layer((6, 6, 8), num_filters=8), aether.Conv_Layer((6, 6, 8), num_filters=8)
+    norm = aether.Layer_Norm()
+    norm.prev, norm.next = first, last
+    x, dy = r.randn(2, 6, 6, 8).astype(np.float32), r.randn(2, 6, 6, 8).astype(np.float32)
+    norm.forward(x, True)
+    norm.backward(dy)
+    assert norm.output._bf16 is None and norm.dinputs._bf16 is None
+    first.precision = last.precision = "bf16"
+    out = norm.forward(x, True)
+    norm.backward(dy)
+    assert np.array_equal(out._bf16.get(), O.bf16_bits(out.get()))
+    assert np.array_equal(norm.dinputs._bf16.get(), O.bf16_bits(norm.dinputs.get()))
+
+
+def test_recorded_and_replayed():
+    """Forward and backward pass in a recording: every replay, with eager work of the same layer kind (and a larger
+    workspace) between, equals the eager result bit for bit."""
+    import aether
+    lib, check = _lib()
+    r = np.random.RandomState(7)
+    rows, c = 300, 130
+    gamma, beta = r.randn(c).astype(np.float32), r.randn(c).astype(np.float32)
+    layer, other = aether.Layer_Norm(), aether.Layer_Norm()
+    layer.set_parameters(gamma, beta)
+    batches = [(r.randn(rows, c).astype(np.float32), r.randn(rows, c).astype(np.float32)) for _ in range(4)]
+    want = []
+    for x, dy in batches:
+        layer.forward(x, True)
+        layer.backward(dy)
+        want.append([t.get() for t in (layer.output, layer.dinputs, layer.dweights, layer.dbiases)])
+    xin, dyin = _dev(batches[0][0]), _dev(batches[0][1])
+    check(lib.aeth_graph_begin())
+    layer.forward(xin, True)
+    layer.backward(dyin)
+    graph = C.c_void_p()
+    check(lib.aeth_graph_end(C.byref(graph)))
+    outs = (layer.output, layer.dinputs, layer.dweights, layer.dbiases)
+    for k, (x, dy) in enumerate(batches):
+        xin.set(x)
+        dyin.set(dy)
+        check(lib.aeth_graph_launch(graph))
+        for t, w in zip(outs, want[k]):
+            assert np.array_equal(t.get(), w)
+        other.forward(r.randn(900 * (k + 1), 700).astype(np.float32), True)
+        other.backward(r.randn(900 * (k + 1), 700).astype(np.float32))
+    check(lib.aeth_graph_destroy(graph))
