@@ -82,6 +82,9 @@ SIGNATURES = {
     "aeth_adam_multi_f32": [_i, _p, _p, _p, _p, _p, _f, _f, _f, _f, _i],
     "aeth_adam_state_step": [_p, _d, _d, _d, _d],
     "aeth_adam_multi_dev_f32": [_i, _p, _p, _p, _p, _p, _f, _f, _f, _p],
+    "aeth_newton_schulz_f32": [_p, _p, _i, _i, _i],
+    "aeth_muon_multi_f32": [_i, _p, _p, _p, _p, _p, _f, _f, _i, _f, _i],
+    "aeth_muon_multi_dev_f32": [_i, _p, _p, _p, _p, _p, _f, _i, _f, _i, _p],
     "aeth_graph_begin": [],
     "aeth_graph_end": [C.POINTER(_p)],
     "aeth_graph_launch": [_p],

@@ -933,10 +933,17 @@ class Optimizer_Adam:
             layer.bias_cache = DeviceTensor.zeros(layer.biases.shape)
         # The updates of all layers of a step go out as one launch: they are queued
         # here and issued by post_update_parameters (or when 32 tensors are waiting).
-        self._pending.append((layer.weights, layer.dweights, layer.weight_momentums, layer.weight_cache))
-        self._pending.append((layer.biases, layer.dbiases, layer.bias_momentums, layer.bias_cache))
+        self._queue((layer.weights, layer.dweights, layer.weight_momentums, layer.weight_cache),
+                    (layer.biases, layer.dbiases, layer.bias_momentums, layer.bias_cache))
+
+    def _queue(self, *tensors):
+        self._pending.extend(tensors)
         if len(self._pending) >= 32:
             self._flush()
+
+    def has_state(self, layer):
+        """Whether an update of this layer has created its moments."""
+        return hasattr(layer, "weight_cache")
 
     def _flush(self):
         import ctypes as C
@@ -974,15 +981,18 @@ class Optimizer_Adam:
     def record_update(self, layers):
         """Queue one whole optimizer step (pre_update, every layer, post_update) in a form
         that can be replayed: learning rate and bias corrections come from device_state()."""
-        import ctypes as C
-        state = self._state
-        self._recorded_params = [t for layer in layers for t in (layer.weights, layer.biases)]
-        b1, b2 = float(np.float32(self.beta_1)), float(np.float32(self.beta_2))
-        _ck(_L().aeth_adam_state_step(state.ptr, float(self.learning_rate), float(self.decay), b1, b2))
         batch = []
         for layer in layers:
             batch.append((layer.weights, layer.dweights, layer.weight_momentums, layer.weight_cache))
             batch.append((layer.biases, layer.dbiases, layer.bias_momentums, layer.bias_cache))
+        self._record_tensors(batch)
+
+    def _record_tensors(self, batch):
+        import ctypes as C
+        state = self._state
+        self._recorded_params = [t[0] for t in batch]
+        b1, b2 = float(np.float32(self.beta_1)), float(np.float32(self.beta_2))
+        _ck(_L().aeth_adam_state_step(state.ptr, float(self.learning_rate), float(self.decay), b1, b2))
         while batch:
             part, batch = batch[:32], batch[32:]
             n = len(part)
@@ -999,3 +1009,134 @@ class Optimizer_Adam:
         self._state_iterations = self.iterations
         for t in getattr(self, "_recorded_params", ()):
             t.touched()
+
+
+# ----------------------------------------------------------------------------------
+# Optimizer_Muon  (no counterpart in the reference; driven by Model as Optimizer_Adam is)
+# ----------------------------------------------------------------------------------
+class Optimizer_Muon:
+    """Weight matrices (dense weights; filters as [fH fW C, D]) move along their momentum with all singular values set to
+    about one (Newton-Schulz products), everything else by Adam: biases, the vectors of the norm layers, the dense layer in
+    front of SoftMax (a classifier head has few, very different columns), and layers whose ``muon`` attribute is False
+    (True takes a head in).  ``learning_rate`` is the matrices', ``adam_learning_rate`` the others'; ``decay`` lowers both.
+
+        m <- momentum m + g;  O = newton_schulz(g + momentum m, or m without nesterov)
+        w <- w (1 - lr weight_decay) - lr sqrt(max(1, n_out / n_in)) O
+    """
+
+    def __init__(self, learning_rate=.02, decay=0., momentum=.95, nesterov=True, ns_steps=5, weight_decay=0.,
+                 adam_learning_rate=.001, epsilon=1e-7, beta_1=0.9, beta_2=.999):
+        if not 0 <= momentum < 1:
+            raise ValueError(f"Expected 0 <= momentum < 1, got {momentum}.")
+        if not 1 <= ns_steps <= 100:
+            raise ValueError(f"Expected 1 to 100 Newton-Schulz steps, got {ns_steps}.")
+        if not weight_decay >= 0:
+            raise ValueError(f"Expected weight_decay >= 0, got {weight_decay}.")
+        self.learning_rate = learning_rate
+        self.current_learning_rate = learning_rate
+        self.decay = decay
+        self.iterations = 0
+        self.momentum = momentum
+        self.nesterov = nesterov
+        self.ns_steps = ns_steps
+        self.weight_decay = weight_decay
+        self.adam = Optimizer_Adam(adam_learning_rate, decay, epsilon, beta_1, beta_2)
+        self._pending = []
+
+    @staticmethod
+    def takes(layer):
+        """Whether the layer's weights are updated as a matrix."""
+        shape = layer.weights.shape
+        wanted = getattr(layer, "muon", None)
+        if wanted is None:
+            wanted = not isinstance(getattr(layer, "next", None), SoftMax)
+        return bool(wanted) and len(shape) >= 2 and shape[-1] > 1 and layer.weights.size > shape[-1]
+
+    def pre_update_parameters(self):
+        if self.decay:
+            self.current_learning_rate = self.learning_rate * (1. / (1. + self.decay * self.iterations))
+        self.adam.pre_update_parameters()
+
+    def update_parameters(self, layer):
+        if not self.takes(layer):
+            self.adam.update_parameters(layer)
+            return
+        if not hasattr(layer, "muon_momentums"):
+            layer.muon_momentums = DeviceTensor.zeros(layer.weights.shape)
+        if not hasattr(layer, "bias_cache"):
+            layer.bias_momentums = DeviceTensor.zeros(layer.biases.shape)
+            layer.bias_cache = DeviceTensor.zeros(layer.biases.shape)
+        # as Adam's: the updates of a step wait for post_update_parameters and go out together
+        self._pending.append((layer.weights, layer.dweights, layer.muon_momentums))
+        self.adam._queue((layer.biases, layer.dbiases, layer.bias_momentums, layer.bias_cache))
+        if len(self._pending) >= 32:
+            self._flush()
+
+    def has_state(self, layer):
+        if layer.weights is None or not self.takes(layer):
+            return self.adam.has_state(layer)
+        return hasattr(layer, "muon_momentums") and hasattr(layer, "bias_cache")
+
+    def _matrices(self, batch):
+        """The host arrays of one call: pointers of weights, gradients, momentums; rows; columns."""
+        import ctypes as C
+        for w, g, m in batch:
+            if g.size != w.size or m.size != w.size:
+                raise ValueError("gradient shape %s does not match parameter shape %s" % (g.shape, w.shape))
+        n = len(batch)
+        pointers = [(C.c_void_p * n)(*[t[k].ptr for t in batch]) for k in range(3)]
+        cols = [t[0].shape[-1] for t in batch]
+        rows = [t[0].size // c for t, c in zip(batch, cols)]
+        return [n] + pointers + [(C.c_int * n)(*rows), (C.c_int * n)(*cols)]
+
+    def _flush(self):
+        while self._pending:
+            batch, self._pending = self._pending[:32], self._pending[32:]
+            _ck(_L().aeth_muon_multi_f32(*self._matrices(batch), self.current_learning_rate, self.momentum,
+                                         int(bool(self.nesterov)), self.weight_decay, self.ns_steps))
+            for t in batch:
+                t[0].touched()                               # the parameters changed in place
+
+    def post_update_parameters(self):
+        self._flush()
+        self.adam.post_update_parameters()
+        self.iterations += 1
+
+    # -- recorded steps: step number and learning rates live on the device ----------------
+    def device_state(self):
+        """Adam's state, and for the matrices {iterations, -, -, lr} in the same form."""
+        self.adam.device_state()
+        if getattr(self, "_state", None) is None:
+            self._state = DeviceTensor(4, np.float64)
+            self._state_iterations = None
+        if self._state_iterations != self.iterations:
+            self._state.set(np.array([self.iterations, 1, 1, self.current_learning_rate], dtype=np.float64))
+            self._state_iterations = self.iterations
+        return self._state
+
+    def record_update(self, layers):
+        """Queue one whole optimizer step in a form that can be replayed (see Optimizer_Adam.record_update)."""
+        matrices, others = [], []
+        for layer in layers:
+            if self.takes(layer):
+                matrices.append((layer.weights, layer.dweights, layer.muon_momentums))
+            else:
+                others.append((layer.weights, layer.dweights, layer.weight_momentums, layer.weight_cache))
+            others.append((layer.biases, layer.dbiases, layer.bias_momentums, layer.bias_cache))
+        self._recorded_params = [t[0] for t in matrices]
+        _ck(_L().aeth_adam_state_step(self._state.ptr, float(self.learning_rate), float(self.decay), 1.0, 1.0))
+        while matrices:
+            part, matrices = matrices[:32], matrices[32:]
+            _ck(_L().aeth_muon_multi_dev_f32(*self._matrices(part), self.momentum, int(bool(self.nesterov)),
+                                             self.weight_decay, self.ns_steps, self._state.ptr))
+        self.adam._record_tensors(others)
+
+    def replayed(self):
+        """Host bookkeeping after a recorded step has run once more."""
+        if self.decay:
+            self.current_learning_rate = self.learning_rate * (1. / (1. + self.decay * self.iterations))
+        self.iterations += 1
+        self._state_iterations = self.iterations
+        for t in getattr(self, "_recorded_params", ()):
+            t.touched()
+        self.adam.replayed()

@@ -197,13 +197,13 @@ class Model:
         the layers' order from the reference's random stream, and copied into the buffers
         the recorded kernels read before every replay.  Regularisers are recorded: their
         sums and their gradient terms are kernels like the rest.  Falls back to normal
-        steps for models the recording cannot express (anything but Adam with the fused
-        softmax / cross-entropy output)."""
+        steps for models the recording cannot express (anything but Adam or Muon with the
+        fused softmax / cross-entropy output)."""
         self._record = bool(enabled)
         if not enabled:
             self._drop_recordings()
         elif not self._can_record():
-            warnings.warn("record_steps: this model cannot be recorded (no Adam / fused softmax cross-entropy); "
+            warnings.warn("record_steps: this model cannot be recorded (no Adam or Muon / fused softmax cross-entropy); "
                           "steps run eagerly", RuntimeWarning, stacklevel=2)
 
     @property
@@ -219,8 +219,8 @@ class Model:
         self._recordings = {}
 
     def _can_record(self):
-        from .layers import Optimizer_Adam
-        if self.softmax_classifier_output is None or not isinstance(self.optimizer, Optimizer_Adam):
+        from .layers import Optimizer_Adam, Optimizer_Muon
+        if self.softmax_classifier_output is None or not isinstance(self.optimizer, (Optimizer_Adam, Optimizer_Muon)):
             return False
         return self.loss.can_defer()
 
@@ -234,16 +234,18 @@ class Model:
         key = (tuple(batch_X.shape), kind, labels.shape)
         recs = self.__dict__.setdefault("_recordings", {})
         rec = recs.get(key)
-        if rec is None or not all(hasattr(l, "weight_cache") for l in self.trainable_layers):
-            # first step of this shape, or no Adam state yet: a normal one (lazy initialisations,
+        lib = _lib.lib()
+        if rec is None or not all(self.optimizer.has_state(l) for l in self.trainable_layers):
+            # first step of this shape, or no optimizer state yet: a normal one (lazy initialisations,
             # workspace sizes)
+            if rec is not None and rec["graph"] is not None:
+                _lib.check(lib.aeth_graph_destroy(rec["graph"]))
             recs[key] = {"graph": None}
             return None
-        lib = _lib.lib()
-        # a recording reads and writes the parameter buffers it was made with: parameters set
-        # anew since then (set_parameters, load_parameters) make it stale
+        # a recording holds the optimizer's update and reads and writes the parameter buffers it was made with:
+        # another optimizer, or parameters set anew since then (set_parameters, load_parameters), make it stale
         params = [(id(l), l.weights.ptr, l.biases.ptr) for l in self.trainable_layers]
-        if rec["graph"] is not None and rec.get("params") != params:
+        if rec["graph"] is not None and (rec.get("params") != params or rec.get("optimizer") is not self.optimizer):
             _lib.check(lib.aeth_graph_destroy(rec["graph"]))
             recs[key] = rec = {"graph": None}
         if rec["graph"] is None:
@@ -270,6 +272,7 @@ class Model:
             _lib.check(rc)
             rec["graph"] = handle
             rec["params"] = params
+            rec["optimizer"] = self.optimizer
             # what the layers point at after this step (output, dinputs, dweights, ...):
             # replays fill the same buffers, so the attributes are put back after steps
             # that ran in between (an evaluation, a step of another shape)

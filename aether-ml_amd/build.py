@@ -15,7 +15,7 @@ OBJ = os.path.join(HERE, "build")
 LIBDIR = os.path.join(HERE, "aether", "lib")
 LIB = os.path.join(LIBDIR, "libaether_hip.so")
 SOURCES = ["runtime.hip", "gather_f32.hip", "gather_bf16.hip", "gather_res9_bf16.hip", "wgrad_f32.hip", "wgrad_bf16.hip", "pair_f32.hip",
-           "layers.hip", "norm.hip"]
+           "layers.hip", "norm.hip", "muon.hip"]
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 FLAGS = [
     "-O3", "--offload-arch=gfx950", "-fPIC", "-std=c++17",

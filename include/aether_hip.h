@@ -335,6 +335,26 @@ int aeth_adam_multi_dev_f32(int count, float* const* host_theta, const float* co
                             float* const* host_m, float* const* host_v, const int64_t* host_n,
                             float beta1, float beta2, float eps, const double* state);
 
+/* The Muon update (no counterpart in the reference): a step along the momentum's singular vectors, for weight matrices.
+ * aeth_newton_schulz_f32 is its orthogonalisation alone: o = X after `steps` (1..100) rounds of
+ *     X = g / |g| (Frobenius);  X <- a X + (b A + c A^2) X,  A = X X^T   (a, b, c) = (3.4445, -4.7750, 2.0315),
+ * which takes every singular value s of g / |g| to p(...p(s)), p(s) = a s + b s^3 + c s^5, and keeps the singular vectors.
+ * Any positive multiple of g gives the same o (there is no epsilon); g = 0 gives 0; a NaN or an infinity makes all of o NaN.
+ * g and o are [rows, cols] and may not overlap; products and sums hold 22 bits or more of every factor.
+ * aeth_muon_multi_f32 updates `count` (1..32) matrices in one call:
+ *     m <- momentum m + grad;  u = grad + momentum m (nesterov != 0) or m;  O = newton_schulz(u);
+ *     theta <- theta (1 - lr weight_decay) - lr sqrt(max(1, cols / rows)) O.
+ * A filter [fH,fW,C,D] is the matrix [fH fW C, D].  The five host_ arrays have `count` entries (device pointers; ints);
+ * empty matrices are skipped, tensors that overlap (a matrix given twice) are refused.  aeth_muon_multi_dev_f32 reads the
+ * learning rate from state[3] of a step state (aeth_adam_state_step above), for recorded steps; same bits. */
+int aeth_newton_schulz_f32(const float* g, float* o, int rows, int cols, int steps);
+int aeth_muon_multi_f32(int count, float* const* host_theta, const float* const* host_grad, float* const* host_m,
+                        const int* host_rows, const int* host_cols,
+                        float lr, float momentum, int nesterov, float weight_decay, int steps);
+int aeth_muon_multi_dev_f32(int count, float* const* host_theta, const float* const* host_grad, float* const* host_m,
+                            const int* host_rows, const int* host_cols,
+                            float momentum, int nesterov, float weight_decay, int steps, const double* state);
+
 /* ---- recorded steps -------------------------------------------------------------------
  * No counterpart in the reference (CuPy launches every kernel from Python each step).
  * Between aeth_graph_begin and aeth_graph_end the library's stream records instead of

@@ -1,0 +1,392 @@
+"""The orthogonalisation, the Muon update and Optimizer_Muon against the formulas in 64 bits (tests/muon_reference.py says
+where the tolerances come from)."""
+import ctypes as C
+
+import numpy as np
+import pytest
+
+from tests import muon_reference as R
+
+pytestmark = pytest.mark.gpu
+
+
+def _lib():
+    from aether import _lib
+    return _lib.lib(), _lib.check
+
+
+def _dev(a):
+    from aether import DeviceTensor
+    return DeviceTensor.from_numpy(a, np.float32)
+
+
+def _ortho(g, steps=5):
+    from aether import DeviceTensor
+    lib, check = _lib()
+    gd, o = _dev(g), DeviceTensor.full(g.shape, np.nan)
+    check(lib.aeth_newton_schulz_f32(gd.ptr, o.ptr, g.shape[0], g.shape[1], steps))
+    return o.get()
+
+
+def _gradient(r, c, seed=0, strong=8):
+    rng = np.random.RandomState(seed + 31 * r + c)
+    k = max(1, min(r, c, strong))
+    low = (rng.randn(r, k) * 2.0 ** (-np.arange(k) / 2.0)) @ rng.randn(k, c)
+    return ((low + rng.randn(r, c)) * 1e-3).astype(np.float32)
+
+
+def _check(g, steps=5, o=None):
+    tol, exact = R.tolerance(g, steps)
+    o = _ortho(g, steps) if o is None else o
+    assert np.all(np.isfinite(o)), "non-finite values (unwritten output?)"
+    off = np.linalg.norm(o - exact)
+    assert off <= tol, "off by %.3g, allowed %.3g (norm %.3g)" % (off, tol, np.linalg.norm(exact))
+
+
+# single rows and columns, both orientations, one less and one more than the tiles and slabs, long thin matrices
+SHAPES = [(1, 1), (1, 7), (9, 1), (2, 2), (2, 3), (5, 4), (15, 17), (16, 16), (27, 32), (31, 33), (32, 32), (33, 31), (48, 20),
+          (63, 65), (64, 64), (64, 576), (576, 64), (65, 64), (10, 300), (300, 10), (96, 96), (100, 1000), (127, 129),
+          (128, 128), (128, 576), (129, 128), (130, 1030), (160, 161), (191, 193), (192, 192), (255, 257), (256, 256),
+          (256, 2048), (2048, 256), (257, 400), (320, 500), (1, 5000), (3, 4097), (4500, 33), (384, 384), (500, 640), (513, 700),
+          (640, 512), (1000, 150), (1024, 512), (1025, 1030), (1300, 1100)]
+
+
+@pytest.mark.parametrize("r,c", SHAPES)
+def test_orthogonalisation(r, c):
+    g = _gradient(r, c)
+    o = _ortho(g)
+    _check(g, o=o)
+    assert np.array_equal(_ortho(g), o)                    # the same bits again
+
+
+@pytest.mark.parametrize("steps", [1, 2, 3, 7, 12])
+def test_steps(steps):
+    for r, c in ((40, 70), (150, 90), (300, 260)):
+        _check(_gradient(r, c, seed=1), steps)
+
+
+@pytest.mark.parametrize("r,c", [(24, 40), (130, 70), (200, 300)])
+def test_transposes_and_multiples(r, c):
+    """The transposed matrix gives the transposed result; a power of two in front changes no bit, other multiples, up to the
+    ends of float32, only the roundings."""
+    g = _gradient(r, c, seed=2)
+    o = _ortho(g)
+    tol, _ = R.tolerance(g)
+    assert np.linalg.norm(_ortho(np.ascontiguousarray(g.T)).T - o) <= 2 * tol
+    for k in (-60, -3, 5, 90):
+        assert np.array_equal(_ortho(g * np.float32(2.0) ** k), o)
+    for f in (3e30, 1e-30):
+        assert np.linalg.norm(_ortho(g * np.float32(f)) - o) <= 2 * tol
+    tiny = (g * np.float32(1e-38)).astype(np.float32)      # denormal numbers: few bits, but a direction
+    _check(tiny)
+
+
+@pytest.mark.parametrize("r,c", [(1, 4), (30, 50), (150, 90), (300, 300)])
+def test_zero_and_deficient_matrices(r, c):
+    assert np.all(_ortho(np.zeros((r, c), np.float32)) == 0)
+    rng = np.random.RandomState(r)
+    one = (rng.randn(r, 1) @ rng.randn(1, c)).astype(np.float32)       # rank 1 up to float32
+    tol, exact = R.tolerance(one)
+    assert np.linalg.norm(_ortho(one) - exact) <= tol
+    g = _gradient(r, c, seed=3)
+    g[r // 2] = 0
+    g[:, c // 3] = 0
+    o = _ortho(g)
+    _check(g, o=o)
+    assert np.all(o[r // 2] == 0) and np.all(o[:, c // 3] == 0)         # products with zeros only
+    single = np.zeros((r, c), np.float32)
+    single[r - 1, c - 1] = -7.5
+    _check(single)
+    q = np.linalg.qr(rng.randn(max(r, c), min(r, c)))[0].astype(np.float32)
+    _check(q if r >= c else np.ascontiguousarray(q.T))
+
+
+@pytest.mark.parametrize("r,c", [(4, 6), (150, 90), (300, 300)])
+@pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf])
+def test_bad_values(r, c, bad):
+    g = _gradient(r, c, seed=4)
+    g[r - 1, 1] = bad
+    assert np.all(np.isnan(_ortho(g)))
+
+
+def test_views_that_are_only_four_byte_aligned():
+    from aether import DeviceTensor
+    lib, check = _lib()
+    for r, c in ((33, 47), (64, 64), (300, 130)):
+        g = _gradient(r, c, seed=5)
+        whole, out = np.full(r * c + 8, 5.0, np.float32), DeviceTensor.full(r * c + 8, 5.0)
+        whole[3:3 + r * c] = g.reshape(-1)
+        gd = _dev(whole)
+        check(lib.aeth_newton_schulz_f32(gd.ptr + 12, out.ptr + 12, r, c, 5))
+        o = out.get()
+        assert np.all(o[:3] == 5) and np.all(o[3 + r * c:] == 5)
+        _check(g, o=o[3:3 + r * c].reshape(r, c))
+
+
+def _multi(tensors, lr=0.02, momentum=0.95, nesterov=1, wd=0.01, steps=5, state=None):
+    """One call on [(theta, grad, mom)]; host copies of (theta, mom) afterwards."""
+    lib, check = _lib()
+    n = len(tensors)
+    dev = [[_dev(a) for a in t] for t in tensors]
+    table = [(C.c_void_p * n)(*[d[k].ptr for d in dev]) for k in range(3)]
+    sizes = [(C.c_int * n)(*[t[0].shape[k] for t in tensors]) for k in range(2)]
+    if state is None:
+        check(lib.aeth_muon_multi_f32(n, *table, *sizes, lr, momentum, nesterov, wd, steps))
+    else:
+        check(lib.aeth_muon_multi_dev_f32(n, *table, *sizes, momentum, nesterov, wd, steps, state.ptr))
+    for t, d in zip(tensors, dev):
+        assert np.array_equal(d[1].get(), t[1])            # the gradients stay
+    return [(d[0].get(), d[2].get()) for d in dev]
+
+
+def _triple(r, c, seed=0):
+    rng = np.random.RandomState(seed + r + 7 * c)
+    return (0.01 * rng.randn(r, c)).astype(np.float32), _gradient(r, c, seed + 1), 3 * _gradient(r, c, seed + 2)
+
+
+CNN3 = [(27, 32), (288, 64), (576, 128), (2048, 256)]
+
+
+@pytest.mark.parametrize("shapes", [[(1, 1)], [(64, 64)], [(256, 10)], [(10, 256)], [(300, 500)], [(1100, 600)], CNN3,
+                                    [(64, 64), (64, 64), (64, 64)], [(5, 9), (700, 700), (1, 3), (130, 64), (64, 130)],
+                                    [(20 + 3 * i, 90 - 2 * i) for i in range(32)]])
+@pytest.mark.parametrize("nesterov", [0, 1])
+def test_update(shapes, nesterov):
+    tensors = [_triple(r, c, seed=10 * i) for i, (r, c) in enumerate(shapes)]
+    got = _multi(tensors, nesterov=nesterov)
+    alone = [_multi([t], nesterov=nesterov)[0] for t in tensors]
+    for t, g, a in zip(tensors, got, alone):
+        want, m, bound = R.update(*t, 0.02, 0.95, nesterov, 0.01)
+        assert np.all(np.abs(g[1] - m) <= R.momentum_bound(t[1], t[2], 0.95))
+        assert np.linalg.norm(g[0] - want) <= bound
+        # a matrix does not depend on what else is in the call beyond the tolerance of its sums
+        assert np.linalg.norm(a[0] - g[0]) <= 2 * bound and np.array_equal(a[1], g[1])
+    again = _multi(tensors, nesterov=nesterov)
+    assert all(np.array_equal(p[0], q[0]) and np.array_equal(p[1], q[1]) for p, q in zip(got, again))
+
+
+def test_update_without_momentum_decay_or_gradient():
+    theta, grad, mom = _triple(40, 60)
+    zero = np.zeros_like(grad)
+    (t, m), = _multi([(theta, zero, zero)], wd=0.5, lr=0.1)
+    keep = np.float32(1) - np.float32(0.1) * np.float32(0.5)
+    assert np.allclose(t, theta * keep, rtol=2.0 ** -22, atol=0) and np.all(m == 0)
+    (t, m), = _multi([(theta, grad, mom)], momentum=0.0, wd=0.0)
+    want, _, bound = R.update(theta, grad, mom, 0.02, 0.0, 1, 0.0)
+    assert np.array_equal(m, grad) and np.linalg.norm(t - want) <= bound
+    (t, m), = _multi([(theta, grad, mom)], lr=0.0)
+    assert np.array_equal(t, theta)
+
+
+def test_learning_rate_on_the_device():
+    from aether import DeviceTensor
+    tensors = [_triple(48, 30), _triple(300, 200)]
+    state = DeviceTensor.from_numpy(np.array([3.0, 1.0, 1.0, 0.0137]), np.float64)
+    a, b = _multi(tensors, lr=0.0137), _multi(tensors, state=state)
+    assert all(np.array_equal(p[0], q[0]) and np.array_equal(p[1], q[1]) for p, q in zip(a, b))
+
+
+def test_empty_matrices_are_skipped():
+    tensors = [_triple(20, 30)]
+    lib, check = _lib()
+    dev = [_dev(a) for a in tensors[0]]
+    table = [(C.c_void_p * 2)(None, d.ptr) for d in dev]
+    check(lib.aeth_muon_multi_f32(2, *table, (C.c_int * 2)(0, 20), (C.c_int * 2)(5, 30), 0.02, 0.95, 1, 0.01, 5))
+    want = _multi(tensors)[0]
+    assert np.array_equal(dev[0].get(), want[0]) and np.array_equal(dev[2].get(), want[1])
+    check(lib.aeth_newton_schulz_f32(None, None, 0, 12, 5))
+    check(lib.aeth_newton_schulz_f32(None, None, 12, 0, 5))
+
+
+def test_recorded_and_replayed():
+    """An update in a recording, replayed with eager updates of larger matrices (which replace the workspace) between: every
+    replay equals the eager step from the same state bit for bit."""
+    lib, check = _lib()
+    tensors = [_triple(96, 130), _triple(40, 20)]
+    _multi(tensors)
+    dev = [[_dev(a) for a in t] for t in tensors]
+    table = [(C.c_void_p * 2)(*[d[k].ptr for d in dev]) for k in range(3)]
+    sizes = [(C.c_int * 2)(*[t[0].shape[k] for t in tensors]) for k in range(2)]
+    check(lib.aeth_graph_begin())
+    check(lib.aeth_muon_multi_f32(2, *table, *sizes, 0.02, 0.95, 1, 0.01, 5))
+    graph = C.c_void_p()
+    check(lib.aeth_graph_end(C.byref(graph)))
+    state = tensors
+    for k in range(4):
+        check(lib.aeth_graph_launch(graph))
+        after = [(d[0].get(), d[2].get()) for d in dev]
+        want = _multi(state)
+        assert all(np.array_equal(a[0], w[0]) and np.array_equal(a[1], w[1]) for a, w in zip(after, want))
+        grads = [_gradient(*t[0].shape, seed=50 + k) for t in tensors]
+        for d, g in zip(dev, grads):
+            d[1].set(g)
+        state = [(a[0], g, a[1]) for a, g in zip(after, grads)]
+        _multi([_triple(300 * (k + 1), 250)])
+    check(lib.aeth_graph_destroy(graph))
+
+
+# ---- the optimizer ---------------------------------------------------------------------------------------------------
+def _network(optimizer, seed=0, norm=True):
+    import aether
+    np.random.seed(seed)
+    model = aether.Model()
+    model.add(aether.Conv_Layer((8, 8, 3), num_filters=16))
+    if norm:
+        model.add(aether.Layer_Norm())
+    model.add(aether.ReLU())
+    model.add(aether.Pooling())
+    model.add(aether.Flatten())
+    model.add(aether.Layer_Dense(256, 48, weight_regularizer_l2=1e-4))
+    if norm:
+        model.add(aether.Layer_Norm())
+    model.add(aether.Leaky_ReLU())
+    model.add(aether.Layer_Dense(48, 10))
+    model.add(aether.SoftMax())
+    model.set(loss=aether.Loss_CategoricalCrossEntropy(label_smoothing=0.01), optimizer=optimizer,
+              accuracy=aether.Accuracy_Categorical())
+    model.finalize()
+    model.loss.new_pass()
+    model.accuracy.new_pass()
+    return model
+
+
+def _batches(n, rows=16, seed=1):
+    r = np.random.RandomState(seed)
+    return [(r.randn(rows, 8, 8, 3).astype(np.float32), r.randint(0, 10, rows)) for _ in range(n)]
+
+
+def _host(model):
+    return [np.asarray(a) for layer in model.trainable_layers for a in layer.get_parameters()]
+
+
+def test_optimizer_steps_follow_the_formulas():
+    """Layer norms, a convolution and dense layers under Muon: after every step matrices are where the formula puts them from
+    the state and gradients before it; biases, gains and the classifier head where Adam's does."""
+    import aether
+    from tests import step_checks
+    opt = aether.Optimizer_Muon(learning_rate=0.05, decay=0.1, weight_decay=0.02, adam_learning_rate=2e-3)
+    model = _network(opt)
+    conv, norm1, dense, norm2, head = model.trainable_layers
+    for it, (x, y) in enumerate(_batches(4)):
+        before = {}
+        for l in model.trainable_layers:
+            if l.weights is not None:
+                before[id(l)] = (l.weights.get(), l.muon_momentums.get() if hasattr(l, "muon_momentums") else None)
+        model.train_step(x, y)
+        lr, lr_adam = 0.05 / (1 + 0.1 * it), 2e-3 / (1 + 0.1 * it)
+        assert opt.iterations == opt.adam.iterations == it + 1 and np.isclose(opt.current_learning_rate, lr)
+        assert [opt.takes(l) for l in model.trainable_layers] == [True, False, True, False, False]
+        for l in (conv, dense):
+            w0, m0 = before[id(l)]
+            shape = (-1, w0.shape[-1])
+            w0, g = w0.reshape(shape), l.dweights.get().reshape(shape)
+            m0 = np.zeros_like(w0) if m0 is None else m0.reshape(shape)
+            want, m, bound = R.update(w0, g, m0, lr, 0.95, True, 0.02)
+            assert np.all(np.abs(l.muon_momentums.get().reshape(shape) - m) <= R.momentum_bound(g, m0, 0.95))
+            assert np.linalg.norm(l.weights.get().reshape(shape) - want) <= bound
+            assert not hasattr(l, "weight_cache")
+        if it == 0:
+            head0 = before[id(head)][0]
+            e = step_checks.update_errors(head0, head.dweights.get(), 0 * head0, 0 * head0, head.weights.get(),
+                                          head.weight_momentums.get(), head.weight_cache.get(), lr_adam, 0)
+            assert max(e) <= 1
+            for l in (conv, norm1, dense, norm2, head):
+                z = np.zeros(l.biases.shape)
+                e = step_checks.update_errors(z, l.dbiases.get(), z, z, l.biases.get(), l.bias_momentums.get(),
+                                              l.bias_cache.get(), lr_adam, 0)
+                assert max(e) <= 1
+
+
+@pytest.mark.parametrize("decay", [0.0, 0.05])
+def test_recorded_steps_equal_eager_steps(decay):
+    """The whole network, norms and optimizer, replayed from a recording: the same bits as eager steps, with evaluations in
+    between and batches of another size."""
+    import aether
+    steps = _batches(6)
+    runs = []
+    for record in (False, True):
+        model = _network(aether.Optimizer_Muon(decay=decay))
+        if record:
+            model.record_steps(True)
+            assert model.recording_active
+        seen = []
+        for k, (x, y) in enumerate(steps):
+            seen.append(model.train_step(x, y)[:3])
+            if k == 3:
+                model.train_step(x[:5], y[:5])
+                model.predict(x[:3])
+        runs.append((seen, _host(model), model.optimizer.iterations, model.optimizer.current_learning_rate))
+        if record:
+            assert any(rec["graph"] for rec in model._recordings.values())
+            model.record_steps(False)
+    assert runs[0][0] == runs[1][0] and runs[0][2:] == runs[1][2:]
+    assert all(np.array_equal(a, b) for a, b in zip(runs[0][1], runs[1][1]))
+
+
+def test_another_optimizer_makes_a_recording_stale():
+    import aether
+    steps = _batches(8)
+    runs = []
+    for record in (False, True):
+        model = _network(aether.Optimizer_Adam(), norm=False)
+        model.record_steps(record)
+        for k, (x, y) in enumerate(steps):
+            if k == 3:
+                model.set(optimizer=aether.Optimizer_Muon())
+            if k == 6:
+                model.set(optimizer=aether.Optimizer_Adam(learning_rate=1e-2))
+            model.train_step(x, y)
+        runs.append(_host(model))
+        model.record_steps(False)
+    assert all(np.array_equal(a, b) for a, b in zip(*runs))
+
+
+def test_which_layers_are_matrices():
+    import aether
+    model = _network(aether.Optimizer_Muon())
+    conv, norm1, dense, norm2, head = model.trainable_layers
+    model.forward(_batches(1)[0][0], training=True)
+    takes = aether.Optimizer_Muon.takes
+    assert takes(conv) and takes(dense) and not takes(head) and not takes(norm1)
+    head.muon, dense.muon = True, False
+    assert takes(head) and not takes(dense)
+    assert not takes(aether.Layer_Dense(1, 9)) and not takes(aether.Layer_Dense(9, 1)) and takes(aether.Layer_Dense(2, 2))
+
+
+def test_a_shared_layer_is_refused_and_a_wrong_gradient_too():
+    import aether
+    opt = aether.Optimizer_Muon()
+    layer = aether.Layer_Dense(6, 5)
+    layer.forward(np.ones((2, 6), np.float32), True)
+    layer.backward(np.ones((2, 5), np.float32))
+    opt.update_parameters(layer)
+    opt.update_parameters(layer)
+    with pytest.raises(ValueError, match="overlap"):
+        opt.post_update_parameters()
+    opt = aether.Optimizer_Muon()
+    layer.dweights = aether.DeviceTensor.zeros((6, 4))
+    opt.update_parameters(layer)
+    with pytest.raises(ValueError, match="gradient shape"):
+        opt.post_update_parameters()
+
+
+def test_training_prints_the_reference_lines_with_muon(capsys):
+    import aether
+    model = _network(aether.Optimizer_Muon(learning_rate=0.01))
+    r = np.random.RandomState(3)
+    X, y = r.randn(40, 8, 8, 3).astype(np.float32), r.randint(0, 10, 40)
+    model.train(X, y, epochs=2, batch_size=16, print_every=1, validation_data=(X[:8], y[:8]))
+    out = capsys.readouterr().out
+    assert out.count("epoch: 2, acc:") == 3 and "lr:: 0.01" in out and "Valdiation" in out
+
+
+def test_parameter_files_with_a_layer_norm(tmp_path):
+    import aether
+    model, other = _network(aether.Optimizer_Muon()), _network(aether.Optimizer_Muon(), seed=5)
+    x, y = _batches(1)[0]
+    model.train_step(x, y)
+    path = str(tmp_path / "p")
+    model.save_parameters(path)
+    other.load_parameters(path)
+    assert all(np.array_equal(a, b) for a, b in zip(_host(model), _host(other)))
+    assert np.array_equal(model.predict(x), other.predict(x))
