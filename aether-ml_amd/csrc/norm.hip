@@ -10,9 +10,12 @@
 // All sums are float32 in a fixed order: results do not depend on timing.
 #include "common.h"
 
+#include <initializer_list>
+
 namespace aeth {
 
 constexpr int kLnThreads = 256;
+constexpr int kLnGrid = 8192;
 
 // float32 -> bfloat16 bits, round to nearest even; NaN stays NaN
 __device__ __forceinline__ unsigned ln_bf16(float f) {
@@ -21,33 +24,203 @@ __device__ __forceinline__ unsigned ln_bf16(float f) {
     return (u + 0x7fffu + ((u >> 16) & 1u)) >> 16;
 }
 
-// sum over the workgroup, the same value in every thread
-__device__ __forceinline__ float ln_block_sum(float v, float* red) {
+typedef float ln_f4 __attribute__((ext_vector_type(4)));
+
+// W consecutive floats (16-byte aligned for W = 4)
+template <int W>
+__device__ __forceinline__ void ln_load(const float* __restrict__ p, float* v) {
+    if (W == 4) {
+        const ln_f4 t = *reinterpret_cast<const ln_f4*>(p);
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
-    __syncthreads();                                     // the last use of `red` is over
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
-    __syncthreads();
-    return (red[0] + red[1]) + (red[2] + red[3]);
+        for (int e = 0; e < W; ++e) v[e] = t[e];
+    } else {
+        v[0] = *p;
+    }
 }
 
-// One workgroup per row, three passes over it.
+template <int W>
+__device__ __forceinline__ void ln_store(float* __restrict__ p, const float* v) {
+    if (W == 4) *reinterpret_cast<ln_f4*>(p) = ln_f4{v[0], v[1], v[2], v[3]};
+    else *p = v[0];
+}
+
+template <int W>
+__device__ __forceinline__ void ln_store16(uint16_t* __restrict__ p, const float* v) {
+    if (W == 4) {
+        const unsigned lo = ln_bf16(v[0]) | (ln_bf16(v[1]) << 16), hi = ln_bf16(v[2]) | (ln_bf16(v[3]) << 16);
+        *reinterpret_cast<uint2*>(p) = uint2{lo, hi};
+    } else {
+        *p = (uint16_t)ln_bf16(v[0]);
+    }
+}
+
+// Sum over aligned groups of L lanes, the same value in every lane of the group: within 16 lanes by the cross-lane paths of
+// the vector unit, beyond by swapping halves.
+template <int kCtrl>
+__device__ __forceinline__ float ln_dpp(float v) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), kCtrl, 0xf, 0xf, true));
+}
+template <int L>
+__device__ __forceinline__ float ln_group_sum(float v) {
+    if (L >= 2) v += ln_dpp<0xb1>(v);                    // quad_perm 1,0,3,2
+    if (L >= 4) v += ln_dpp<0x4e>(v);                    // quad_perm 2,3,0,1
+    if (L >= 8) v += ln_dpp<0x141>(v);                   // row_half_mirror
+    if (L >= 16) v += ln_dpp<0x140>(v);                  // row_mirror
+    if (L >= 32) v += __shfl_xor(v, 16, 64);
+    if (L >= 64) v += __shfl_xor(v, 32, 64);
+    return v;
+}
+
+// Sum over the workgroup's T threads, the same value in every thread.  Two slots of `red`, used in turn, need one barrier a
+// sum: a wave can be at most one barrier ahead of the slowest.
+template <int T>
+__device__ __forceinline__ float ln_block_sum(float v, float (*red)[T / 64], int& turn) {
+    v = ln_group_sum<64>(v);
+    if ((threadIdx.x & 63) == 0) red[turn][threadIdx.x >> 6] = v;
+    __syncthreads();
+    float s = red[turn][0];
+#pragma unroll
+    for (int w = 1; w < T / 64; ++w) s += red[turn][w];
+    turn ^= 1;
+    return s;
+}
+
+// ---- forward -----------------------------------------------------------------------------------------------------------
+// Bound: HBM, 8 bytes an element (10 with the bfloat16 copy).  A row is read once and stays in registers: lane s of the row's
+// L lanes (or of the workgroup's T threads) holds the W-float units s, s + L, ... (V of them); the mean, then the sum of
+// squares of what is left, then the output, so that no cancellation of two large sums enters the variance.
+// Units are 16 bytes where C and every pointer allow it, 4 bytes otherwise.
+
+// Rows of at most 64 V units: a row per L lanes, 256 / L rows a workgroup; gamma and beta stay in registers over the rows.
+template <int L, int V, int W>
+__global__ __launch_bounds__(256) void ln_fwd_wave(const float* __restrict__ x, const float* __restrict__ gamma,
+                                                   const float* __restrict__ beta, float* __restrict__ save_mean,
+                                                   float* __restrict__ save_invstd, float* __restrict__ y,
+                                                   uint16_t* __restrict__ y16, int rows, int C, float eps) {
+    const int s = threadIdx.x % L;
+    float g[V][W], b[V][W];
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        const int c = (s + L * j) * W;
+        if (c < C) {
+            ln_load<W>(gamma + c, g[j]);
+            ln_load<W>(beta + c, b[j]);
+        }
+    }
+    const int step = gridDim.x * (256 / L);
+    for (int64_t r = (int64_t)blockIdx.x * (256 / L) + threadIdx.x / L; r < rows; r += step) {
+        const size_t at = (size_t)r * C;
+        float v[V][W], sum = 0.f;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const int c = (s + L * j) * W;
+            if (c < C) ln_load<W>(x + at + c, v[j]);
+#pragma unroll
+            for (int e = 0; e < W; ++e) {
+                if (c >= C) v[j][e] = 0.f;
+                sum += v[j][e];
+            }
+        }
+        const float mean = ln_group_sum<L>(sum) / (float)C;
+        float q = 0.f;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const bool in = (s + L * j) * W < C;
+#pragma unroll
+            for (int e = 0; e < W; ++e) {
+                v[j][e] -= mean;
+                q += in ? v[j][e] * v[j][e] : 0.f;
+            }
+        }
+        const float invstd = 1.0f / sqrtf(ln_group_sum<L>(q) / (float)C + eps);
+        if (save_mean != nullptr && s == 0) {
+            save_mean[r] = mean;
+            save_invstd[r] = invstd;
+        }
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const int c = (s + L * j) * W;
+            if (c < C) {
+#pragma unroll
+                for (int e = 0; e < W; ++e) v[j][e] = v[j][e] * invstd * g[j][e] + b[j][e];
+                ln_store<W>(y + at + c, v[j]);
+                if (y16 != nullptr) ln_store16<W>(y16 + at + c, v[j]);
+            }
+        }
+    }
+}
+
+// Longer rows, up to T V units: a row per workgroup.
+template <int T, int V, int W>
+__global__ __launch_bounds__(T) void ln_fwd_block(const float* __restrict__ x, const float* __restrict__ gamma,
+                                                  const float* __restrict__ beta, float* __restrict__ save_mean,
+                                                  float* __restrict__ save_invstd, float* __restrict__ y,
+                                                  uint16_t* __restrict__ y16, int rows, int C, float eps) {
+    __shared__ float red[2][T / 64];
+    int turn = 0;
+    for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
+        const size_t at = (size_t)r * C;
+        float v[V][W], sum = 0.f;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const int c = (threadIdx.x + T * j) * W;
+            if (c < C) ln_load<W>(x + at + c, v[j]);
+#pragma unroll
+            for (int e = 0; e < W; ++e) {
+                if (c >= C) v[j][e] = 0.f;
+                sum += v[j][e];
+            }
+        }
+        const float mean = ln_block_sum<T>(sum, red, turn) / (float)C;
+        float q = 0.f;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const bool in = (int)(threadIdx.x + T * j) * W < C;
+#pragma unroll
+            for (int e = 0; e < W; ++e) {
+                v[j][e] -= mean;
+                q += in ? v[j][e] * v[j][e] : 0.f;
+            }
+        }
+        const float invstd = 1.0f / sqrtf(ln_block_sum<T>(q, red, turn) / (float)C + eps);
+        if (save_mean != nullptr && threadIdx.x == 0) {
+            save_mean[r] = mean;
+            save_invstd[r] = invstd;
+        }
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const int c = (threadIdx.x + T * j) * W;
+            if (c < C) {
+                float g[W], b[W];
+                ln_load<W>(gamma + c, g);
+                ln_load<W>(beta + c, b);
+#pragma unroll
+                for (int e = 0; e < W; ++e) v[j][e] = v[j][e] * invstd * g[e] + b[e];
+                ln_store<W>(y + at + c, v[j]);
+                if (y16 != nullptr) ln_store16<W>(y16 + at + c, v[j]);
+            }
+        }
+    }
+}
+
+// Rows of any length: three passes over the row.
 __global__ __launch_bounds__(kLnThreads) void ln_fwd_rows(const float* __restrict__ x, const float* __restrict__ gamma,
                                                           const float* __restrict__ beta, float* __restrict__ save_mean,
                                                           float* __restrict__ save_invstd, float* __restrict__ y,
                                                           uint16_t* __restrict__ y16, int rows, int C, float eps) {
-    __shared__ float red[4];
+    __shared__ float red[2][kLnThreads / 64];
+    int turn = 0;
     for (int r = blockIdx.x; r < rows; r += gridDim.x) {
         const float* xr = x + (size_t)r * C;
         float s = 0.f;
         for (int c = threadIdx.x; c < C; c += kLnThreads) s += xr[c];
-        const float mean = ln_block_sum(s, red) / (float)C;
+        const float mean = ln_block_sum<kLnThreads>(s, red, turn) / (float)C;
         float q = 0.f;
         for (int c = threadIdx.x; c < C; c += kLnThreads) {
             const float d = xr[c] - mean;
             q += d * d;
         }
-        const float invstd = 1.0f / sqrtf(ln_block_sum(q, red) / (float)C + eps);
+        const float invstd = 1.0f / sqrtf(ln_block_sum<kLnThreads>(q, red, turn) / (float)C + eps);
         if (threadIdx.x == 0 && save_mean != nullptr) {
             save_mean[r] = mean;
             save_invstd[r] = invstd;
@@ -64,7 +237,8 @@ __global__ __launch_bounds__(kLnThreads) void ln_bwd_rows(const float* __restric
                                                           const float* __restrict__ gamma, const float* __restrict__ mean,
                                                           const float* __restrict__ invstd, float* __restrict__ dx,
                                                           uint16_t* __restrict__ dx16, int rows, int C) {
-    __shared__ float red[4];
+    __shared__ float red[2][kLnThreads / 64];
+    int turn = 0;
     for (int r = blockIdx.x; r < rows; r += gridDim.x) {
         const size_t at = (size_t)r * C;
         const float m = mean[r], is = invstd[r];
@@ -74,8 +248,8 @@ __global__ __launch_bounds__(kLnThreads) void ln_bwd_rows(const float* __restric
             s1 += g;
             s2 += g * ((x[at + c] - m) * is);
         }
-        const float c1 = ln_block_sum(s1, red) / (float)C;
-        const float c2 = ln_block_sum(s2, red) / (float)C;
+        const float c1 = ln_block_sum<kLnThreads>(s1, red, turn) / (float)C;
+        const float c2 = ln_block_sum<kLnThreads>(s2, red, turn) / (float)C;
         for (int c = threadIdx.x; c < C; c += kLnThreads) {
             const float v = is * (dy[at + c] * gamma[c] - c1 - (x[at + c] - m) * is * c2);
             dx[at + c] = v;
@@ -126,6 +300,39 @@ static bool ln_apart(const void* a, const void* b, int64_t na, int64_t nb) {
     return p == nullptr || q == nullptr || p + na <= q || q + nb <= p;
 }
 
+static bool ln_vec4(int C, std::initializer_list<const void*> pointers) {
+    if (C % 4 != 0) return false;
+    for (const void* p : pointers)
+        if ((reinterpret_cast<uintptr_t>(p) & 15) != 0) return false;
+    return true;
+}
+
+typedef void (*LnFwd)(const float*, const float*, const float*, float*, float*, float*, uint16_t*, int, int, float);
+
+// The kernel for rows of `units` W-float units, its threads and the rows it takes at a time.
+template <int W>
+static LnFwd ln_fwd_kernel(int units, int* threads, int* rows_per_block) {
+    constexpr int F = 4 / W;                             // 4-byte units: four times as many of them for the same registers
+    *threads = 256;
+    const auto wave = [&](LnFwd k, int lanes) { *rows_per_block = 256 / lanes; return k; };
+    if (units <= 4) return wave(ln_fwd_wave<4, 1, W>, 4);
+    if (units <= 8) return wave(ln_fwd_wave<8, 1, W>, 8);
+    if (units <= 16) return wave(ln_fwd_wave<16, 1, W>, 16);
+    if (units <= 32) return wave(ln_fwd_wave<32, 1, W>, 32);
+    if (units <= 64) return wave(ln_fwd_wave<64, 1, W>, 64);
+    if (units <= 128) return wave(ln_fwd_wave<64, 2, W>, 64);
+    if (units <= 256) return wave(ln_fwd_wave<64, 4, W>, 64);
+    *rows_per_block = 1;
+    if (units <= 512 * F) return ln_fwd_block<256, 2 * F, W>;
+    if (units <= 1024 * F) return ln_fwd_block<256, 4 * F, W>;
+    if (units <= 2048 * F) return ln_fwd_block<256, 8 * F, W>;
+    *threads = 1024;
+    if (units <= 4096 * F) return ln_fwd_block<1024, 4 * F, W>;
+    if (units <= 8192 * F) return ln_fwd_block<1024, 8 * F, W>;
+    *threads = 256;
+    return ln_fwd_rows;
+}
+
 // The arguments are checked before the context: a bad call is refused alike with and without a GPU.
 static int ln_fwd_impl(const float* x, const float* gamma, const float* beta, float* save_mean, float* save_invstd, float* y,
                        uint16_t* y16, int rows, int C, float eps) {
@@ -137,8 +344,12 @@ static int ln_fwd_impl(const float* x, const float* gamma, const float* beta, fl
     AETH_CHECK_ARG(ln_apart(x, y, 4 * n, 4 * n) && ln_apart(x, y16, 4 * n, 2 * n) && ln_apart(y, y16, 4 * n, 2 * n));
     AETH_REQUIRE_INIT();
     if (rows == 0) return AETH_OK;
-    hipLaunchKernelGGL(ln_fwd_rows, dim3(rows < 65536 ? rows : 65536), dim3(kLnThreads), 0, ctx().stream, x, gamma, beta,
-                       save_mean, save_invstd, y, y16, rows, C, eps);
+    int threads, per;
+    const LnFwd kernel = ln_vec4(C, {x, gamma, beta, y, y16}) ? ln_fwd_kernel<4>(C / 4, &threads, &per)
+                                                              : ln_fwd_kernel<1>(C, &threads, &per);
+    const int want = cdiv(rows, per);
+    hipLaunchKernelGGL(kernel, dim3(want < kLnGrid ? want : kLnGrid), dim3(threads), 0, ctx().stream, x, gamma, beta, save_mean,
+                       save_invstd, y, y16, rows, C, eps);
     AETH_LAUNCH_CHECK();
     return AETH_OK;
 }
