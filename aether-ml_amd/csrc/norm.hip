@@ -233,6 +233,181 @@ __global__ __launch_bounds__(kLnThreads) void ln_fwd_rows(const float* __restric
     }
 }
 
+// ---- backward ----------------------------------------------------------------------------------------------------------
+// Bound: HBM, 12 bytes an element (14 with the bfloat16 copy).  x and dy are read once: the same lanes hold the row while its
+// two sums are taken, and the lane that owns a column adds its dy xhat and dy over all rows it sees.  A workgroup walks many
+// rows and leaves one partial row of dgamma and one of dbeta, part[block][2][C]; ln_bwd_finish adds those in block order.
+
+// Rows of at most 64 V units, as ln_fwd_wave; T / L rows at a time.
+template <int T, int L, int V, int W>
+__global__ __launch_bounds__(T) void ln_bwd_wave(const float* __restrict__ x, const float* __restrict__ dy,
+                                                 const float* __restrict__ gamma, const float* __restrict__ mean,
+                                                 const float* __restrict__ invstd, float* __restrict__ dx,
+                                                 uint16_t* __restrict__ dx16, int rows, int C, float* __restrict__ part) {
+    __shared__ float red[T / 64][L * V * W];
+    const int s = threadIdx.x % L;
+    float gm[V][W], dg[V][W], db[V][W];
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        const int c = (s + L * j) * W;
+#pragma unroll
+        for (int e = 0; e < W; ++e) dg[j][e] = db[j][e] = gm[j][e] = 0.f;
+        if (c < C) ln_load<W>(gamma + c, gm[j]);
+    }
+    const int step = gridDim.x * (T / L);
+    for (int64_t r = (int64_t)blockIdx.x * (T / L) + threadIdx.x / L; r < rows; r += step) {
+        const size_t at = (size_t)r * C;
+        const float m = mean[r], is = invstd[r];
+        float xh[V][W], g[V][W], s1 = 0.f, s2 = 0.f;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const int c = (s + L * j) * W;
+            if (c < C) {
+                ln_load<W>(x + at + c, xh[j]);
+                ln_load<W>(dy + at + c, g[j]);
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const bool in = (s + L * j) * W < C;
+#pragma unroll
+            for (int e = 0; e < W; ++e) {
+                xh[j][e] = in ? (xh[j][e] - m) * is : 0.f;
+                const float d = in ? g[j][e] : 0.f;
+                dg[j][e] += d * xh[j][e];
+                db[j][e] += d;
+                g[j][e] = d * gm[j][e];
+                s1 += g[j][e];
+                s2 += g[j][e] * xh[j][e];
+            }
+        }
+        const float c1 = ln_group_sum<L>(s1) / (float)C, c2 = ln_group_sum<L>(s2) / (float)C;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const int c = (s + L * j) * W;
+            if (c < C) {
+                float v[W];
+#pragma unroll
+                for (int e = 0; e < W; ++e) v[e] = is * (g[j][e] - c1 - xh[j][e] * c2);
+                ln_store<W>(dx + at + c, v);
+                if (dx16 != nullptr) ln_store16<W>(dx16 + at + c, v);
+            }
+        }
+    }
+    // the rows of a wave, then the waves in order
+    float* out = part + (size_t)blockIdx.x * 2 * C;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+#pragma unroll
+            for (int e = 0; e < W; ++e) {
+                float v = k == 0 ? dg[j][e] : db[j][e];
+#pragma unroll
+                for (int o = L; o < 64; o <<= 1) v += __shfl_xor(v, o, 64);
+                if ((threadIdx.x & 63) < L) red[threadIdx.x >> 6][(s + L * j) * W + e] = v;
+            }
+        __syncthreads();
+        for (int c = threadIdx.x; c < C; c += T) {
+            float v = red[0][c];
+#pragma unroll
+            for (int w = 1; w < T / 64; ++w) v += red[w][c];
+            out[(size_t)k * C + c] = v;
+        }
+        __syncthreads();
+    }
+}
+
+// Longer rows, up to T V units: a row per workgroup.
+template <int T, int V, int W>
+__global__ __launch_bounds__(T) void ln_bwd_block(const float* __restrict__ x, const float* __restrict__ dy,
+                                                  const float* __restrict__ gamma, const float* __restrict__ mean,
+                                                  const float* __restrict__ invstd, float* __restrict__ dx,
+                                                  uint16_t* __restrict__ dx16, int rows, int C, float* __restrict__ part) {
+    __shared__ float red1[2][T / 64], red2[2][T / 64];
+    int turn = 0;
+    float dg[V][W], db[V][W];
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+#pragma unroll
+        for (int e = 0; e < W; ++e) dg[j][e] = db[j][e] = 0.f;
+    for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
+        const size_t at = (size_t)r * C;
+        const float m = mean[r], is = invstd[r];
+        float xh[V][W], g[V][W], s1 = 0.f, s2 = 0.f;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const int c = (threadIdx.x + T * j) * W;
+            if (c < C) {
+                ln_load<W>(x + at + c, xh[j]);
+                ln_load<W>(dy + at + c, g[j]);
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const int c = (threadIdx.x + T * j) * W;
+            float gm[W];
+            if (c < C) ln_load<W>(gamma + c, gm);
+#pragma unroll
+            for (int e = 0; e < W; ++e) {
+                xh[j][e] = c < C ? (xh[j][e] - m) * is : 0.f;
+                const float d = c < C ? g[j][e] : 0.f;
+                dg[j][e] += d * xh[j][e];
+                db[j][e] += d;
+                g[j][e] = c < C ? d * gm[e] : 0.f;
+                s1 += g[j][e];
+                s2 += g[j][e] * xh[j][e];
+            }
+        }
+        // (both sums behind one barrier; the slots are used in turn as in ln_block_sum)
+        s1 = ln_group_sum<64>(s1);
+        s2 = ln_group_sum<64>(s2);
+        if ((threadIdx.x & 63) == 0) {
+            red1[turn][threadIdx.x >> 6] = s1;
+            red2[turn][threadIdx.x >> 6] = s2;
+        }
+        __syncthreads();
+        s1 = red1[turn][0];
+        s2 = red2[turn][0];
+#pragma unroll
+        for (int w = 1; w < T / 64; ++w) {
+            s1 += red1[turn][w];
+            s2 += red2[turn][w];
+        }
+        turn ^= 1;
+        const float c1 = s1 / (float)C, c2 = s2 / (float)C;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const int c = (threadIdx.x + T * j) * W;
+            if (c < C) {
+                float v[W];
+#pragma unroll
+                for (int e = 0; e < W; ++e) v[e] = is * (g[j][e] - c1 - xh[j][e] * c2);
+                ln_store<W>(dx + at + c, v);
+                if (dx16 != nullptr) ln_store16<W>(dx16 + at + c, v);
+            }
+        }
+    }
+    float* out = part + (size_t)blockIdx.x * 2 * C;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        const int c = (threadIdx.x + T * j) * W;
+        if (c < C) {
+            if (W == 4 && (reinterpret_cast<uintptr_t>(out) & 15) == 0) {
+                ln_store<W>(out + c, dg[j]);
+                ln_store<W>(out + C + c, db[j]);
+            } else {
+#pragma unroll
+                for (int e = 0; e < W; ++e) {
+                    out[c + e] = dg[j][e];
+                    out[C + c + e] = db[j][e];
+                }
+            }
+        }
+    }
+}
+
+// Rows of any length: the gradient of the rows in two passes, the column sums in a kernel of their own.
 __global__ __launch_bounds__(kLnThreads) void ln_bwd_rows(const float* __restrict__ x, const float* __restrict__ dy,
                                                           const float* __restrict__ gamma, const float* __restrict__ mean,
                                                           const float* __restrict__ invstd, float* __restrict__ dx,
@@ -258,7 +433,7 @@ __global__ __launch_bounds__(kLnThreads) void ln_bwd_rows(const float* __restric
     }
 }
 
-// Partial sums of dy xhat and dy over a run of rows: 64 columns x 4 row lanes per workgroup, part[2][runs][C].
+// Partial sums of dy xhat and dy over a run of rows: 64 columns x 4 row lanes per workgroup, part[run][2][C].
 __global__ __launch_bounds__(kLnThreads) void ln_bwd_columns(const float* __restrict__ x, const float* __restrict__ dy,
                                                              const float* __restrict__ mean,
                                                              const float* __restrict__ invstd, int rows, int C, int run,
@@ -278,21 +453,34 @@ __global__ __launch_bounds__(kLnThreads) void ln_bwd_columns(const float* __rest
     red[1][w][lane] = b;
     __syncthreads();
     if (w < 2 && c < C)
-        part[((size_t)w * gridDim.y + blockIdx.y) * C + c] =
+        part[((size_t)blockIdx.y * 2 + w) * C + c] =
             (red[w][0][lane] + red[w][1][lane]) + (red[w][2][lane] + red[w][3][lane]);
 }
 
-__global__ __launch_bounds__(kLnThreads) void ln_bwd_finish(const float* __restrict__ part, int runs, int C,
-                                                            float* __restrict__ dgamma, float* __restrict__ dbeta) {
-    const int c = blockIdx.x * kLnThreads + threadIdx.x;
-    if (c >= C) return;
-    float a = 0.f, b = 0.f;
-    for (int i = 0; i < runs; ++i) {
-        a += part[(size_t)i * C + c];
-        b += part[((size_t)runs + i) * C + c];
+// dgamma | dbeta = the partial rows part[block][2C], added in block order: 64 columns a workgroup, 16 lanes of blocks each.
+__global__ __launch_bounds__(1024) void ln_bwd_finish(const float* __restrict__ part, int blocks, int C,
+                                                      float* __restrict__ dgamma, float* __restrict__ dbeta) {
+    __shared__ float red[16][64];
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    const int64_t c = (int64_t)blockIdx.x * 64 + lane, C2 = 2 * (int64_t)C;
+    float a[4] = {0.f, 0.f, 0.f, 0.f};
+    if (c < C2) {
+        int i = w;
+        for (; i + 48 < blocks; i += 64) {
+#pragma unroll
+            for (int u = 0; u < 4; ++u) a[u] += part[(i + 16 * u) * C2 + c];
+        }
+        for (; i < blocks; i += 16) a[0] += part[i * C2 + c];
     }
-    dgamma[c] = a;
-    dbeta[c] = b;
+    red[w][lane] = (a[0] + a[1]) + (a[2] + a[3]);
+    __syncthreads();
+    if (w == 0 && c < C2) {
+        float v = red[0][lane];
+#pragma unroll
+        for (int k = 1; k < 16; ++k) v += red[k][lane];
+        if (c < C) dgamma[c] = v;
+        else dbeta[c - C] = v;
+    }
 }
 
 static bool ln_apart(const void* a, const void* b, int64_t na, int64_t nb) {
@@ -333,6 +521,39 @@ static LnFwd ln_fwd_kernel(int units, int* threads, int* rows_per_block) {
     return ln_fwd_rows;
 }
 
+typedef void (*LnBwd)(const float*, const float*, const float*, const float*, const float*, float*, uint16_t*, int, int,
+                      float*);
+
+// As ln_fwd_kernel; `cap`: the most workgroups to launch.  NULL: rows too long for the registers of a workgroup.
+template <int W>
+static LnBwd ln_bwd_kernel(int units, int* threads, int* rows_per_block, int* cap) {
+    constexpr int F = 4 / W;
+    constexpr int T = 512;
+    *threads = T;
+    *cap = 512;
+    const auto wave = [&](LnBwd k, int lanes) { *rows_per_block = T / lanes; return k; };
+    if (units <= 4) return wave(ln_bwd_wave<T, 4, 1, W>, 4);
+    if (units <= 8) return wave(ln_bwd_wave<T, 8, 1, W>, 8);
+    if (units <= 16) return wave(ln_bwd_wave<T, 16, 1, W>, 16);
+    if (units <= 32) return wave(ln_bwd_wave<T, 32, 1, W>, 32);
+    if (units <= 64) return wave(ln_bwd_wave<T, 64, 1, W>, 64);
+    if (units <= 128) return wave(ln_bwd_wave<T, 64, 2, W>, 64);
+    if (units <= 256) return wave(ln_bwd_wave<T, 64, 4, W>, 64);
+    *rows_per_block = 1;
+    *threads = 256;
+    *cap = 768;
+    if (units <= 512 * F) return ln_bwd_block<256, 2 * F, W>;
+    if (units <= 1024 * F) return ln_bwd_block<256, 4 * F, W>;
+    *threads = 512;
+    *cap = 512;
+    if (units <= 2048 * F) return ln_bwd_block<512, 4 * F, W>;
+    *threads = 1024;
+    *cap = 256;
+    if (units <= 4096 * F) return ln_bwd_block<1024, 4 * F, W>;
+    *rows_per_block = 256;
+    return nullptr;
+}
+
 // The arguments are checked before the context: a bad call is refused alike with and without a GPU.
 static int ln_fwd_impl(const float* x, const float* gamma, const float* beta, float* save_mean, float* save_invstd, float* y,
                        uint16_t* y16, int rows, int C, float eps) {
@@ -363,23 +584,29 @@ static int ln_bwd_impl(const float* x, const float* dy, const float* gamma, cons
     AETH_CHECK_ARG(ln_apart(x, dx16, 4 * n, 2 * n) && ln_apart(dy, dx16, 4 * n, 2 * n) && ln_apart(dx, dx16, 4 * n, 2 * n));
     AETH_REQUIRE_INIT();
     hipStream_t st = ctx().stream;
-    int runs = cdiv(rows, 256);
-    if (runs > 256) runs = 256;
-    const int run = runs > 0 ? cdiv(rows, runs) : 0;
-    if (runs > 0) runs = cdiv(rows, run);
+    int threads, per, cap, blocks = 0;
     void* ws = nullptr;
-    if (runs > 0) {
-        const int rc = workspace((int64_t)2 * runs * C * sizeof(float), &ws);
+    if (rows > 0) {
+        const LnBwd kernel = ln_vec4(C, {x, dy, gamma, dx, dx16}) ? ln_bwd_kernel<4>(C / 4, &threads, &per, &cap)
+                                                                  : ln_bwd_kernel<1>(C, &threads, &per, &cap);
+        blocks = cdiv(rows, per) < cap ? cdiv(rows, per) : cap;
+        const int run = cdiv(rows, blocks);
+        if (kernel == nullptr) blocks = cdiv(rows, run);
+        const int rc = workspace((int64_t)2 * blocks * C * sizeof(float), &ws);
         if (rc) return rc;
-        hipLaunchKernelGGL(ln_bwd_rows, dim3(rows < 65536 ? rows : 65536), dim3(kLnThreads), 0, st, x, dy, gamma, mean, invstd,
-                           dx, dx16, rows, C);
-        AETH_LAUNCH_CHECK();
-        hipLaunchKernelGGL(ln_bwd_columns, dim3(cdiv(C, 64), runs), dim3(kLnThreads), 0, st, x, dy, mean, invstd, rows, C, run,
-                           (float*)ws);
+        if (kernel != nullptr) {
+            hipLaunchKernelGGL(kernel, dim3(blocks), dim3(threads), 0, st, x, dy, gamma, mean, invstd, dx, dx16, rows, C,
+                               (float*)ws);
+        } else {
+            hipLaunchKernelGGL(ln_bwd_rows, dim3(rows < kLnGrid ? rows : kLnGrid), dim3(kLnThreads), 0, st, x, dy, gamma, mean,
+                               invstd, dx, dx16, rows, C);
+            AETH_LAUNCH_CHECK();
+            hipLaunchKernelGGL(ln_bwd_columns, dim3(cdiv(C, 64), blocks), dim3(kLnThreads), 0, st, x, dy, mean, invstd, rows, C,
+                               run, (float*)ws);
+        }
         AETH_LAUNCH_CHECK();
     }
-    hipLaunchKernelGGL(ln_bwd_finish, dim3(cdiv(C, kLnThreads)), dim3(kLnThreads), 0, st, (const float*)ws, runs, C, dgamma,
-                       dbeta);
+    hipLaunchKernelGGL(ln_bwd_finish, dim3(cdiv(2 * (int64_t)C, 64)), dim3(1024), 0, st, (const float*)ws, blocks, C, dgamma, dbeta);
     AETH_LAUNCH_CHECK();
     return AETH_OK;
 }
