@@ -10,12 +10,12 @@
 // All sums are float32 in a fixed order: results do not depend on timing.
 #include "common.h"
 
-#include <initializer_list>
-
 namespace aeth {
 
-constexpr int kLnThreads = 256;
-constexpr int kLnGrid = 8192;
+constexpr int kLnLong = 1024;                            // threads of the kernels for rows of any length
+
+// Outputs of this size and more are stored with the non-temporal hint: the next kernel will not find them in a cache anyway.
+constexpr int64_t kLnStreamBytes = 64 << 20;
 
 // float32 -> bfloat16 bits, round to nearest even; NaN stays NaN
 __device__ __forceinline__ unsigned ln_bf16(float f) {
@@ -24,38 +24,63 @@ __device__ __forceinline__ unsigned ln_bf16(float f) {
     return (u + 0x7fffu + ((u >> 16) & 1u)) >> 16;
 }
 
-typedef float ln_f4 __attribute__((ext_vector_type(4)));
+// A row is handled in units of four consecutive floats: unit k is columns 4k .. 4k + 3, and lane s of the row's L lanes holds units
+// s, s + L, ..., V of them.  Where C is no multiple of four, units start at any float, which 16-byte loads and stores of the
+// vector unit take, and the row's last unit is read from its last four columns; places behind the row's end read there too.  So
+// no load waits for a branch (units that went through the rest float by float: 1000000 x 20 backward 124 us instead of 64,
+// 400000 x 100 203 instead of 103).  V is the least that covers the row: only a lane's last unit can be such a one.
+typedef float ln_f4 __attribute__((ext_vector_type(4), aligned(4)));
+typedef unsigned ln_u2 __attribute__((ext_vector_type(2), aligned(2)));
 
-// W consecutive floats (16-byte aligned for W = 4)
-template <int W>
-__device__ __forceinline__ void ln_load(const float* __restrict__ p, float* v) {
-    if (W == 4) {
-        const ln_f4 t = *reinterpret_cast<const ln_f4*>(p);
+// kTiny: rows of one to three floats, which no 16-byte load fits (V = 1; only own columns are read).
+template <int V, bool kTiny = false>
+struct LnLane {
+    int c0, step;                                        // first column of unit 0, columns from unit to unit
+    int last, skip;                                      // first column read for the last unit; so many of its four are not its own
+    __device__ __forceinline__ LnLane(int s, int L, int C) {
+        c0 = 4 * s;
+        step = 4 * L;
+        const int c = c0 + step * (V - 1);
+        last = c + 4 <= C ? c : C - 4;
+        skip = c + 4 <= C ? 0 : c < C ? c - last : 4;
+    }
+    __device__ __forceinline__ int at(int j) const { return j == V - 1 ? last : c0 + step * j; }
+    __device__ __forceinline__ bool own(int j, int e) const { return j < V - 1 || e >= skip; }
+    __device__ __forceinline__ void load(const float* __restrict__ row, int j, float* v) const {
+        if (kTiny) {
 #pragma unroll
-        for (int e = 0; e < W; ++e) v[e] = t[e];
-    } else {
-        v[0] = *p;
+            for (int e = 0; e < 4; ++e) v[e] = own(j, e) ? row[at(j) + e] : 0.f;
+        } else {
+            const ln_f4 t = *reinterpret_cast<const ln_f4*>(row + at(j));
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = t[e];
+        }
     }
-}
-
-template <int W>
-__device__ __forceinline__ void ln_store(float* __restrict__ p, const float* v) {
-    if (W == 4) *reinterpret_cast<ln_f4*>(p) = ln_f4{v[0], v[1], v[2], v[3]};
-    else *p = v[0];
-}
-
-template <int W>
-__device__ __forceinline__ void ln_store16(uint16_t* __restrict__ p, const float* v) {
-    if (W == 4) {
-        const unsigned lo = ln_bf16(v[0]) | (ln_bf16(v[1]) << 16), hi = ln_bf16(v[2]) | (ln_bf16(v[3]) << 16);
-        *reinterpret_cast<uint2*>(p) = uint2{lo, hi};
-    } else {
-        *p = (uint16_t)ln_bf16(v[0]);
+    __device__ __forceinline__ void store(float* __restrict__ row, int j, const float* v, bool stream) const {
+        if (j < V - 1 || skip == 0) {
+            const ln_f4 t = {v[0], v[1], v[2], v[3]};
+            if (stream) __builtin_nontemporal_store(t, reinterpret_cast<ln_f4*>(row + at(j)));
+            else *reinterpret_cast<ln_f4*>(row + at(j)) = t;
+        } else if (skip < 4) {
+#pragma unroll
+            for (int e = 1; e < 4; ++e)
+                if (own(j, e)) row[at(j) + e] = v[e];
+        }
     }
-}
+    __device__ __forceinline__ void store16(uint16_t* __restrict__ row, int j, const float* v) const {
+        if (j < V - 1 || skip == 0) {
+            *reinterpret_cast<ln_u2*>(row + at(j)) =
+                ln_u2{ln_bf16(v[0]) | (ln_bf16(v[1]) << 16), ln_bf16(v[2]) | (ln_bf16(v[3]) << 16)};
+        } else if (skip < 4) {
+#pragma unroll
+            for (int e = 1; e < 4; ++e)
+                if (own(j, e)) row[at(j) + e] = (uint16_t)ln_bf16(v[e]);
+        }
+    }
+};
 
 // Sum over aligned groups of L lanes, the same value in every lane of the group: within 16 lanes by the cross-lane paths of
-// the vector unit, beyond by swapping halves.
+// the vector unit, beyond through the LDS crossbar.
 template <int kCtrl>
 __device__ __forceinline__ float ln_dpp(float v) {
     return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), kCtrl, 0xf, 0xf, true));
@@ -71,241 +96,281 @@ __device__ __forceinline__ float ln_group_sum(float v) {
     return v;
 }
 
-// Sum over the workgroup's T threads, the same value in every thread.  Two slots of `red`, used in turn, need one barrier a
-// sum: a wave can be at most one barrier ahead of the slowest.
-template <int T>
-__device__ __forceinline__ float ln_block_sum(float v, float (*red)[T / 64], int& turn) {
-    v = ln_group_sum<64>(v);
-    if ((threadIdx.x & 63) == 0) red[turn][threadIdx.x >> 6] = v;
-    __syncthreads();
-    float s = red[turn][0];
+// Sums over the workgroup (up to 16 waves), the same values in every thread.  Two slots, used in turn, need one barrier a sum: a
+// wave can be at most one barrier ahead of the slowest.
+struct LnTeam {
+    float (*red)[2][16];                                 // [slot][which sum][wave]
+    int turn = 0;
+    __device__ __forceinline__ explicit LnTeam(float (*r)[2][16]) : red(r) {}
+    template <int N>
+    __device__ __forceinline__ void sum(float* v) {
+        const int waves = blockDim.x >> 6;
 #pragma unroll
-    for (int w = 1; w < T / 64; ++w) s += red[turn][w];
-    turn ^= 1;
-    return s;
-}
+        for (int i = 0; i < N; ++i) {
+            v[i] = ln_group_sum<64>(v[i]);
+            if ((threadIdx.x & 63) == 0) red[turn][i][threadIdx.x >> 6] = v[i];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            v[i] = red[turn][i][0];
+            for (int w = 1; w < waves; ++w) v[i] += red[turn][i][w];
+        }
+        turn ^= 1;
+    }
+};
 
 // ---- forward -----------------------------------------------------------------------------------------------------------
-// Bound: HBM, 8 bytes an element (10 with the bfloat16 copy).  A row is read once and stays in registers: lane s of the row's
-// L lanes (or of the workgroup's T threads) holds the W-float units s, s + L, ... (V of them); the mean, then the sum of
+// Bound: HBM, 8 bytes an element (10 with the bfloat16 copy): 16384 x 8192 201 us = 5.3 TB/s, the rate of a copy; rows that no
+// power of two divides 4.2-5.2 TB/s.  A row is read once and stays in registers: the mean, then the sum of
 // squares of what is left, then the output, so that no cancellation of two large sums enters the variance.
-// Units are 16 bytes where C and every pointer allow it, 4 bytes otherwise.
+struct LnFwdArgs {
+    const float *x, *gamma, *beta;
+    float *mean, *invstd, *y;
+    uint16_t* y16;
+    int rows, C;
+    float inv_c, eps;
+    bool stream;
+};
 
-// Rows of at most 64 V units: a row per L lanes, 256 / L rows a workgroup; gamma and beta stay in registers over the rows.
-template <int L, int V, int W>
-__global__ __launch_bounds__(256) void ln_fwd_wave(const float* __restrict__ x, const float* __restrict__ gamma,
-                                                   const float* __restrict__ beta, float* __restrict__ save_mean,
-                                                   float* __restrict__ save_invstd, float* __restrict__ y,
-                                                   uint16_t* __restrict__ y16, int rows, int C, float eps) {
-    const int s = threadIdx.x % L;
-    float g[V][W], b[V][W];
+// The row's values in v become its output.  Columns that the last unit reads but does not own count 0 times.  `sum(float)`: over
+// the row's lanes; `affine(j, g, b)`: gamma and beta of unit j.
+template <int V, bool kTiny, typename Sum, typename Affine>
+__device__ __forceinline__ void ln_fwd_row(const LnFwdArgs& p, int64_t r, const LnLane<V, kTiny>& u, float (*v)[4], bool first,
+                                           Sum sum, Affine affine) {
+    float s = 0.f;
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s += u.own(j, e) ? v[j][e] : 0.f;
+    const float mean = sum(s) * p.inv_c;
+    float q = 0.f;
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            v[j][e] -= mean;
+            q += u.own(j, e) ? v[j][e] * v[j][e] : 0.f;
+        }
+    const float invstd = 1.0f / sqrtf(sum(q) * p.inv_c + p.eps);
+    if (first && p.mean != nullptr) {
+        p.mean[r] = mean;
+        p.invstd[r] = invstd;
+    }
+    const size_t at = (size_t)r * p.C;
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-        const int c = (s + L * j) * W;
-        if (c < C) {
-            ln_load<W>(gamma + c, g[j]);
-            ln_load<W>(beta + c, b[j]);
+        float g[4], b[4];
+        affine(j, g, b);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[j][e] = v[j][e] * invstd * g[e] + b[e];
+        u.store(p.y + at, j, v[j], p.stream);
+        if (p.y16 != nullptr) u.store16(p.y16 + at, j, v[j]);
+    }
+}
+
+// Rows of at most L V units, 256 / L of them at a time; gamma and beta of up to four units stay in registers over the rows.
+template <int L, int V, bool kTiny = false>
+__global__ __launch_bounds__(256) void ln_fwd_wave(const LnFwdArgs p) {
+    constexpr int K = V <= 4 ? V : 1;
+    const int s = threadIdx.x % L, C = p.C;
+    const LnLane<V, kTiny> u(s, L, C);
+    float gk[K][4], bk[K][4];
+    if (V <= 4) {
+#pragma unroll
+        for (int j = 0; j < K; ++j) {
+            u.load(p.gamma, j, gk[j]);
+            u.load(p.beta, j, bk[j]);
         }
     }
     const int step = gridDim.x * (256 / L);
-    for (int64_t r = (int64_t)blockIdx.x * (256 / L) + threadIdx.x / L; r < rows; r += step) {
-        const size_t at = (size_t)r * C;
-        float v[V][W], sum = 0.f;
+    for (int64_t r = (int64_t)blockIdx.x * (256 / L) + threadIdx.x / L; r < p.rows; r += step) {
+        float v[V][4];
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-            const int c = (s + L * j) * W;
-            if (c < C) ln_load<W>(x + at + c, v[j]);
+        for (int j = 0; j < V; ++j) u.load(p.x + (size_t)r * C, j, v[j]);
+        ln_fwd_row(p, r, u, v, s == 0, [](float a) { return ln_group_sum<L>(a); },
+                   [&](int j, float* g, float* b) {
+                       if (V <= 4) {
 #pragma unroll
-            for (int e = 0; e < W; ++e) {
-                if (c >= C) v[j][e] = 0.f;
-                sum += v[j][e];
-            }
-        }
-        const float mean = ln_group_sum<L>(sum) / (float)C;
-        float q = 0.f;
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-            const bool in = (s + L * j) * W < C;
-#pragma unroll
-            for (int e = 0; e < W; ++e) {
-                v[j][e] -= mean;
-                q += in ? v[j][e] * v[j][e] : 0.f;
-            }
-        }
-        const float invstd = 1.0f / sqrtf(ln_group_sum<L>(q) / (float)C + eps);
-        if (save_mean != nullptr && s == 0) {
-            save_mean[r] = mean;
-            save_invstd[r] = invstd;
-        }
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-            const int c = (s + L * j) * W;
-            if (c < C) {
-#pragma unroll
-                for (int e = 0; e < W; ++e) v[j][e] = v[j][e] * invstd * g[j][e] + b[j][e];
-                ln_store<W>(y + at + c, v[j]);
-                if (y16 != nullptr) ln_store16<W>(y16 + at + c, v[j]);
-            }
-        }
+                           for (int e = 0; e < 4; ++e) {
+                               g[e] = gk[V <= 4 ? j : 0][e];
+                               b[e] = bk[V <= 4 ? j : 0][e];
+                           }
+                       } else {
+                           u.load(p.gamma, j, g);
+                           u.load(p.beta, j, b);
+                       }
+                   });
     }
 }
 
-// Longer rows, up to T V units: a row per workgroup.
-template <int T, int V, int W>
-__global__ __launch_bounds__(T) void ln_fwd_block(const float* __restrict__ x, const float* __restrict__ gamma,
-                                                  const float* __restrict__ beta, float* __restrict__ save_mean,
-                                                  float* __restrict__ save_invstd, float* __restrict__ y,
-                                                  uint16_t* __restrict__ y16, int rows, int C, float eps) {
-    __shared__ float red[2][T / 64];
-    int turn = 0;
-    for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
-        const size_t at = (size_t)r * C;
-        float v[V][W], sum = 0.f;
+// Longer rows, up to blockDim V units: a row per workgroup.
+template <int T, int V>
+__global__ __launch_bounds__(T) void ln_fwd_block(const LnFwdArgs p) {
+    __shared__ float red[2][2][16];
+    LnTeam team(red);
+    const int C = p.C;
+    const LnLane<V> u(threadIdx.x, blockDim.x, C);
+    for (int64_t r = blockIdx.x; r < p.rows; r += gridDim.x) {
+        float v[V][4];
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-            const int c = (threadIdx.x + T * j) * W;
-            if (c < C) ln_load<W>(x + at + c, v[j]);
-#pragma unroll
-            for (int e = 0; e < W; ++e) {
-                if (c >= C) v[j][e] = 0.f;
-                sum += v[j][e];
-            }
-        }
-        const float mean = ln_block_sum<T>(sum, red, turn) / (float)C;
-        float q = 0.f;
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-            const bool in = (int)(threadIdx.x + T * j) * W < C;
-#pragma unroll
-            for (int e = 0; e < W; ++e) {
-                v[j][e] -= mean;
-                q += in ? v[j][e] * v[j][e] : 0.f;
-            }
-        }
-        const float invstd = 1.0f / sqrtf(ln_block_sum<T>(q, red, turn) / (float)C + eps);
-        if (save_mean != nullptr && threadIdx.x == 0) {
-            save_mean[r] = mean;
-            save_invstd[r] = invstd;
-        }
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-            const int c = (threadIdx.x + T * j) * W;
-            if (c < C) {
-                float g[W], b[W];
-                ln_load<W>(gamma + c, g);
-                ln_load<W>(beta + c, b);
-#pragma unroll
-                for (int e = 0; e < W; ++e) v[j][e] = v[j][e] * invstd * g[e] + b[e];
-                ln_store<W>(y + at + c, v[j]);
-                if (y16 != nullptr) ln_store16<W>(y16 + at + c, v[j]);
-            }
-        }
+        for (int j = 0; j < V; ++j) u.load(p.x + (size_t)r * C, j, v[j]);
+        ln_fwd_row(p, r, u, v, threadIdx.x == 0, [&](float a) { team.sum<1>(&a); return a; },
+                   [&](int j, float* g, float* b) {
+                       u.load(p.gamma, j, g);
+                       u.load(p.beta, j, b);
+                   });
     }
 }
 
 // Rows of any length: three passes over the row.
-__global__ __launch_bounds__(kLnThreads) void ln_fwd_rows(const float* __restrict__ x, const float* __restrict__ gamma,
-                                                          const float* __restrict__ beta, float* __restrict__ save_mean,
-                                                          float* __restrict__ save_invstd, float* __restrict__ y,
-                                                          uint16_t* __restrict__ y16, int rows, int C, float eps) {
-    __shared__ float red[2][kLnThreads / 64];
-    int turn = 0;
-    for (int r = blockIdx.x; r < rows; r += gridDim.x) {
-        const float* xr = x + (size_t)r * C;
+__global__ __launch_bounds__(kLnLong) void ln_fwd_rows(const LnFwdArgs p) {
+    __shared__ float red[2][2][16];
+    LnTeam team(red);
+    const int C = p.C;
+    for (int64_t r = blockIdx.x; r < p.rows; r += gridDim.x) {
+        const float* xr = p.x + (size_t)r * C;
         float s = 0.f;
-        for (int c = threadIdx.x; c < C; c += kLnThreads) s += xr[c];
-        const float mean = ln_block_sum<kLnThreads>(s, red, turn) / (float)C;
+        for (int64_t c = threadIdx.x; c < C; c += kLnLong) s += xr[c];
+        team.sum<1>(&s);
+        const float mean = s * p.inv_c;
         float q = 0.f;
-        for (int c = threadIdx.x; c < C; c += kLnThreads) {
+        for (int64_t c = threadIdx.x; c < C; c += kLnLong) {
             const float d = xr[c] - mean;
             q += d * d;
         }
-        const float invstd = 1.0f / sqrtf(ln_block_sum<kLnThreads>(q, red, turn) / (float)C + eps);
-        if (threadIdx.x == 0 && save_mean != nullptr) {
-            save_mean[r] = mean;
-            save_invstd[r] = invstd;
+        team.sum<1>(&q);
+        const float invstd = 1.0f / sqrtf(q * p.inv_c + p.eps);
+        if (threadIdx.x == 0 && p.mean != nullptr) {
+            p.mean[r] = mean;
+            p.invstd[r] = invstd;
         }
-        for (int c = threadIdx.x; c < C; c += kLnThreads) {
-            const float v = (xr[c] - mean) * invstd * gamma[c] + beta[c];
-            y[(size_t)r * C + c] = v;
-            if (y16 != nullptr) y16[(size_t)r * C + c] = (uint16_t)ln_bf16(v);
+        for (int64_t c = threadIdx.x; c < C; c += kLnLong) {
+            const float v = (xr[c] - mean) * invstd * p.gamma[c] + p.beta[c];
+            p.y[(size_t)r * C + c] = v;
+            if (p.y16 != nullptr) p.y16[(size_t)r * C + c] = (uint16_t)ln_bf16(v);
         }
     }
 }
 
 // ---- backward ----------------------------------------------------------------------------------------------------------
-// Bound: HBM, 12 bytes an element (14 with the bfloat16 copy).  x and dy are read once: the same lanes hold the row while its
+// Bound: HBM, 12 bytes an element (14 with the bfloat16 copy): 65536 x 1024 152 us = 5.3 TB/s, 802816 x 64 115 us = 5.4 TB/s, ragged
+// rows 4.6-5.2 TB/s; a short call (5003 x 1537, 92 MB, 23 us) pays for two launches.  x and dy are read once: the same lanes hold the row while its
 // two sums are taken, and the lane that owns a column adds its dy xhat and dy over all rows it sees.  A workgroup walks many
 // rows and leaves one partial row of dgamma and one of dbeta, part[block][2][C]; ln_bwd_finish adds those in block order.
+struct LnBwdArgs {
+    const float *x, *dy, *gamma, *mean, *invstd;
+    float* dx;
+    uint16_t* dx16;
+    int rows, C;
+    float inv_c;
+    float* part;
+    bool stream;
+};
 
-// Rows of at most 64 V units, as ln_fwd_wave; T / L rows at a time.
-template <int T, int L, int V, int W>
-__global__ __launch_bounds__(T) void ln_bwd_wave(const float* __restrict__ x, const float* __restrict__ dy,
-                                                 const float* __restrict__ gamma, const float* __restrict__ mean,
-                                                 const float* __restrict__ invstd, float* __restrict__ dx,
-                                                 uint16_t* __restrict__ dx16, int rows, int C, float* __restrict__ part) {
-    __shared__ float red[T / 64][L * V * W];
-    const int s = threadIdx.x % L;
-    float gm[V][W], dg[V][W], db[V][W];
+// What a lane holds of a row: x and dy as loaded.
+template <int V>
+struct LnBwdRow {
+    float x[V][4], dy[V][4], mean, invstd;
+    template <bool kTiny>
+    __device__ __forceinline__ void load(const LnBwdArgs& p, int64_t r, const LnLane<V, kTiny>& u) {
+        const size_t at = (size_t)r * p.C;
+        mean = p.mean[r];
+        invstd = p.invstd[r];
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            u.load(p.x + at, j, x[j]);
+            u.load(p.dy + at, j, dy[j]);
+        }
+    }
+};
+
+// gamma of a lane's units, 0 in the places that a unit does not own: their g is 0 in the sums (or NaN, in a row that has one), their
+// dx is not written, their column sums are dropped.
+template <int V, bool kTiny>
+__device__ __forceinline__ void ln_gains(const LnBwdArgs& p, const LnLane<V, kTiny>& u, float (*gm)[4]) {
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-        const int c = (s + L * j) * W;
+        u.load(p.gamma, j, gm[j]);
 #pragma unroll
-        for (int e = 0; e < W; ++e) dg[j][e] = db[j][e] = gm[j][e] = 0.f;
-        if (c < C) ln_load<W>(gamma + c, gm[j]);
+        for (int e = 0; e < 4; ++e)
+            if (!u.own(j, e)) gm[j][e] = 0.f;
     }
+}
+
+// One row: its part of the column sums, and its dx.  `sum(float*)`: two sums over the row's lanes.
+template <int V, bool kTiny, typename Sum>
+__device__ __forceinline__ void ln_bwd_row(const LnBwdArgs& p, int64_t r, const LnLane<V, kTiny>& u, LnBwdRow<V>& w,
+                                           const float (*gm)[4], float (*dg)[4], float (*db)[4], Sum sum) {
+    float s[2] = {0.f, 0.f};
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const float xh = (w.x[j][e] - w.mean) * w.invstd, d = w.dy[j][e], g = d * gm[j][e];
+            dg[j][e] = fmaf(d, xh, dg[j][e]);
+            db[j][e] += d;
+            s[0] += g;
+            s[1] = fmaf(g, xh, s[1]);
+            w.x[j][e] = xh;
+            w.dy[j][e] = g;
+        }
+    sum(s);
+    const float c1 = s[0] * p.inv_c, c2 = s[1] * p.inv_c;
+    const size_t at = (size_t)r * p.C;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        float v[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = w.invstd * (w.dy[j][e] - c1 - w.x[j][e] * c2);
+        u.store(p.dx + at, j, v, p.stream);
+        if (p.dx16 != nullptr) u.store16(p.dx16 + at, j, v);
+    }
+}
+
+// Rows of at most L V units, T / L of them at a time.  Up to V = 6 the next row's loads are on their way while this row's sums are
+// taken (beyond there are no registers for it; after the last row that row is read once more rather than have a branch around
+// the loads).
+template <int T, int L, int V, bool kTiny = false>
+__global__ __launch_bounds__(T) void ln_bwd_wave(const LnBwdArgs p) {
+    constexpr bool kAhead = V <= 6;
+    __shared__ float red[T / 64][L * V * 4];
+    const int s = threadIdx.x % L, C = p.C;
+    const LnLane<V, kTiny> u(s, L, C);
+    float gm[V][4], dg[V][4], db[V][4];
+    ln_gains(p, u, gm);
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) dg[j][e] = db[j][e] = 0.f;
     const int step = gridDim.x * (T / L);
-    for (int64_t r = (int64_t)blockIdx.x * (T / L) + threadIdx.x / L; r < rows; r += step) {
-        const size_t at = (size_t)r * C;
-        const float m = mean[r], is = invstd[r];
-        float xh[V][W], g[V][W], s1 = 0.f, s2 = 0.f;
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-            const int c = (s + L * j) * W;
-            if (c < C) {
-                ln_load<W>(x + at + c, xh[j]);
-                ln_load<W>(dy + at + c, g[j]);
-            }
-        }
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-            const bool in = (s + L * j) * W < C;
-#pragma unroll
-            for (int e = 0; e < W; ++e) {
-                xh[j][e] = in ? (xh[j][e] - m) * is : 0.f;
-                const float d = in ? g[j][e] : 0.f;
-                dg[j][e] += d * xh[j][e];
-                db[j][e] += d;
-                g[j][e] = d * gm[j][e];
-                s1 += g[j][e];
-                s2 += g[j][e] * xh[j][e];
-            }
-        }
-        const float c1 = ln_group_sum<L>(s1) / (float)C, c2 = ln_group_sum<L>(s2) / (float)C;
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-            const int c = (s + L * j) * W;
-            if (c < C) {
-                float v[W];
-#pragma unroll
-                for (int e = 0; e < W; ++e) v[e] = is * (g[j][e] - c1 - xh[j][e] * c2);
-                ln_store<W>(dx + at + c, v);
-                if (dx16 != nullptr) ln_store16<W>(dx16 + at + c, v);
-            }
-        }
+    int64_t r = (int64_t)blockIdx.x * (T / L) + threadIdx.x / L;
+    LnBwdRow<V> next;
+    if (kAhead && r < p.rows) next.load(p, r, u);
+    while (r < p.rows) {
+        LnBwdRow<V> w;
+        if (kAhead) w = next;
+        else w.load(p, r, u);
+        const int64_t now = r;
+        r += step;
+        if (kAhead) next.load(p, r < p.rows ? r : now, u);
+        ln_bwd_row(p, now, u, w, gm, dg, db, [](float* a) {
+            a[0] = ln_group_sum<L>(a[0]);
+            a[1] = ln_group_sum<L>(a[1]);
+        });
     }
     // the rows of a wave, then the waves in order
-    float* out = part + (size_t)blockIdx.x * 2 * C;
+    float* out = p.part + (size_t)blockIdx.x * 2 * C;
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
 #pragma unroll
         for (int j = 0; j < V; ++j)
 #pragma unroll
-            for (int e = 0; e < W; ++e) {
+            for (int e = 0; e < 4; ++e) {
                 float v = k == 0 ? dg[j][e] : db[j][e];
 #pragma unroll
                 for (int o = L; o < 64; o <<= 1) v += __shfl_xor(v, o, 64);
-                if ((threadIdx.x & 63) < L) red[threadIdx.x >> 6][(s + L * j) * W + e] = v;
+                if ((threadIdx.x & 63) < L && u.own(j, e)) red[threadIdx.x >> 6][u.at(j) + e] = v;
             }
         __syncthreads();
         for (int c = threadIdx.x; c < C; c += T) {
@@ -318,168 +383,128 @@ __global__ __launch_bounds__(T) void ln_bwd_wave(const float* __restrict__ x, co
     }
 }
 
-// Longer rows, up to T V units: a row per workgroup.
-template <int T, int V, int W>
-__global__ __launch_bounds__(T) void ln_bwd_block(const float* __restrict__ x, const float* __restrict__ dy,
-                                                  const float* __restrict__ gamma, const float* __restrict__ mean,
-                                                  const float* __restrict__ invstd, float* __restrict__ dx,
-                                                  uint16_t* __restrict__ dx16, int rows, int C, float* __restrict__ part) {
-    __shared__ float red1[2][T / 64], red2[2][T / 64];
-    int turn = 0;
-    float dg[V][W], db[V][W];
+// Longer rows, up to blockDim V units: a row per workgroup.  Up to V = 4 with the next row on its way and gamma in registers.
+template <int T, int V>
+__global__ __launch_bounds__(T) void ln_bwd_block(const LnBwdArgs p) {
+    constexpr bool kAhead = V <= 4;
+    __shared__ float red[2][2][16];
+    LnTeam team(red);
+    const int C = p.C;
+    const LnLane<V> u(threadIdx.x, blockDim.x, C);
+    float gm[V][4], dg[V][4], db[V][4];
+    if (kAhead) ln_gains(p, u, gm);
 #pragma unroll
     for (int j = 0; j < V; ++j)
 #pragma unroll
-        for (int e = 0; e < W; ++e) dg[j][e] = db[j][e] = 0.f;
-    for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
-        const size_t at = (size_t)r * C;
-        const float m = mean[r], is = invstd[r];
-        float xh[V][W], g[V][W], s1 = 0.f, s2 = 0.f;
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-            const int c = (threadIdx.x + T * j) * W;
-            if (c < C) {
-                ln_load<W>(x + at + c, xh[j]);
-                ln_load<W>(dy + at + c, g[j]);
-            }
+        for (int e = 0; e < 4; ++e) dg[j][e] = db[j][e] = 0.f;
+    int64_t r = blockIdx.x;
+    LnBwdRow<V> next;
+    if (kAhead && r < p.rows) next.load(p, r, u);
+    while (r < p.rows) {
+        LnBwdRow<V> w;
+        if (kAhead) {
+            w = next;
+        } else {
+            w.load(p, r, u);
+            ln_gains(p, u, gm);
         }
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-            const int c = (threadIdx.x + T * j) * W;
-            float gm[W];
-            if (c < C) ln_load<W>(gamma + c, gm);
-#pragma unroll
-            for (int e = 0; e < W; ++e) {
-                xh[j][e] = c < C ? (xh[j][e] - m) * is : 0.f;
-                const float d = c < C ? g[j][e] : 0.f;
-                dg[j][e] += d * xh[j][e];
-                db[j][e] += d;
-                g[j][e] = c < C ? d * gm[e] : 0.f;
-                s1 += g[j][e];
-                s2 += g[j][e] * xh[j][e];
-            }
-        }
-        // (both sums behind one barrier; the slots are used in turn as in ln_block_sum)
-        s1 = ln_group_sum<64>(s1);
-        s2 = ln_group_sum<64>(s2);
-        if ((threadIdx.x & 63) == 0) {
-            red1[turn][threadIdx.x >> 6] = s1;
-            red2[turn][threadIdx.x >> 6] = s2;
-        }
-        __syncthreads();
-        s1 = red1[turn][0];
-        s2 = red2[turn][0];
-#pragma unroll
-        for (int w = 1; w < T / 64; ++w) {
-            s1 += red1[turn][w];
-            s2 += red2[turn][w];
-        }
-        turn ^= 1;
-        const float c1 = s1 / (float)C, c2 = s2 / (float)C;
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-            const int c = (threadIdx.x + T * j) * W;
-            if (c < C) {
-                float v[W];
-#pragma unroll
-                for (int e = 0; e < W; ++e) v[e] = is * (g[j][e] - c1 - xh[j][e] * c2);
-                ln_store<W>(dx + at + c, v);
-                if (dx16 != nullptr) ln_store16<W>(dx16 + at + c, v);
-            }
-        }
+        const int64_t now = r;
+        r += gridDim.x;
+        if (kAhead) next.load(p, r < p.rows ? r : now, u);
+        ln_bwd_row(p, now, u, w, gm, dg, db, [&](float* a) { team.sum<2>(a); });
     }
-    float* out = part + (size_t)blockIdx.x * 2 * C;
+    float* out = p.part + (size_t)blockIdx.x * 2 * C;
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-        const int c = (threadIdx.x + T * j) * W;
-        if (c < C) {
-            if (W == 4 && (reinterpret_cast<uintptr_t>(out) & 15) == 0) {
-                ln_store<W>(out + c, dg[j]);
-                ln_store<W>(out + C + c, db[j]);
-            } else {
-#pragma unroll
-                for (int e = 0; e < W; ++e) {
-                    out[c + e] = dg[j][e];
-                    out[C + c + e] = db[j][e];
-                }
-            }
-        }
+        u.store(out, j, dg[j], false);
+        u.store(out + C, j, db[j], false);
     }
 }
 
-// Rows of any length: the gradient of the rows in two passes, the column sums in a kernel of their own.
-__global__ __launch_bounds__(kLnThreads) void ln_bwd_rows(const float* __restrict__ x, const float* __restrict__ dy,
-                                                          const float* __restrict__ gamma, const float* __restrict__ mean,
-                                                          const float* __restrict__ invstd, float* __restrict__ dx,
-                                                          uint16_t* __restrict__ dx16, int rows, int C) {
-    __shared__ float red[2][kLnThreads / 64];
-    int turn = 0;
-    for (int r = blockIdx.x; r < rows; r += gridDim.x) {
+// Rows of any length: the gradient of the rows in two passes over each, the column sums in a kernel of their own.
+__global__ __launch_bounds__(kLnLong) void ln_bwd_rows(const LnBwdArgs p) {
+    __shared__ float red[2][2][16];
+    LnTeam team(red);
+    const int C = p.C;
+    for (int64_t r = blockIdx.x; r < p.rows; r += gridDim.x) {
         const size_t at = (size_t)r * C;
-        const float m = mean[r], is = invstd[r];
-        float s1 = 0.f, s2 = 0.f;
-        for (int c = threadIdx.x; c < C; c += kLnThreads) {
-            const float g = dy[at + c] * gamma[c];
-            s1 += g;
-            s2 += g * ((x[at + c] - m) * is);
+        const float m = p.mean[r], is = p.invstd[r];
+        float s[2] = {0.f, 0.f};
+        for (int64_t c = threadIdx.x; c < C; c += kLnLong) {
+            const float g = p.dy[at + c] * p.gamma[c];
+            s[0] += g;
+            s[1] += g * ((p.x[at + c] - m) * is);
         }
-        const float c1 = ln_block_sum<kLnThreads>(s1, red, turn) / (float)C;
-        const float c2 = ln_block_sum<kLnThreads>(s2, red, turn) / (float)C;
-        for (int c = threadIdx.x; c < C; c += kLnThreads) {
-            const float v = is * (dy[at + c] * gamma[c] - c1 - (x[at + c] - m) * is * c2);
-            dx[at + c] = v;
-            if (dx16 != nullptr) dx16[at + c] = (uint16_t)ln_bf16(v);
+        team.sum<2>(s);
+        const float c1 = s[0] * p.inv_c, c2 = s[1] * p.inv_c;
+        for (int64_t c = threadIdx.x; c < C; c += kLnLong) {
+            const float v = is * (p.dy[at + c] * p.gamma[c] - c1 - (p.x[at + c] - m) * is * c2);
+            p.dx[at + c] = v;
+            if (p.dx16 != nullptr) p.dx16[at + c] = (uint16_t)ln_bf16(v);
         }
     }
 }
 
 // Partial sums of dy xhat and dy over a run of rows: 64 columns x 4 row lanes per workgroup, part[run][2][C].
-__global__ __launch_bounds__(kLnThreads) void ln_bwd_columns(const float* __restrict__ x, const float* __restrict__ dy,
-                                                             const float* __restrict__ mean,
-                                                             const float* __restrict__ invstd, int rows, int C, int run,
-                                                             float* __restrict__ part) {
+__global__ __launch_bounds__(256) void ln_bwd_columns(const LnBwdArgs p, int run) {
     __shared__ float red[2][4][64];
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    const int c = blockIdx.x * 64 + lane;
-    const int beg = blockIdx.y * run, end = min(rows, beg + run);
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, C = p.C;
+    const int64_t c = (int64_t)blockIdx.x * 64 + lane;
+    const int beg = blockIdx.y * run, end = min(p.rows, beg + run);
     float a = 0.f, b = 0.f;
     if (c < C)
         for (int r = beg + w; r < end; r += 4) {
-            const float g = dy[(size_t)r * C + c];
-            a += g * ((x[(size_t)r * C + c] - mean[r]) * invstd[r]);
+            const float g = p.dy[(size_t)r * C + c];
+            a += g * ((p.x[(size_t)r * C + c] - p.mean[r]) * p.invstd[r]);
             b += g;
         }
     red[0][w][lane] = a;
     red[1][w][lane] = b;
     __syncthreads();
     if (w < 2 && c < C)
-        part[((size_t)blockIdx.y * 2 + w) * C + c] =
+        p.part[((size_t)blockIdx.y * 2 + w) * C + c] =
             (red[w][0][lane] + red[w][1][lane]) + (red[w][2][lane] + red[w][3][lane]);
 }
 
-// dgamma | dbeta = the partial rows part[block][2C], added in block order: 64 columns a workgroup, 16 lanes of blocks each.
+// dgamma | dbeta = the partial rows part[block][2C] added up: 32 columns (128 bytes of a row) a workgroup, 128 lanes of blocks
+// each, so that all of a lane's few loads are in flight at once; then the lanes by a tree.  Fixed order.
 __global__ __launch_bounds__(1024) void ln_bwd_finish(const float* __restrict__ part, int blocks, int C,
                                                       float* __restrict__ dgamma, float* __restrict__ dbeta) {
-    __shared__ float red[16][64];
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    const int64_t c = (int64_t)blockIdx.x * 64 + lane, C2 = 2 * (int64_t)C;
+    __shared__ float red[128][33];
+    const int unit = threadIdx.x & 7, w = threadIdx.x >> 3;
+    const int64_t c = ((int64_t)blockIdx.x * 8 + unit) * 4, C2 = 2 * (int64_t)C;
     float a[4] = {0.f, 0.f, 0.f, 0.f};
-    if (c < C2) {
-        int i = w;
-        for (; i + 48 < blocks; i += 64) {
+    if (c + 4 <= C2) {
+        for (int i0 = w; i0 < blocks; i0 += 512) {
+            ln_f4 v[4];
 #pragma unroll
-            for (int u = 0; u < 4; ++u) a[u] += part[(i + 16 * u) * C2 + c];
+            for (int k = 0; k < 4; ++k) {
+                const int i = i0 + 128 * k;
+                v[k] = i < blocks ? *reinterpret_cast<const ln_f4*>(part + i * C2 + c) : ln_f4{0.f, 0.f, 0.f, 0.f};
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) a[e] += v[k][e];
         }
-        for (; i < blocks; i += 16) a[0] += part[i * C2 + c];
-    }
-    red[w][lane] = (a[0] + a[1]) + (a[2] + a[3]);
-    __syncthreads();
-    if (w == 0 && c < C2) {
-        float v = red[0][lane];
+    } else {                                             // (the last two columns of an odd C)
+        for (int i = w; i < blocks; i += 128)
 #pragma unroll
-        for (int k = 1; k < 16; ++k) v += red[k][lane];
-        if (c < C) dgamma[c] = v;
-        else dbeta[c - C] = v;
+            for (int e = 0; e < 4; ++e) a[e] += c + e < C2 ? part[i * C2 + c + e] : 0.f;
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) red[w][unit * 4 + e] = a[e];
+    __syncthreads();
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const int col = wave * 2 + h;
+        const int64_t k = (int64_t)blockIdx.x * 32 + col;
+        const float v = ln_group_sum<64>(red[lane][col] + red[lane + 64][col]);
+        if (lane == 0 && k < C2) {
+            if (k < C) dgamma[k] = v;
+            else dbeta[k - C] = v;
+        }
     }
 }
 
@@ -488,70 +513,98 @@ static bool ln_apart(const void* a, const void* b, int64_t na, int64_t nb) {
     return p == nullptr || q == nullptr || p + na <= q || q + nb <= p;
 }
 
-static bool ln_vec4(int C, std::initializer_list<const void*> pointers) {
-    if (C % 4 != 0) return false;
-    for (const void* p : pointers)
-        if ((reinterpret_cast<uintptr_t>(p) & 15) != 0) return false;
-    return true;
+// How a row is laid over lanes: the way with the fewest idle places, and of those the one with the most lanes (802816 x 64 backward:
+// 16 lanes of one unit 114 us, 4 of four 123).  Up to 512 units (2048 columns) a row has L lanes of a wave, beyond a workgroup of
+// whole waves, as long as `most` units a lane allow; there, of equals, the fewest waves.
+// Idle places cost what used ones do: 65536 x 1028 forward took 200 us on 256 lanes of two units, half of them idle, where
+// 65536 x 1024 took 97.
+struct LnShape {
+    int lanes;                                           // of a wave; 0: a workgroup a row; -1: rows of any length
+    int v, threads;
+    bool tiny;
+};
+static LnShape ln_shape(int C, int most_threads, int most) {
+    const int units = cdiv(C, 4);
+    if (C < 4) return LnShape{4, 1, 0, true};
+    LnShape best{-1, 0, kLnLong, false};
+    if (units <= 512) {
+        for (int lanes = 64; lanes >= 4; lanes >>= 1) {
+            const int v = cdiv(units, lanes);
+            if (v <= (lanes == 64 ? 8 : 4) && (best.lanes < 0 || lanes * v < best.lanes * best.v)) best = LnShape{lanes, v, 0, false};
+        }
+        return best;
+    }
+    for (int v = 1; v <= most; ++v) {
+        const int threads = cdiv(cdiv(units, v), 64) * 64;
+        if (threads <= most_threads && (best.lanes < 0 || threads * v <= best.threads * best.v)) best = LnShape{0, v, threads, false};
+    }
+    return best;
 }
 
-typedef void (*LnFwd)(const float*, const float*, const float*, float*, float*, float*, uint16_t*, int, int, float);
+typedef void (*LnFwd)(const LnFwdArgs);
+typedef void (*LnBwd)(const LnBwdArgs);
 
-// The kernel for rows of `units` W-float units, its threads and the rows it takes at a time.
-template <int W>
-static LnFwd ln_fwd_kernel(int units, int* threads, int* rows_per_block) {
-    constexpr int F = 4 / W;                             // 4-byte units: four times as many of them for the same registers
-    *threads = 256;
-    const auto wave = [&](LnFwd k, int lanes) { *rows_per_block = 256 / lanes; return k; };
-    if (units <= 4) return wave(ln_fwd_wave<4, 1, W>, 4);
-    if (units <= 8) return wave(ln_fwd_wave<8, 1, W>, 8);
-    if (units <= 16) return wave(ln_fwd_wave<16, 1, W>, 16);
-    if (units <= 32) return wave(ln_fwd_wave<32, 1, W>, 32);
-    if (units <= 64) return wave(ln_fwd_wave<64, 1, W>, 64);
-    if (units <= 128) return wave(ln_fwd_wave<64, 2, W>, 64);
-    if (units <= 256) return wave(ln_fwd_wave<64, 4, W>, 64);
-    *rows_per_block = 1;
-    if (units <= 512 * F) return ln_fwd_block<256, 2 * F, W>;
-    if (units <= 1024 * F) return ln_fwd_block<256, 4 * F, W>;
-    if (units <= 2048 * F) return ln_fwd_block<256, 8 * F, W>;
-    *threads = 1024;
-    if (units <= 4096 * F) return ln_fwd_block<1024, 4 * F, W>;
-    if (units <= 8192 * F) return ln_fwd_block<1024, 8 * F, W>;
-    *threads = 256;
+template <int L>
+static LnFwd ln_fwd_wave_of(int v) {
+    static const LnFwd k[4] = {ln_fwd_wave<L, 1>, ln_fwd_wave<L, 2>, ln_fwd_wave<L, 3>, ln_fwd_wave<L, 4>};
+    return k[v - 1];
+}
+template <int T>
+static LnFwd ln_fwd_block_of(int v) {
+    static const LnFwd k[8] = {ln_fwd_block<T, 1>, ln_fwd_block<T, 2>, ln_fwd_block<T, 3>, ln_fwd_block<T, 4>,
+                               ln_fwd_block<T, 5>, ln_fwd_block<T, 6>, ln_fwd_block<T, 7>, ln_fwd_block<T, 8>};
+    return k[v - 1];
+}
+static LnFwd ln_fwd_kernel(const LnShape& s) {
+    static const LnFwd wide[4] = {ln_fwd_wave<64, 5>, ln_fwd_wave<64, 6>, ln_fwd_wave<64, 7>, ln_fwd_wave<64, 8>};
+    if (s.tiny) return ln_fwd_wave<4, 1, true>;
+    switch (s.lanes) {
+        case 4: return ln_fwd_wave_of<4>(s.v);
+        case 8: return ln_fwd_wave_of<8>(s.v);
+        case 16: return ln_fwd_wave_of<16>(s.v);
+        case 32: return ln_fwd_wave_of<32>(s.v);
+        case 64: return s.v > 4 ? wide[s.v - 5] : ln_fwd_wave_of<64>(s.v);
+        case 0: return s.threads <= 512 ? ln_fwd_block_of<512>(s.v) : ln_fwd_block_of<1024>(s.v);
+    }
     return ln_fwd_rows;
 }
 
-typedef void (*LnBwd)(const float*, const float*, const float*, const float*, const float*, float*, uint16_t*, int, int,
-                      float*);
+constexpr int kLnBwdWaveThreads = 512;
+template <int L>
+static LnBwd ln_bwd_wave_of(int v) {
+    constexpr int T = kLnBwdWaveThreads;
+    static const LnBwd k[4] = {ln_bwd_wave<T, L, 1>, ln_bwd_wave<T, L, 2>, ln_bwd_wave<T, L, 3>, ln_bwd_wave<T, L, 4>};
+    return k[v - 1];
+}
+static LnBwd ln_bwd_kernel(const LnShape& s) {
+    constexpr int T = kLnBwdWaveThreads;
+    static const LnBwd wide[4] = {ln_bwd_wave<T, 64, 5>, ln_bwd_wave<T, 64, 6>, ln_bwd_wave<T, 64, 7>, ln_bwd_wave<T, 64, 8>};
+    static const LnBwd block[8] = {ln_bwd_block<512, 1>, ln_bwd_block<512, 2>, ln_bwd_block<512, 3>, ln_bwd_block<512, 4>,
+                                   ln_bwd_block<512, 5>, ln_bwd_block<512, 6>, ln_bwd_block<512, 7>, ln_bwd_block<512, 8>};
+    if (s.tiny) return ln_bwd_wave<T, 4, 1, true>;
+    switch (s.lanes) {
+        case 4: return ln_bwd_wave_of<4>(s.v);
+        case 8: return ln_bwd_wave_of<8>(s.v);
+        case 16: return ln_bwd_wave_of<16>(s.v);
+        case 32: return ln_bwd_wave_of<32>(s.v);
+        case 64: return s.v > 4 ? wide[s.v - 5] : ln_bwd_wave_of<64>(s.v);
+        case 0: return s.threads <= 512 ? block[s.v - 1] : s.v == 6 ? ln_bwd_block<768, 6> : ln_bwd_block<768, 7>;
+    }
+    return ln_bwd_rows;
+}
 
-// As ln_fwd_kernel; `cap`: the most workgroups to launch.  NULL: rows too long for the registers of a workgroup.
-template <int W>
-static LnBwd ln_bwd_kernel(int units, int* threads, int* rows_per_block, int* cap) {
-    constexpr int F = 4 / W;
-    constexpr int T = 512;
-    *threads = T;
-    *cap = 512;
-    const auto wave = [&](LnBwd k, int lanes) { *rows_per_block = T / lanes; return k; };
-    if (units <= 4) return wave(ln_bwd_wave<T, 4, 1, W>, 4);
-    if (units <= 8) return wave(ln_bwd_wave<T, 8, 1, W>, 8);
-    if (units <= 16) return wave(ln_bwd_wave<T, 16, 1, W>, 16);
-    if (units <= 32) return wave(ln_bwd_wave<T, 32, 1, W>, 32);
-    if (units <= 64) return wave(ln_bwd_wave<T, 64, 1, W>, 64);
-    if (units <= 128) return wave(ln_bwd_wave<T, 64, 2, W>, 64);
-    if (units <= 256) return wave(ln_bwd_wave<T, 64, 4, W>, 64);
-    *rows_per_block = 1;
-    *threads = 256;
-    *cap = 768;
-    if (units <= 512 * F) return ln_bwd_block<256, 2 * F, W>;
-    if (units <= 1024 * F) return ln_bwd_block<256, 4 * F, W>;
-    *threads = 512;
-    *cap = 512;
-    if (units <= 2048 * F) return ln_bwd_block<512, 4 * F, W>;
-    *threads = 1024;
-    *cap = 256;
-    if (units <= 4096 * F) return ln_bwd_block<1024, 4 * F, W>;
-    *rows_per_block = 256;
-    return nullptr;
+// Backward: with the next row on its way where that fits 512 threads, else without; then 768 threads, whose 168 registers take up to
+// seven units.
+static LnShape ln_bwd_shape(int C) {
+    LnShape s = ln_shape(C, 512, 4);
+    if (s.lanes < 0) s = ln_shape(C, 512, 8);
+    if (s.lanes < 0) s = ln_shape(C, 768, 7);
+    return s;
+}
+static LnShape ln_fwd_shape(int C) {
+    LnShape s = ln_shape(C, 512, 8);
+    if (s.lanes < 0) s = ln_shape(C, 1024, 8);
+    return s;
 }
 
 // The arguments are checked before the context: a bad call is refused alike with and without a GPU.
@@ -565,12 +618,13 @@ static int ln_fwd_impl(const float* x, const float* gamma, const float* beta, fl
     AETH_CHECK_ARG(ln_apart(x, y, 4 * n, 4 * n) && ln_apart(x, y16, 4 * n, 2 * n) && ln_apart(y, y16, 4 * n, 2 * n));
     AETH_REQUIRE_INIT();
     if (rows == 0) return AETH_OK;
-    int threads, per;
-    const LnFwd kernel = ln_vec4(C, {x, gamma, beta, y, y16}) ? ln_fwd_kernel<4>(C / 4, &threads, &per)
-                                                              : ln_fwd_kernel<1>(C, &threads, &per);
-    const int want = cdiv(rows, per);
-    hipLaunchKernelGGL(kernel, dim3(want < kLnGrid ? want : kLnGrid), dim3(threads), 0, ctx().stream, x, gamma, beta, save_mean,
-                       save_invstd, y, y16, rows, C, eps);
+    const LnShape s = ln_fwd_shape(C);
+    const int threads = s.lanes > 0 ? 256 : s.threads, turns = s.lanes > 0 ? cdiv(rows, 256 / s.lanes) : rows;
+    // workgroups that walk the rows, 1024 threads a CU: 16384 x 8192 took 204 us with 1024 workgroups of 256 threads, 207 with
+    // 4096, 218 with one a row; pixels x64 with twin 95.7, 98.6, 98.9
+    const int cap = 256 * 1024 / threads;
+    const LnFwdArgs p{x, gamma, beta, save_mean, save_invstd, y, y16, rows, C, 1.0f / (float)C, eps, 4 * n >= kLnStreamBytes};
+    hipLaunchKernelGGL(ln_fwd_kernel(s), dim3(turns < cap ? turns : cap), dim3(threads), 0, ctx().stream, p);
     AETH_LAUNCH_CHECK();
     return AETH_OK;
 }
@@ -584,29 +638,34 @@ static int ln_bwd_impl(const float* x, const float* dy, const float* gamma, cons
     AETH_CHECK_ARG(ln_apart(x, dx16, 4 * n, 2 * n) && ln_apart(dy, dx16, 4 * n, 2 * n) && ln_apart(dx, dx16, 4 * n, 2 * n));
     AETH_REQUIRE_INIT();
     hipStream_t st = ctx().stream;
-    int threads, per, cap, blocks = 0;
+    int blocks = 0;
     void* ws = nullptr;
     if (rows > 0) {
-        const LnBwd kernel = ln_vec4(C, {x, dy, gamma, dx, dx16}) ? ln_bwd_kernel<4>(C / 4, &threads, &per, &cap)
-                                                                  : ln_bwd_kernel<1>(C, &threads, &per, &cap);
-        blocks = cdiv(rows, per) < cap ? cdiv(rows, per) : cap;
-        const int run = cdiv(rows, blocks);
-        if (kernel == nullptr) blocks = cdiv(rows, run);
+        const LnShape s = ln_bwd_shape(C);
+        int threads = s.threads, turns = rows, cap;
+        if (s.lanes > 0) {
+            threads = kLnBwdWaveThreads;
+            turns = cdiv(rows, threads / s.lanes);
+            cap = 256;                                   // (pixels x64 with twin: 512 workgroups 143 us, 256 129)
+        } else {
+            // whole workgroups a CU, 512 threads of them (16384 x 5000: 182 us with 512 threads a CU, 193 with 640 and 768, 197 with
+            // 1024; 4096 x 16384: 171, 171, 170, 183); more leave more partial rows, a part of one leaves CUs idle
+            cap = s.lanes < 0 ? 64 : 256 * (threads < 512 ? 512 / threads : 1);
+        }
+        // as many workgroups as are needed for each to take no more rows than with `cap` of them
+        const int run = cdiv(turns, cap);
+        blocks = cdiv(turns, run);
         const int rc = workspace((int64_t)2 * blocks * C * sizeof(float), &ws);
         if (rc) return rc;
-        if (kernel != nullptr) {
-            hipLaunchKernelGGL(kernel, dim3(blocks), dim3(threads), 0, st, x, dy, gamma, mean, invstd, dx, dx16, rows, C,
-                               (float*)ws);
-        } else {
-            hipLaunchKernelGGL(ln_bwd_rows, dim3(rows < kLnGrid ? rows : kLnGrid), dim3(kLnThreads), 0, st, x, dy, gamma, mean,
-                               invstd, dx, dx16, rows, C);
-            AETH_LAUNCH_CHECK();
-            hipLaunchKernelGGL(ln_bwd_columns, dim3(cdiv(C, 64), blocks), dim3(kLnThreads), 0, st, x, dy, mean, invstd, rows, C,
-                               run, (float*)ws);
-        }
+        const LnBwdArgs p{x, dy, gamma, mean, invstd, dx, dx16, rows, C, 1.0f / (float)C, (float*)ws, 4 * n >= kLnStreamBytes};
+        hipLaunchKernelGGL(ln_bwd_kernel(s), dim3(s.lanes < 0 ? (rows < 4096 ? rows : 4096) : blocks), dim3(threads), 0, st, p);
         AETH_LAUNCH_CHECK();
+        if (s.lanes < 0) {
+            hipLaunchKernelGGL(ln_bwd_columns, dim3(cdiv(C, 64), blocks), dim3(256), 0, st, p, run);
+            AETH_LAUNCH_CHECK();
+        }
     }
-    hipLaunchKernelGGL(ln_bwd_finish, dim3(cdiv(2 * (int64_t)C, 64)), dim3(1024), 0, st, (const float*)ws, blocks, C, dgamma, dbeta);
+    hipLaunchKernelGGL(ln_bwd_finish, dim3(cdiv(2 * (int64_t)C, 32)), dim3(1024), 0, st, (const float*)ws, blocks, C, dgamma, dbeta);
     AETH_LAUNCH_CHECK();
     return AETH_OK;
 }
