@@ -7,161 +7,246 @@
 //
 // Every singular value s of X goes to p(s) = a s + b s^3 + c s^5; from s <= 1 (the norm bounds them) all stay below 1.21 and
 // those that are not tiny end in about [0.7, 1.2]: u's singular vectors with singular values near one.
-#include "common.h"
+#include "split_gemm.h"
 
 #include <math.h>
 
 namespace aeth {
 
-constexpr float kNsA = 3.4445f, kNsB = -4.7750f, kNsC = 2.0315f;
-constexpr int kMuonMax = 32;
-constexpr int kNormBlocks = 256;
-
-// One matrix of a call.  g is the update itself where m is NULL (orthogonalisation alone).
+// One matrix of a call.  mom == NULL: grad is the update itself (orthogonalisation alone, written to out).
 struct MuonMatrix {
-    float* theta;       // the weights; NULL: write X to out
+    float* theta;
     const float* grad;
     float* mom;
     float* out;
     int rows, cols;
-    int m, n;           // the shorter and the longer side
+    float gain;
 };
 
-__device__ __forceinline__ double wave_sum(double v) {
+struct MuonTable {
+    int count;
+    MuonMatrix t[kMuonMax];
+    int parts[kMuonMax];                                 // workgroups of muon_momentum
+    int first[kMuonMax];                                 // first workgroup of muon_split
+    char *same[kMuonMax], *turned[kMuonMax];             // X in the matrix's own orientation and transposed
+    double* sums;                                        // [count][kMuonParts]
+};
+typedef const MuonTable __attribute__((address_space(4)))* muon_table_ptr;
+
+__device__ __forceinline__ double muon_block_sum(double v, double* red) {
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
-    return v;
-}
-
-__device__ __forceinline__ double block_sum(double v, double* red) {
-    v = wave_sum(v);
-    __syncthreads();
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
     __syncthreads();
     return (red[0] + red[1]) + (red[2] + red[3]);
 }
 
-// m <- mu m + g and the partial sums of u^2.  They are 64-bit: no gradient overflows or vanishes in the square.
-__global__ __launch_bounds__(256) void muon_momentum(MuonMatrix t, float mu, int nesterov, double* __restrict__ part) {
+// The update u from a gradient and the new momentum.
+__device__ __forceinline__ float muon_update(float g, float m, float mu, int nesterov) { return nesterov ? fmaf(mu, m, g) : m; }
+
+// m <- mu m + g and the partial sums of u^2, blockIdx.y = matrix.  They are 64-bit: no gradient overflows or vanishes in the square.
+// Bound: HBM, 12 bytes an element.
+__global__ __launch_bounds__(256) void muon_momentum(const MuonTable tb, float mu, int nesterov) {
     __shared__ double red[4];
-    const int64_t n = (int64_t)t.rows * t.cols;
+    const muon_table_ptr args = (muon_table_ptr)__builtin_amdgcn_kernarg_segment_ptr();
+    const int k = blockIdx.y, parts = args->parts[k];
+    if ((int)blockIdx.x >= parts) return;
+    const float* __restrict__ grad = args->t[k].grad;
+    float* __restrict__ mom = args->t[k].mom;
+    const int64_t n = (int64_t)args->t[k].rows * args->t[k].cols, n4 = n / 4, step = (int64_t)parts * 256;
+    typedef float f4u __attribute__((ext_vector_type(4), aligned(4)));
     double s = 0.0;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
-        float u = t.grad[i];
-        if (t.mom != nullptr) {
-            const float g = u;
-            const float v = mu * t.mom[i] + g;
-            t.mom[i] = v;
-            u = nesterov ? g + mu * v : v;
-        }
+    const auto one = [&](float g, float m) {
+        const float u = mom != nullptr ? muon_update(g, m, mu, nesterov) : g;
         s += (double)u * (double)u;
+    };
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n4; i += step) {
+        const f4u g = *reinterpret_cast<const f4u*>(grad + 4 * i);
+        f4u m = {0.f, 0.f, 0.f, 0.f};
+        if (mom != nullptr) {
+            m = *reinterpret_cast<const f4u*>(mom + 4 * i);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) m[e] = fmaf(mu, m[e], g[e]);
+            *reinterpret_cast<f4u*>(mom + 4 * i) = m;
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) one(g[e], m[e]);
     }
-    s = block_sum(s, red);
-    if (threadIdx.x == 0) part[blockIdx.x] = s;
+    if (blockIdx.x == 0 && threadIdx.x < n - 4 * n4) {
+        const int64_t i = 4 * n4 + threadIdx.x;
+        float m = 0.f;
+        if (mom != nullptr) mom[i] = m = fmaf(mu, mom[i], grad[i]);
+        one(grad[i], m);
+    }
+    s = muon_block_sum(s, red);
+    if (threadIdx.x == 0) args->sums[k * kMuonParts + blockIdx.x] = s;
 }
 
-// X = u / |u|, transposed to [m][n] where the matrix is tall
-__global__ __launch_bounds__(256) void muon_normalise(MuonMatrix t, float mu, int nesterov, const double* __restrict__ part,
-                                                      int parts, float* __restrict__ X) {
+// X = u / |u| and its transpose as float16 halves, a 32 x 32 block a wave; padding becomes 0.
+// Bound: HBM, 8 bytes read and 8 written an element.
+__global__ __launch_bounds__(256) void muon_split(const MuonTable tb, float mu, int nesterov) {
     __shared__ double red[4];
-    const double sum = block_sum((int)threadIdx.x < parts ? part[threadIdx.x] : 0.0, red);
-    const double inv = sum != 0.0 ? 1.0 / sqrt(sum) : 0.0;
-    const int64_t n = (int64_t)t.rows * t.cols;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
-        float u = t.grad[i];
-        if (t.mom != nullptr) u = nesterov ? u + mu * t.mom[i] : t.mom[i];
-        const int64_t r = i / t.cols, c = i % t.cols;
-        X[t.rows <= t.cols ? i : c * t.rows + r] = (float)((double)u * inv);
-    }
-}
-
-// out = alpha R + beta P Q (R may be NULL), or P Q^T: 64 x 64 per workgroup, 4 x 4 per thread, slabs of 16 through LDS
-template <bool kTransposed>
-__global__ __launch_bounds__(256) void muon_product(const float* __restrict__ P, const float* __restrict__ Q,
-                                                    const float* __restrict__ R, float* __restrict__ out, int M, int N,
-                                                    int K, float alpha, float beta) {
-    __shared__ float p[16][65], q[16][65];
-    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-    const int i0 = blockIdx.y * 64, j0 = blockIdx.x * 64;
-    float acc[4][4] = {};
-    for (int k0 = 0; k0 < K; k0 += 16) {
-        for (int e = threadIdx.x; e < 1024; e += 256) {
-            const int k = e & 15, r = e >> 4;
-            p[k][r] = i0 + r < M && k0 + k < K ? P[(size_t)(i0 + r) * K + k0 + k] : 0.f;
-            if (kTransposed) {
-                q[k][r] = j0 + r < N && k0 + k < K ? Q[(size_t)(j0 + r) * K + k0 + k] : 0.f;
-            } else {
-                const int kk = e >> 6, c = e & 63;
-                q[kk][c] = j0 + c < N && k0 + kk < K ? Q[(size_t)(k0 + kk) * N + j0 + c] : 0.f;
-            }
+    __shared__ float blocks[4][32][33];
+    const muon_table_ptr args = (muon_table_ptr)__builtin_amdgcn_kernarg_segment_ptr();
+    int k = 0;
+    while (k + 1 < tb.count && (int)blockIdx.x >= args->first[k + 1]) ++k;
+    const double sum = muon_block_sum((int)threadIdx.x < args->parts[k] ? args->sums[k * kMuonParts + threadIdx.x] : 0.0, red);
+    const double inv = sum != 0.0 ? (double)kScaleX / sqrt(sum) : 0.0;
+    const float* __restrict__ grad = args->t[k].grad;
+    const float* __restrict__ mom = args->t[k].mom;
+    const int rows = args->t[k].rows, cols = args->t[k].cols;
+    const int64_t rp = muon_pad(rows), cp = muon_pad(cols), across = cp / 32;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, l32 = lane & 31, lh = lane >> 5;
+    const int64_t b = ((int64_t)blockIdx.x - args->first[k]) * 4 + wave;
+    if (b >= rp / 32 * across) return;
+    const int64_t r = b / across * 32, c = b % across * 32;
+    float(*blk)[33] = blocks[wave];
+#pragma unroll
+    for (int v = 0; v < 16; ++v) {
+        const int64_t y = r + 2 * v + lh, x = c + l32;
+        float u = 0.f;
+        if (y < rows && x < cols) {
+            u = grad[y * cols + x];
+            if (mom != nullptr) u = muon_update(u, mom[y * cols + x], mu, nesterov);
         }
-        __syncthreads();
-#pragma unroll
-        for (int k = 0; k < 16; ++k)
-#pragma unroll
-            for (int a = 0; a < 4; ++a)
-#pragma unroll
-                for (int b = 0; b < 4; ++b) acc[a][b] += p[k][ty + 16 * a] * q[k][tx + 16 * b];
-        __syncthreads();
+        blk[2 * v + lh][l32] = (float)((double)u * inv);
     }
-    for (int a = 0; a < 4; ++a)
-        for (int b = 0; b < 4; ++b) {
-            const int i = i0 + ty + 16 * a, j = j0 + tx + 16 * b;
-            if (i >= M || j >= N) continue;
-            const size_t at = (size_t)i * N + j;
-            out[at] = (R != nullptr ? alpha * R[at] : 0.f) + beta * acc[a][b];
+    __builtin_amdgcn_wave_barrier();
+    char* same = args->same[k] + (size_t)(r + l32) * cp * 4 + (size_t)(c / 32) * 128 + 32 * lh;
+    char* turned = args->turned[k] + (size_t)(c + l32) * rp * 4 + (size_t)(r / 32) * 128 + 32 * lh;
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+        half8 h, l, ht, lt;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            _Float16 x, y;
+            split_half(blk[l32][16 * lh + 8 * q + e], x, y);
+            h[e] = x;
+            l[e] = y;
+            split_half(blk[16 * lh + 8 * q + e][l32], x, y);
+            ht[e] = x;
+            lt[e] = y;
         }
-}
-
-// theta <- theta (1 - lr wd) - lr gain X, or out = X
-__global__ __launch_bounds__(256) void muon_apply(MuonMatrix t, const float* __restrict__ X, float lr,
-                                                  const double* __restrict__ state, float wd, float gain) {
-    if (state != nullptr) lr = (float)state[3];
-    const float keep = 1.0f - lr * wd, step = lr * gain;
-    const int64_t n = (int64_t)t.rows * t.cols;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
-        const int64_t r = i / t.cols, c = i % t.cols;
-        const float o = X[t.rows <= t.cols ? i : c * t.rows + r];
-        if (t.theta != nullptr) t.theta[i] = keep * t.theta[i] - step * o;
-        else t.out[i] = o;
+        *reinterpret_cast<half8*>(same + 16 * q) = h;
+        *reinterpret_cast<half8*>(same + 16 * q + 64) = l;
+        *reinterpret_cast<half8*>(turned + 16 * q) = ht;
+        *reinterpret_cast<half8*>(turned + 16 * q + 64) = lt;
     }
 }
 
-static int muon_matrix(const MuonMatrix& t, float lr, const double* state, float mu, int nesterov, float wd, int steps) {
-    const int64_t m = t.m, n = t.n;
-    void* ws;
-    const int rc = workspace((2 * m * n + 2 * m * m) * (int64_t)sizeof(float) + kNormBlocks * (int64_t)sizeof(double), &ws);
-    if (rc) return rc;
-    double* part = (double*)ws;
-    float* X = (float*)(part + kNormBlocks);
-    float* Y = X + m * n;
-    float* A = Y + m * n;
-    float* B = A + m * m;
-    hipStream_t st = ctx().stream;
-    const int64_t size = m * n;
-    const int blocks = size > 4096 * kNormBlocks ? kNormBlocks : cdiv(size, 4096);
-    hipLaunchKernelGGL(muon_momentum, dim3(blocks), dim3(256), 0, st, t, mu, nesterov, part);
-    AETH_LAUNCH_CHECK();
-    hipLaunchKernelGGL(muon_normalise, dim3(cdiv(size, 1024) < 4096 ? cdiv(size, 1024) : 4096), dim3(256), 0, st, t, mu,
-                       nesterov, part, blocks, X);
-    AETH_LAUNCH_CHECK();
-    const dim3 small(cdiv(m, 64), cdiv(m, 64)), wide(cdiv(n, 64), cdiv(m, 64));
-    for (int s = 0; s < steps; ++s) {
-        hipLaunchKernelGGL((muon_product<true>), small, dim3(256), 0, st, X, X, nullptr, A, t.m, t.m, t.n, 0.f, 1.f);
-        AETH_LAUNCH_CHECK();
-        hipLaunchKernelGGL((muon_product<false>), small, dim3(256), 0, st, A, A, A, B, t.m, t.m, t.m, kNsB, kNsC);
-        AETH_LAUNCH_CHECK();
-        hipLaunchKernelGGL((muon_product<false>), wide, dim3(256), 0, st, B, X, X, Y, t.m, t.n, t.m, kNsA, 1.f);
-        AETH_LAUNCH_CHECK();
-        float* swap = X;
-        X = Y;
-        Y = swap;
+// One launch for one product of every matrix, in tiles of BM x BN.
+template <int BM, int BN, int WM, int WN, int NBUF, int USE>
+static int muon_launch(SplitTable tb, float lr, const double* state, float wd) {
+    constexpr bool kSym = USE == kSplitGram || USE == kSplitPoly;
+    int64_t tiles = 0;
+    for (int i = 0; i < tb.count; ++i) {
+        tb.p[i].first = (int)tiles;
+        tb.p[i].tm = cdiv(tb.p[i].M, BM);
+        tb.p[i].tn = cdiv(tb.p[i].N, BN);
+        tiles += muon_tiles(tb.p[i].M, tb.p[i].N, BM, BN, kSym);
     }
-    const float gain = t.cols > t.rows ? sqrtf((float)t.cols / (float)t.rows) : 1.f;
-    hipLaunchKernelGGL(muon_apply, dim3(cdiv(size, 1024) < 4096 ? cdiv(size, 1024) : 4096), dim3(256), 0, st, t, X, lr, state,
-                       wd, gain);
+    hipLaunchKernelGGL((split_product<BM, BN, WM, WN, NBUF, USE>), dim3((unsigned)tiles), dim3(64 * (BM / WM) * (BN / WN)), 0,
+                       ctx().stream, tb, lr, state, wd);
     AETH_LAUNCH_CHECK();
     return AETH_OK;
+}
+
+template <int USE>
+static int muon_product(const SplitTable& tb, float lr, const double* state, float wd) {
+    constexpr bool kSym = USE == kSplitGram || USE == kSplitPoly;
+    int64_t tiles = 0;
+    for (int i = 0; i < tb.count; ++i) tiles += muon_tiles(tb.p[i].M, tb.p[i].N, 128, 128, kSym);
+    if (tiles >= 256) return muon_launch<128, 128, 64, 64, 2, USE>(tb, lr, state, wd);
+    return muon_launch<64, 64, 32, 32, 4, USE>(tb, lr, state, wd);
+}
+
+// The whole update of at most kMuonMax matrices that share the workspace.
+static int muon_group(const MuonMatrix* t, int count, float lr, const double* state, float mu, int nesterov, float wd, int steps) {
+    MuonTable tb = {};
+    SplitTable gram = {}, poly = {}, step[2] = {}, apply = {};
+    MuonLayout at[kMuonMax];
+    int64_t bytes = (int64_t)count * kMuonParts * sizeof(double), blocks = 0;
+    int parts = 1;
+    tb.count = gram.count = poly.count = step[0].count = step[1].count = apply.count = count;
+    for (int i = 0; i < count; ++i) {
+        const int m = t[i].rows < t[i].cols ? t[i].rows : t[i].cols, n = t[i].rows < t[i].cols ? t[i].cols : t[i].rows;
+        at[i] = muon_layout(m, n, bytes);
+        bytes = at[i].end;
+        const int64_t size = (int64_t)m * n;
+        tb.t[i] = t[i];
+        tb.parts[i] = size > 4096 * (int64_t)kMuonParts ? kMuonParts : cdiv(size, 4096);
+        if (tb.parts[i] > parts) parts = tb.parts[i];
+        tb.first[i] = (int)blocks;
+        blocks += cdiv(at[i].mp / 32 * (at[i].np / 32), 4);
+    }
+    void* ws;
+    const int rc = workspace(bytes, &ws);
+    if (rc) return rc;
+    char* base = static_cast<char*>(ws);
+    tb.sums = static_cast<double*>(ws);
+    for (int i = 0; i < count; ++i) {
+        char *x = base + at[i].x, *xt[2] = {base + at[i].xt0, base + at[i].xt1}, *a = base + at[i].a, *b = base + at[i].b;
+        const bool tall = t[i].rows > t[i].cols;
+        const int mp = (int)at[i].mp, np = (int)at[i].np;
+        tb.same[i] = tall ? xt[0] : x;
+        tb.turned[i] = tall ? x : xt[0];
+        SplitProduct p = {};
+        p.rows = t[i].rows;
+        p.cols = t[i].cols;
+        p.theta = t[i].theta;
+        p.out = t[i].out;
+        p.gain = t[i].gain;
+        p.P = p.Q = x, p.D1 = a, p.M = p.N = mp, p.K = np;
+        gram.p[i] = p;
+        p.P = p.Q = p.A = a, p.D1 = b, p.K = mp;
+        poly.p[i] = p;
+        for (int s = 0; s < 2; ++s) {
+            p.P = b, p.Q = xt[s], p.D1 = x, p.D2 = xt[1 - s], p.M = mp, p.N = np;
+            step[s].p[i] = p;
+        }
+        // the last product comes out in the weights' own orientation: X = B X, or its transpose Xt B (B is symmetric)
+        const char* last = xt[(steps - 1) & 1];
+        p.P = tall ? last : b, p.Q = tall ? b : last, p.M = tall ? np : mp, p.N = tall ? mp : np;
+        apply.p[i] = p;
+    }
+    hipStream_t st = ctx().stream;
+    hipLaunchKernelGGL(muon_momentum, dim3(parts, count), dim3(256), 0, st, tb, mu, nesterov);
+    AETH_LAUNCH_CHECK();
+    hipLaunchKernelGGL(muon_split, dim3((unsigned)blocks), dim3(256), 0, st, tb, mu, nesterov);
+    AETH_LAUNCH_CHECK();
+    for (int s = 0; s < steps; ++s) {
+        int e = muon_product<kSplitGram>(gram, lr, state, wd);
+        if (e == AETH_OK) e = muon_product<kSplitPoly>(poly, lr, state, wd);
+        if (e == AETH_OK)
+            e = s + 1 < steps ? muon_product<kSplitStep>(step[s & 1], lr, state, wd) : muon_product<kSplitApply>(apply, lr, state, wd);
+        if (e) return e;
+    }
+    return AETH_OK;
+}
+
+// Matrices whose buffers together pass this go out in several groups, one after the other.
+constexpr int64_t kMuonWorkspace = (int64_t)4 << 30;
+
+static int muon_run(MuonMatrix* t, int count, float lr, const double* state, float mu, int nesterov, float wd, int steps) {
+    for (int i = 0; i < count;) {
+        int64_t bytes = 0;
+        int k = 0;
+        while (i + k < count) {
+            const MuonMatrix& x = t[i + k];
+            const int64_t more = muon_layout(x.rows < x.cols ? x.rows : x.cols, x.rows < x.cols ? x.cols : x.rows, 0).end;
+            if (k > 0 && bytes + more > kMuonWorkspace) break;
+            bytes += more;
+            ++k;
+        }
+        const int rc = muon_group(t + i, k, lr, state, mu, nesterov, wd, steps);
+        if (rc) return rc;
+        i += k;
+    }
+    return AETH_OK;
+}
+
+static bool muon_size(int rows, int cols) {
+    return rows >= 0 && cols >= 0 && rows <= kMuonLongest && cols <= kMuonLongest && (int64_t)rows * cols < ((int64_t)1 << 31);
 }
 
 static bool muon_apart(const void* a, int64_t na, const void* b, int64_t nb) {
@@ -183,11 +268,11 @@ static int muon_multi_impl(const char* fn, int count, float* const* theta, const
     int k = 0;
     for (int i = 0; i < count; ++i) {
         const int r = rows[i], c = cols[i];
-        if (r < 0 || c < 0 || (int64_t)r * c >= ((int64_t)1 << 31))
-            return fail(AETH_E_INVALID, "%s: matrix %d is %d x %d", fn, i, r, c);
+        if (!muon_size(r, c))
+            return fail(AETH_E_INVALID, "%s: matrix %d is %d x %d (sides of at most %d, below 2^31 elements)", fn, i, r, c, kMuonLongest);
         if (r == 0 || c == 0) continue;
         if (!theta[i] || !grad[i] || !mom[i]) return fail(AETH_E_INVALID, "%s: matrix %d has a NULL tensor", fn, i);
-        t[k++] = MuonMatrix{theta[i], grad[i], mom[i], nullptr, r, c, r < c ? r : c, r < c ? c : r};
+        t[k++] = MuonMatrix{theta[i], grad[i], mom[i], nullptr, r, c, c > r ? sqrtf((float)c / (float)r) : 1.f};
     }
     // what is written (weights, momentum) may overlap nothing else of the call
     for (int i = 0; i < k; ++i) {
@@ -201,11 +286,7 @@ static int muon_multi_impl(const char* fn, int count, float* const* theta, const
         }
     }
     if (!ctx().ready) return fail(AETH_E_STATE, "%s: aeth_init has not been called", fn);
-    for (int i = 0; i < k; ++i) {
-        const int rc = muon_matrix(t[i], lr, state, mu, nesterov, wd, steps);
-        if (rc) return rc;
-    }
-    return AETH_OK;
+    return muon_run(t, k, lr, state, mu, nesterov, wd, steps);
 }
 
 }  // namespace aeth
@@ -215,14 +296,14 @@ using namespace aeth;
 extern "C" {
 
 int aeth_newton_schulz_f32(const float* g, float* o, int rows, int cols, int steps) {
-    AETH_CHECK_ARG(rows >= 0 && cols >= 0 && (int64_t)rows * cols < ((int64_t)1 << 31));
+    AETH_CHECK_ARG(muon_size(rows, cols));
     AETH_CHECK_ARG(steps >= 1 && steps <= 100);
     const int64_t bytes = (int64_t)rows * cols * 4;
     AETH_CHECK_ARG(bytes == 0 || (g && o && muon_apart(g, bytes, o, bytes)));
     AETH_REQUIRE_INIT();
     if (bytes == 0) return AETH_OK;
-    const MuonMatrix t{nullptr, g, nullptr, o, rows, cols, rows < cols ? rows : cols, rows < cols ? cols : rows};
-    return muon_matrix(t, 0.f, nullptr, 0.f, 0, 0.f, steps);
+    MuonMatrix t{nullptr, g, nullptr, o, rows, cols, 1.f};
+    return muon_run(&t, 1, 0.f, nullptr, 0.f, 0, 0.f, steps);
 }
 
 int aeth_muon_multi_f32(int count, float* const* host_theta, const float* const* host_grad, float* const* host_m,

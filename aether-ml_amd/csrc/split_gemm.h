@@ -1,0 +1,268 @@
+// Products of matrices whose elements are held as two float16 halves.
+//
+// x = hi + lo with hi = float16(x) and lo = float16(x - hi): 22 bits of x where neither half leaves float16's normal range, for
+// which every matrix is scaled by a power of two (kScale*).  hi.hi + hi.lo + lo.hi is x y up to 2^-22 of |x y| (the product of
+// the low halves is left out), each of the three a float16 MFMA with float32 accumulation.  Three float16 products take 0.19 of the
+// time of one float32 MFMA product of the same size at their peaks (2.5 PFLOP/s and 157 TFLOP/s), and are closer to it than
+// float32 sums of this length are to each other.
+#pragma once
+
+#include "conv_common.h"
+#include "muon_plan.h"
+
+namespace aeth {
+
+typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+typedef _Float16 half4 __attribute__((ext_vector_type(4)));
+
+// What a product's result becomes.
+enum SplitUse {
+    kSplitGram,          // D1 = P Q^T, symmetric
+    kSplitPoly,          // D1 = a I + b A + c P Q^T, symmetric (P = Q = A)
+    kSplitStep,          // D1 = P Q^T and D2 its transpose
+    kSplitApply,         // theta <- keep theta - step P Q^T, or out = P Q^T; float32, [rows][cols]
+};
+
+struct SplitProduct {
+    const char *P, *Q, *A;
+    char *D1, *D2;
+    float *theta, *out;
+    int M, N, K;         // padded: rows of P, rows of Q, their columns
+    int rows, cols;      // of theta
+    int first;           // this product's first tile
+    int tm, tn;          // tiles down and across
+    float gain;
+};
+
+struct SplitTable {
+    int count;
+    SplitProduct p[kMuonMax];
+};
+
+// Scales of the stored halves: X's elements are at most 1.21 (the step's polynomial maps [0, 1.21] into itself), A = X X^T's at most
+// 1.47, the polynomial's a I + b A + c A^2 at most 3.45: all below 65504 times their scale's inverse.
+constexpr float kScaleX = 32768.f, kScaleA = 32768.f, kScaleB = 16384.f;
+constexpr float kNsA = 3.4445f, kNsB = -4.7750f, kNsC = 2.0315f;
+
+__device__ __forceinline__ void split_half(float v, _Float16& hi, _Float16& lo) {
+    hi = (_Float16)v;
+    lo = (_Float16)(v - (float)hi);
+}
+
+template <int N>
+__device__ __forceinline__ void wait_loads() {           // at most N of this wave's loads are still on their way; its LDS reads are done
+    static_assert(N < 64, "vmcnt has six bits");
+    __builtin_amdgcn_s_waitcnt((N & 15) | (7 << 4) | (0 << 8) | ((N >> 4) << 14));
+}
+
+// Rows of slabs: row r's slab s (32 columns) is 128 bytes at r * pitch + s * 128, high halves first.
+// One workgroup: BM x BN of the result, waves of WM x WN, slabs through a ring of NBUF LDS buffers, loaded straight into LDS
+// NBUF - 1 slabs ahead.  16-byte chunk c of row r lies at c ^ ((r >> 1) & 7): the 16 rows that a fragment read takes at a time
+// then lie in different banks.
+template <int BM, int BN, int WM, int WN, int NBUF, int USE>
+__global__ __launch_bounds__(64 * (BM / WM) * (BN / WN)) void split_product(const SplitTable tb, float lr,
+                                                                           const double* __restrict__ state, float wd) {
+    constexpr int WAVES = (BM / WM) * (BN / WN), TM = WM / 32, TN = WN / 32;
+    constexpr int AL = BM / 8 / WAVES, BL = BN / 8 / WAVES;
+    static_assert(AL * 8 * WAVES == BM && BL * 8 * WAVES == BN, "whole loads a wave");
+    constexpr int BUF = (BM + BN) * 128;
+    static_assert(NBUF * BUF >= WAVES * 32 * 33 * 4, "the epilogue's blocks fit");
+    constexpr bool kSym = USE == kSplitGram || USE == kSplitPoly;
+    __shared__ __attribute__((aligned(1024))) char lds[NBUF * BUF];
+
+    const int tile = xcd_contiguous_id(blockIdx.x, gridDim.x);
+    // the product's numbers by scalar loads from the kernel's arguments (an index into the struct itself would copy it to memory)
+    typedef const SplitTable __attribute__((address_space(4)))* table_ptr;
+    const table_ptr args = (table_ptr)__builtin_amdgcn_kernarg_segment_ptr();
+    int at = 0;
+    while (at + 1 < tb.count && tile >= args->p[at + 1].first) ++at;
+    SplitProduct pr = tb.p[0];
+    __builtin_memcpy(&pr, (const void*)(args->p + at), sizeof(pr));
+    int ti, tj;
+    if (kSym) {
+        muon_triangle(tile - pr.first, &ti, &tj);
+    } else {
+        // bands of four tile rows, walked column by column: neighbours in time share operands in their XCD's L2
+        const int t = tile - pr.first, band = t / (4 * pr.tn), in = t - band * 4 * pr.tn;
+        const int height = min(4, pr.tm - band * 4);
+        tj = in / height;
+        ti = band * 4 + in - tj * height;
+    }
+    const int K = pr.K, slabs = K / 32;
+    const unsigned pitch = (unsigned)K * 4u;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const int l32 = lane & 31, lh = lane >> 5;
+    const int r0 = ti * BM, c0 = tj * BN;
+    const u32x4 rp = raw_rsrc(pr.P + (size_t)r0 * pitch, (unsigned)min(pr.M - r0, BM) * pitch);
+    const u32x4 rq = raw_rsrc(pr.Q + (size_t)c0 * pitch, (unsigned)min(pr.N - c0, BN) * pitch);
+    unsigned vp[AL], vq[BL];                             // (rows behind the matrix are behind the descriptor's end: they read as zeros)
+#pragma unroll
+    for (int i = 0; i < AL; ++i) {
+        const unsigned r = (unsigned)(wave * AL + i) * 8 + (lane >> 3);
+        vp[i] = r * pitch + (((unsigned)lane & 7u) ^ ((r >> 1) & 7u)) * 16u;
+    }
+#pragma unroll
+    for (int i = 0; i < BL; ++i) {
+        const unsigned r = (unsigned)(wave * BL + i) * 8 + (lane >> 3);
+        vq[i] = r * pitch + (((unsigned)lane & 7u) ^ ((r >> 1) & 7u)) * 16u;
+    }
+    const unsigned lds0 = lds_address(lds);
+    const auto issue = [&](int s, int buf) {
+        const unsigned base = lds0 + (unsigned)buf * BUF, off = (unsigned)s * 128u;
+#pragma unroll
+        for (int i = 0; i < AL; ++i) lds_direct_load16_s(rp, base + (unsigned)(wave * AL + i) * 1024u, vp[i], off);
+#pragma unroll
+        for (int i = 0; i < BL; ++i) lds_direct_load16_s(rq, base + BM * 128u + (unsigned)(wave * BL + i) * 1024u, vq[i], off);
+    };
+
+    f16v acc[TM][TN];
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int j = 0; j < TN; ++j)
+#pragma unroll
+            for (int v = 0; v < 16; ++v) acc[i][j][v] = 0.f;
+
+    const int wm = (wave / (BN / WN)) * WM, wn = (wave % (BN / WN)) * WN;
+    const unsigned sw = (unsigned)(lh ^ ((l32 >> 1) & 7)) * 16u;
+    const unsigned fa = (unsigned)(wm + l32) * 128u + sw, fb = (unsigned)(BM + wn + l32) * 128u + sw;
+    const auto multiply = [&](int buf) {
+        const char* b = lds + buf * BUF;
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            half8 ah[TM], al[TM], bh[TN], bl[TN];
+#pragma unroll
+            for (int i = 0; i < TM; ++i) {
+                ah[i] = *reinterpret_cast<const half8*>(b + ((fa ^ (t * 32u)) + i * 4096u));
+                al[i] = *reinterpret_cast<const half8*>(b + ((fa ^ (t * 32u + 64u)) + i * 4096u));
+            }
+#pragma unroll
+            for (int j = 0; j < TN; ++j) {
+                bh[j] = *reinterpret_cast<const half8*>(b + ((fb ^ (t * 32u)) + j * 4096u));
+                bl[j] = *reinterpret_cast<const half8*>(b + ((fb ^ (t * 32u + 64u)) + j * 4096u));
+            }
+#pragma unroll
+            for (int i = 0; i < TM; ++i)
+#pragma unroll
+                for (int j = 0; j < TN; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah[i], bl[j], acc[i][j], 0, 0, 0);
+#pragma unroll
+            for (int i = 0; i < TM; ++i)
+#pragma unroll
+                for (int j = 0; j < TN; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(al[i], bh[j], acc[i][j], 0, 0, 0);
+#pragma unroll
+            for (int i = 0; i < TM; ++i)
+#pragma unroll
+                for (int j = 0; j < TN; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah[i], bh[j], acc[i][j], 0, 0, 0);
+        }
+    };
+#pragma unroll
+    for (int d = 0; d < NBUF - 1; ++d)
+        if (d < slabs) issue(d, d);
+    int buf = 0, next = NBUF - 1;
+    for (int s = 0; s < slabs; ++s) {
+        // slab s has landed: the loads of at most NBUF - 2 later ones are on their way
+        if (s + NBUF - 2 < slabs) wait_loads<(AL + BL) * (NBUF - 2)>();
+        else wait_loads<0>();
+        asm volatile("s_barrier" ::: "memory");          // for every wave; and every wave is done with slab s - 1, whose buffer is next
+        if (s + NBUF - 1 < slabs) issue(s + NBUF - 1, next);
+        multiply(buf);
+        buf = buf + 1 == NBUF ? 0 : buf + 1;
+        next = next + 1 == NBUF ? 0 : next + 1;
+    }
+    wait_loads<0>();
+    asm volatile("s_barrier" ::: "memory");              // the epilogue uses the buffers as well
+
+    // block (i, j) of a wave: acc[v] = result[r][c], r = 8 (v / 4) + 4 lh + v % 4, c = l32 of the block
+    float(*blk)[33] = reinterpret_cast<float(*)[33]>(lds + wave * (32 * 33 * 4));
+    constexpr float kOut = USE == kSplitGram   ? kScaleA / (kScaleX * kScaleX)
+                           : USE == kSplitPoly ? kNsC * kScaleB / (kScaleA * kScaleA)
+                           : USE == kSplitStep ? 1.f / kScaleB
+                                               : 1.f / (kScaleB * kScaleX);
+    if (USE == kSplitApply) {
+        if (state != nullptr) lr = (float)state[3];
+        const float keep = 1.0f - lr * wd, step = lr * pr.gain;
+#pragma unroll
+        for (int i = 0; i < TM; ++i)
+#pragma unroll
+            for (int j = 0; j < TN; ++j) {
+                const int c = c0 + wn + 32 * j + l32;
+#pragma unroll
+                for (int v = 0; v < 16; ++v) {
+                    const int r = r0 + wm + 32 * i + 8 * (v >> 2) + 4 * lh + (v & 3);
+                    if (r < pr.rows && c < pr.cols) {
+                        const size_t k = (size_t)r * pr.cols + c;
+                        const float o = acc[i][j][v] * kOut;
+                        if (pr.theta != nullptr) pr.theta[k] = keep * pr.theta[k] - step * o;
+                        else pr.out[k] = o;
+                    }
+                }
+            }
+        return;
+    }
+    const size_t pitch1 = (size_t)pr.N * 4, pitch2 = (size_t)pr.M * 4;
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int j = 0; j < TN; ++j) {
+            const int r = r0 + wm + 32 * i, c = c0 + wn + 32 * j;
+            if (r >= pr.M || c >= pr.N) continue;        // (whole blocks: both are multiples of 32)
+            if (kSym && r > c) continue;                 // (below the diagonal of a diagonal tile: written from above it)
+            float o[16];
+#pragma unroll
+            for (int v = 0; v < 16; ++v) o[v] = acc[i][j][v] * kOut;
+            if (USE == kSplitPoly) {
+                // A[r][c] read as A[c][r]: four consecutive rows a load
+                const char* a = pr.A + (size_t)(c + l32) * pitch2 + (size_t)(r / 32) * 128 + 8 * lh;
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const half4 h = *reinterpret_cast<const half4*>(a + 16 * q), l = *reinterpret_cast<const half4*>(a + 16 * q + 64);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) o[4 * q + e] += ((float)h[e] + (float)l[e]) * (kNsB * kScaleB / kScaleA);
+                }
+                if (r == c)
+#pragma unroll
+                    for (int v = 0; v < 16; ++v)
+                        if (8 * (v >> 2) + 4 * lh + (v & 3) == l32) o[v] += kNsA * kScaleB;
+            }
+            // transposed: row c + l32, four consecutive columns a piece (not for diagonal blocks of a symmetric result: each
+            // place is written once, by one lane)
+            char* d2 = kSym ? pr.D1 : pr.D2;
+            if (!(kSym && r == c)) {
+                char* d = d2 + (size_t)(c + l32) * pitch2 + (size_t)(r / 32) * 128 + 8 * lh;
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    half4 h, l;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        _Float16 x, y;
+                        split_half(o[4 * q + e], x, y);
+                        h[e] = x;
+                        l[e] = y;
+                    }
+                    *reinterpret_cast<half4*>(d + 16 * q) = h;
+                    *reinterpret_cast<half4*>(d + 16 * q + 64) = l;
+                }
+            }
+            // as it is: through LDS, so that a lane has 16 consecutive columns of row r + l32
+#pragma unroll
+            for (int v = 0; v < 16; ++v) blk[8 * (v >> 2) + 4 * lh + (v & 3)][l32] = o[v];
+            __builtin_amdgcn_wave_barrier();
+            char* d = pr.D1 + (size_t)(r + l32) * pitch1 + (size_t)(c / 32) * 128 + 32 * lh;
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+                half8 h, l;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    _Float16 x, y;
+                    split_half(blk[l32][16 * lh + 8 * q + e], x, y);
+                    h[e] = x;
+                    l[e] = y;
+                }
+                *reinterpret_cast<half8*>(d + 16 * q) = h;
+                *reinterpret_cast<half8*>(d + 16 * q + 64) = l;
+            }
+            __builtin_amdgcn_wave_barrier();
+        }
+}
+
+}  // namespace aeth

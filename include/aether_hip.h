@@ -340,7 +340,7 @@ int aeth_adam_multi_dev_f32(int count, float* const* host_theta, const float* co
  *     X = g / |g| (Frobenius);  X <- a X + (b A + c A^2) X,  A = X X^T   (a, b, c) = (3.4445, -4.7750, 2.0315),
  * which takes every singular value s of g / |g| to p(...p(s)), p(s) = a s + b s^3 + c s^5, and keeps the singular vectors.
  * Any positive multiple of g gives the same o (there is no epsilon); g = 0 gives 0; a NaN or an infinity makes all of o NaN.
- * g and o are [rows, cols] and may not overlap; products and sums hold 22 bits or more of every factor.
+ * g and o are [rows, cols], sides of at most 2^21, and may not overlap; products and sums hold 22 bits or more of every factor.
  * aeth_muon_multi_f32 updates `count` (1..32) matrices in one call:
  *     m <- momentum m + grad;  u = grad + momentum m (nesterov != 0) or m;  O = newton_schulz(u);
  *     theta <- theta (1 - lr weight_decay) - lr sqrt(max(1, cols / rows)) O.
