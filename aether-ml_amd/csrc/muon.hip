@@ -112,8 +112,8 @@ __global__ __launch_bounds__(256) void muon_split(const MuonTable tb, float mu, 
         blk[2 * v + lh][l32] = (float)((double)u * inv);
     }
     __builtin_amdgcn_wave_barrier();
-    char* same = args->same[k] + (size_t)(r + l32) * cp * 4 + (size_t)(c / 32) * 128 + 32 * lh;
-    char* turned = args->turned[k] + (size_t)(c + l32) * rp * 4 + (size_t)(r / 32) * 128 + 32 * lh;
+    char* same = args->same[k] + ((size_t)(c / 32) * rp + r + l32) * 128 + 32 * lh;
+    char* turned = args->turned[k] + ((size_t)(r / 32) * cp + c + l32) * 128 + 32 * lh;
 #pragma unroll
     for (int q = 0; q < 2; ++q) {
         half8 h, l, ht, lt;
@@ -153,11 +153,16 @@ static int muon_launch(SplitTable tb, float lr, const double* state, float wd) {
 
 template <int USE>
 static int muon_product(const SplitTable& tb, float lr, const double* state, float wd) {
+    // (kMuonTileTable's order)
     constexpr bool kSym = USE == kSplitGram || USE == kSplitPoly;
-    int64_t tiles = 0;
-    for (int i = 0; i < tb.count; ++i) tiles += muon_tiles(tb.p[i].M, tb.p[i].N, 128, 128, kSym);
-    if (tiles >= 256) return muon_launch<128, 128, 64, 64, 2, USE>(tb, lr, state, wd);
-    return muon_launch<64, 64, 32, 32, 4, USE>(tb, lr, state, wd);
+    MuonShape shapes[kMuonMax];
+    for (int i = 0; i < tb.count; ++i) shapes[i] = MuonShape{tb.p[i].M, tb.p[i].N, tb.p[i].K};
+    const int tile = muon_choose(shapes, tb.count, kSym);
+    if (tile == 0) return muon_launch<64, 64, 32, 32, 4, USE>(tb, lr, state, wd);
+    if (tile == 1) return muon_launch<96, 96, 96, 32, 3, USE>(tb, lr, state, wd);
+    if (tile == 2) return muon_launch<128, 128, 64, 64, 4, USE>(tb, lr, state, wd);
+    if constexpr (kSym) return muon_launch<192, 192, 96, 96, 3, USE>(tb, lr, state, wd);
+    else return muon_launch<256, 128, 64, 64, 3, USE>(tb, lr, state, wd);
 }
 
 // The whole update of at most kMuonMax matrices that share the workspace.

@@ -1,8 +1,7 @@
 // How a call's matrices are laid out and cut into tiles for the Newton-Schulz products.  Free of HIP calls, so that the host
 // can check it without a GPU.
 //
-// A matrix is held as two float16 halves (split_gemm.h) in rows of slabs: 32 columns are 64 bytes of high halves and 64 bytes
-// of low ones.  Rows and columns are padded to multiples of 32 with zeros; zeros stay zeros through all products.
+// A matrix is held as two float16 halves (split_gemm.h) in slabs of 32 columns.  Rows and columns are padded to multiples of 32 with zeros; zeros stay zeros through all products.
 #pragma once
 
 #include <stdint.h>
@@ -53,6 +52,58 @@ MUON_HD void muon_triangle(int t, int* i, int* j) {
 static inline int64_t muon_tiles(int64_t rows, int64_t cols, int bm, int bn, bool symmetric) {
     const int64_t tm = (rows + bm - 1) / bm, tn = (cols + bn - 1) / bn;
     return symmetric ? tm * (tm + 1) / 2 : tm * tn;
+}
+
+// The tile shapes a product can be cut into, with what a tile costs: `start` us a launch, then us a slab of 32 columns on a CU
+// whose neighbours are idle (`alone`) and with a tile on every CU (`full`: the tiles then share the L2 caches' bandwidth and the
+// power that the matrix units may draw).  Measured on square and wide products of 64 to 4096 rows; a CU takes what its tiles
+// cost one after the other, whether they are on it together or not.
+struct MuonTile {
+    int bm, bn;
+    bool symmetric, general;     // offered for symmetric results, for others
+    float start, alone, full;
+};
+constexpr int kMuonTiles = 5;
+static const MuonTile kMuonTileTable[kMuonTiles] = {
+    {64, 64, true, true, 3.5f, 0.24f, 0.25f},
+    {96, 96, true, true, 5.0f, 0.41f, 0.50f},
+    {128, 128, true, true, 6.0f, 0.53f, 0.80f},
+    {192, 192, true, false, 8.0f, 1.05f, 1.45f},
+    {256, 128, false, true, 7.0f, 0.95f, 1.17f},
+};
+constexpr int kMuonCus = 256;
+
+struct MuonShape {
+    int64_t rows, cols, k;       // padded
+};
+
+// What a launch of these products costs with one tile shape, in us.
+static inline float muon_cost(const MuonTile& t, const MuonShape* p, int count, bool symmetric) {
+    int64_t tiles = 0, slabs = 0;
+    float longest = 0.f;
+    for (int i = 0; i < count; ++i) {
+        const int64_t n = muon_tiles(p[i].rows, p[i].cols, t.bm, t.bn, symmetric);
+        tiles += n;
+        slabs += n * (p[i].k / 32);
+        const float mine = (float)((n + kMuonCus - 1) / kMuonCus) * (float)(p[i].k / 32);
+        if (mine > longest) longest = mine;
+    }
+    const float even = (float)slabs / kMuonCus, share = tiles < kMuonCus ? (float)tiles / kMuonCus : 1.f;
+    return t.start + (longest > even ? longest : even) * (t.alone + (t.full - t.alone) * share);
+}
+
+static inline int muon_choose(const MuonShape* p, int count, bool symmetric) {
+    int best = -1;
+    float least = 0.f;
+    for (int i = 0; i < kMuonTiles; ++i) {
+        if (!(symmetric ? kMuonTileTable[i].symmetric : kMuonTileTable[i].general)) continue;
+        const float c = muon_cost(kMuonTileTable[i], p, count, symmetric);
+        if (best < 0 || c < least) {
+            best = i;
+            least = c;
+        }
+    }
+    return best;
 }
 
 }  // namespace aeth

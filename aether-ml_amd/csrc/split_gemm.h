@@ -10,6 +10,8 @@
 #include "conv_common.h"
 #include "muon_plan.h"
 
+#include <type_traits>
+
 namespace aeth {
 
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
@@ -55,7 +57,8 @@ __device__ __forceinline__ void wait_loads() {           // at most N of this wa
     __builtin_amdgcn_s_waitcnt((N & 15) | (7 << 4) | (0 << 8) | ((N >> 4) << 14));
 }
 
-// Rows of slabs: row r's slab s (32 columns) is 128 bytes at r * pitch + s * 128, high halves first.
+// A matrix lies slab by slab: slab s holds columns 32 s .. 32 s + 31 of all R rows, row r's 128 bytes (64 of high halves, 64 of low)
+// at (s R + r) * 128, so that what a tile reads at a time is one contiguous piece and no offset grows with the matrix.
 // One workgroup: BM x BN of the result, waves of WM x WN, slabs through a ring of NBUF LDS buffers, loaded straight into LDS
 // NBUF - 1 slabs ahead.  16-byte chunk c of row r lies at c ^ ((r >> 1) & 7): the 16 rows that a fragment read takes at a time
 // then lie in different banks.
@@ -89,30 +92,33 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN)) void split_product(cons
         ti = band * 4 + in - tj * height;
     }
     const int K = pr.K, slabs = K / 32;
-    const unsigned pitch = (unsigned)K * 4u;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int l32 = lane & 31, lh = lane >> 5;
     const int r0 = ti * BM, c0 = tj * BN;
-    const u32x4 rp = raw_rsrc(pr.P + (size_t)r0 * pitch, (unsigned)min(pr.M - r0, BM) * pitch);
-    const u32x4 rq = raw_rsrc(pr.Q + (size_t)c0 * pitch, (unsigned)min(pr.N - c0, BN) * pitch);
+    const char *sp = pr.P + (size_t)r0 * 128, *sq = pr.Q + (size_t)c0 * 128;         // the next slab's rows
+    const unsigned np = (unsigned)min(pr.M - r0, BM) * 128u, nq = (unsigned)min(pr.N - c0, BN) * 128u;
+    const size_t dp = (size_t)pr.M * 128, dq = (size_t)pr.N * 128;
     unsigned vp[AL], vq[BL];                             // (rows behind the matrix are behind the descriptor's end: they read as zeros)
 #pragma unroll
     for (int i = 0; i < AL; ++i) {
         const unsigned r = (unsigned)(wave * AL + i) * 8 + (lane >> 3);
-        vp[i] = r * pitch + (((unsigned)lane & 7u) ^ ((r >> 1) & 7u)) * 16u;
+        vp[i] = r * 128u + (((unsigned)lane & 7u) ^ ((r >> 1) & 7u)) * 16u;
     }
 #pragma unroll
     for (int i = 0; i < BL; ++i) {
         const unsigned r = (unsigned)(wave * BL + i) * 8 + (lane >> 3);
-        vq[i] = r * pitch + (((unsigned)lane & 7u) ^ ((r >> 1) & 7u)) * 16u;
+        vq[i] = r * 128u + (((unsigned)lane & 7u) ^ ((r >> 1) & 7u)) * 16u;
     }
     const unsigned lds0 = lds_address(lds);
-    const auto issue = [&](int s, int buf) {
-        const unsigned base = lds0 + (unsigned)buf * BUF, off = (unsigned)s * 128u;
-#pragma unroll
-        for (int i = 0; i < AL; ++i) lds_direct_load16_s(rp, base + (unsigned)(wave * AL + i) * 1024u, vp[i], off);
-#pragma unroll
-        for (int i = 0; i < BL; ++i) lds_direct_load16_s(rq, base + BM * 128u + (unsigned)(wave * BL + i) * 1024u, vq[i], off);
+    constexpr int LOADS = AL + BL;
+    const auto load = [&](int i, int buf) {              // one of a wave's loads of the next slab
+        const unsigned base = lds0 + (unsigned)buf * BUF;
+        if (i < AL) lds_direct_load16(raw_rsrc(sp, np), base + (unsigned)(wave * AL + i) * 1024u, vp[i]);
+        else lds_direct_load16(raw_rsrc(sq, nq), base + BM * 128u + (unsigned)(wave * BL + i - AL) * 1024u, vq[i - AL]);
+    };
+    const auto advance = [&] {
+        sp += dp;
+        sq += dq;
     };
 
     f16v acc[TM][TN];
@@ -126,48 +132,75 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN)) void split_product(cons
     const int wm = (wave / (BN / WN)) * WM, wn = (wave % (BN / WN)) * WN;
     const unsigned sw = (unsigned)(lh ^ ((l32 >> 1) & 7)) * 16u;
     const unsigned fa = (unsigned)(wm + l32) * 128u + sw, fb = (unsigned)(BM + wn + l32) * 128u + sw;
-    const auto multiply = [&](int buf) {
+    // One slab: two steps of 16 columns, three products each.  The next slab's loads go out one by one between the MFMAs: a wave
+    // that issues them all at once waits for the load unit's queue with its MFMAs behind it (4096 x 4096, tiles of 256 x 128: 307 us
+    // a product, tiles of 192 x 192 for the symmetric ones 194 us; all at once 215 us for these).
+    const auto multiply = [&](int buf, int into, auto loads) {
         const char* b = lds + buf * BUF;
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-            half8 ah[TM], al[TM], bh[TN], bl[TN];
+        half8 f[2][2 * TM + 2 * TN];                     // high and low halves of both operands' rows, for either step
+        const auto read = [&](int t) {
 #pragma unroll
             for (int i = 0; i < TM; ++i) {
-                ah[i] = *reinterpret_cast<const half8*>(b + ((fa ^ (t * 32u)) + i * 4096u));
-                al[i] = *reinterpret_cast<const half8*>(b + ((fa ^ (t * 32u + 64u)) + i * 4096u));
+                f[t][i] = *reinterpret_cast<const half8*>(b + ((fa ^ (t * 32u)) + i * 4096u));
+                f[t][TM + i] = *reinterpret_cast<const half8*>(b + ((fa ^ (t * 32u + 64u)) + i * 4096u));
             }
 #pragma unroll
             for (int j = 0; j < TN; ++j) {
-                bh[j] = *reinterpret_cast<const half8*>(b + ((fb ^ (t * 32u)) + j * 4096u));
-                bl[j] = *reinterpret_cast<const half8*>(b + ((fb ^ (t * 32u + 64u)) + j * 4096u));
+                f[t][2 * TM + j] = *reinterpret_cast<const half8*>(b + ((fb ^ (t * 32u)) + j * 4096u));
+                f[t][2 * TM + TN + j] = *reinterpret_cast<const half8*>(b + ((fb ^ (t * 32u + 64u)) + j * 4096u));
             }
+        };
+        read(0);
 #pragma unroll
-            for (int i = 0; i < TM; ++i)
+        for (int t = 0; t < 2; ++t) {
 #pragma unroll
-                for (int j = 0; j < TN; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah[i], bl[j], acc[i][j], 0, 0, 0);
+            for (int g = 0; g < 3; ++g) {                // high.low, low.high, high.high
+                if (t == 0 && g == 1) read(1);
 #pragma unroll
-            for (int i = 0; i < TM; ++i)
+                for (int i = 0; i < TM; ++i) {
+                    const half8 x = f[t][(g == 1 ? TM : 0) + i];
 #pragma unroll
-                for (int j = 0; j < TN; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(al[i], bh[j], acc[i][j], 0, 0, 0);
+                    for (int j = 0; j < TN; ++j)
+                        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, f[t][2 * TM + (g == 0 ? TN : 0) + j], acc[i][j], 0, 0, 0);
+                    constexpr int GROUPS = 6 * TM;
+                    const int u = (t * 3 + g) * TM + i;
+                    if (decltype(loads)::value) {
 #pragma unroll
-            for (int i = 0; i < TM; ++i)
-#pragma unroll
-                for (int j = 0; j < TN; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah[i], bh[j], acc[i][j], 0, 0, 0);
+                        for (int k = u * LOADS / GROUPS; k < (u + 1) * LOADS / GROUPS; ++k) {
+                            __builtin_amdgcn_sched_barrier(0);
+                            load(k, into);
+                            __builtin_amdgcn_sched_barrier(0);
+                        }
+                    }
+                }
+            }
         }
+        if (decltype(loads)::value) advance();
     };
 #pragma unroll
     for (int d = 0; d < NBUF - 1; ++d)
-        if (d < slabs) issue(d, d);
+        if (d < slabs) {
+#pragma unroll
+            for (int i = 0; i < LOADS; ++i) load(i, d);
+            advance();
+        }
     int buf = 0, next = NBUF - 1;
-    for (int s = 0; s < slabs; ++s) {
-        // slab s has landed: the loads of at most NBUF - 2 later ones are on their way
-        if (s + NBUF - 2 < slabs) wait_loads<(AL + BL) * (NBUF - 2)>();
-        else wait_loads<0>();
-        asm volatile("s_barrier" ::: "memory");          // for every wave; and every wave is done with slab s - 1, whose buffer is next
-        if (s + NBUF - 1 < slabs) issue(s + NBUF - 1, next);
-        multiply(buf);
+    const auto turn = [&] {
         buf = buf + 1 == NBUF ? 0 : buf + 1;
         next = next + 1 == NBUF ? 0 : next + 1;
+    };
+    int s = 0;
+    for (; s + NBUF - 1 < slabs; ++s) {
+        wait_loads<LOADS * (NBUF - 2)>();                // slab s has landed (NBUF - 2 later ones are on their way)
+        asm volatile("s_barrier" ::: "memory");          // for every wave; and every wave is done with slab s - 1, whose buffer is next
+        multiply(buf, next, std::true_type{});
+        turn();
+    }
+    for (; s < slabs; ++s) {
+        wait_loads<0>();
+        asm volatile("s_barrier" ::: "memory");
+        multiply(buf, next, std::false_type{});
+        turn();
     }
     wait_loads<0>();
     asm volatile("s_barrier" ::: "memory");              // the epilogue uses the buffers as well
@@ -199,7 +232,6 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN)) void split_product(cons
             }
         return;
     }
-    const size_t pitch1 = (size_t)pr.N * 4, pitch2 = (size_t)pr.M * 4;
 #pragma unroll
     for (int i = 0; i < TM; ++i)
 #pragma unroll
@@ -212,7 +244,7 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN)) void split_product(cons
             for (int v = 0; v < 16; ++v) o[v] = acc[i][j][v] * kOut;
             if (USE == kSplitPoly) {
                 // A[r][c] read as A[c][r]: four consecutive rows a load
-                const char* a = pr.A + (size_t)(c + l32) * pitch2 + (size_t)(r / 32) * 128 + 8 * lh;
+                const char* a = pr.A + ((size_t)(r / 32) * pr.M + c + l32) * 128 + 8 * lh;
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
                     const half4 h = *reinterpret_cast<const half4*>(a + 16 * q), l = *reinterpret_cast<const half4*>(a + 16 * q + 64);
@@ -228,7 +260,7 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN)) void split_product(cons
             // place is written once, by one lane)
             char* d2 = kSym ? pr.D1 : pr.D2;
             if (!(kSym && r == c)) {
-                char* d = d2 + (size_t)(c + l32) * pitch2 + (size_t)(r / 32) * 128 + 8 * lh;
+                char* d = d2 + ((size_t)(r / 32) * pr.N + c + l32) * 128 + 8 * lh;
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
                     half4 h, l;
@@ -247,7 +279,7 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN)) void split_product(cons
 #pragma unroll
             for (int v = 0; v < 16; ++v) blk[8 * (v >> 2) + 4 * lh + (v & 3)][l32] = o[v];
             __builtin_amdgcn_wave_barrier();
-            char* d = pr.D1 + (size_t)(r + l32) * pitch1 + (size_t)(c / 32) * 128 + 32 * lh;
+            char* d = pr.D1 + ((size_t)(c / 32) * pr.M + r + l32) * 128 + 32 * lh;
 #pragma unroll
             for (int q = 0; q < 2; ++q) {
                 half8 h, l;
