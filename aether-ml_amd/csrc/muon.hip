@@ -83,54 +83,55 @@ __global__ __launch_bounds__(256) void muon_momentum(const MuonTable tb, float m
 }
 
 // X = u / |u| and its transpose as float16 halves, a 32 x 32 block a wave; padding becomes 0.
-// Bound: HBM, 8 bytes read and 8 written an element.
+// Bound: HBM, 8 bytes read and 8 written an element; for small matrices the chain partial sums - norm - loads - stores, so the loads
+// go out first, all at once (behind a branch each they came back one by one: 576 x 64 10 us).
 __global__ __launch_bounds__(256) void muon_split(const MuonTable tb, float mu, int nesterov) {
     __shared__ double red[4];
-    __shared__ float blocks[4][32][33];
+    __shared__ unsigned blocks[4][32][33];
     const muon_table_ptr args = (muon_table_ptr)__builtin_amdgcn_kernarg_segment_ptr();
     int k = 0;
     while (k + 1 < tb.count && (int)blockIdx.x >= args->first[k + 1]) ++k;
-    const double sum = muon_block_sum((int)threadIdx.x < args->parts[k] ? args->sums[k * kMuonParts + threadIdx.x] : 0.0, red);
-    const double inv = sum != 0.0 ? (double)kScaleX / sqrt(sum) : 0.0;
     const float* __restrict__ grad = args->t[k].grad;
     const float* __restrict__ mom = args->t[k].mom;
     const int rows = args->t[k].rows, cols = args->t[k].cols;
     const int64_t rp = muon_pad(rows), cp = muon_pad(cols), across = cp / 32;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, l32 = lane & 31, lh = lane >> 5;
     const int64_t b = ((int64_t)blockIdx.x - args->first[k]) * 4 + wave;
-    if (b >= rp / 32 * across) return;
-    const int64_t r = b / across * 32, c = b % across * 32;
-    float(*blk)[33] = blocks[wave];
+    const bool mine = b < rp / 32 * across;
+    const int64_t r = mine ? b / across * 32 : 0, c = mine ? b % across * 32 : 0;
+    const int64_t x = c + l32, xc = x < cols ? x : cols - 1;
+    float u[16], m[16];
 #pragma unroll
     for (int v = 0; v < 16; ++v) {
-        const int64_t y = r + 2 * v + lh, x = c + l32;
-        float u = 0.f;
-        if (y < rows && x < cols) {
-            u = grad[y * cols + x];
-            if (mom != nullptr) u = muon_update(u, mom[y * cols + x], mu, nesterov);
-        }
-        blk[2 * v + lh][l32] = (float)((double)u * inv);
+        const int64_t y = r + 2 * v + lh, at = (y < rows ? y : rows - 1) * cols + xc;
+        u[v] = grad[at];
+        m[v] = mom != nullptr ? mom[at] : 0.f;
+    }
+    const double sum = muon_block_sum((int)threadIdx.x < args->parts[k] ? args->sums[k * kMuonParts + threadIdx.x] : 0.0, red);
+    // 1 / |u| as a power of two and a factor near one: u times the power is exact, whatever its size
+    int power = 0;
+    const float factor = sum != 0.0 ? (float)frexp((double)kScaleX / sqrt(sum), &power) : 0.f;
+    if (!mine) return;
+    unsigned(*blk)[33] = blocks[wave];
+#pragma unroll
+    for (int v = 0; v < 16; ++v) {
+        const float w = mom != nullptr ? muon_update(u[v], m[v], mu, nesterov) : u[v];
+        const bool in = r + 2 * v + lh < rows && x < cols;
+        blk[2 * v + lh][l32] = split_pack(in ? ldexpf(w, power) * factor : 0.f);
     }
     __builtin_amdgcn_wave_barrier();
     char* same = args->same[k] + ((size_t)(c / 32) * rp + r + l32) * 128 + 32 * lh;
     char* turned = args->turned[k] + ((size_t)(r / 32) * cp + c + l32) * 128 + 32 * lh;
 #pragma unroll
     for (int q = 0; q < 2; ++q) {
-        half8 h, l, ht, lt;
+        unsigned s[8], t[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            _Float16 x, y;
-            split_half(blk[l32][16 * lh + 8 * q + e], x, y);
-            h[e] = x;
-            l[e] = y;
-            split_half(blk[16 * lh + 8 * q + e][l32], x, y);
-            ht[e] = x;
-            lt[e] = y;
+            s[e] = blk[l32][16 * lh + 8 * q + e];
+            t[e] = blk[16 * lh + 8 * q + e][l32];
         }
-        *reinterpret_cast<half8*>(same + 16 * q) = h;
-        *reinterpret_cast<half8*>(same + 16 * q + 64) = l;
-        *reinterpret_cast<half8*>(turned + 16 * q) = ht;
-        *reinterpret_cast<half8*>(turned + 16 * q + 64) = lt;
+        split_store<8>(same + 16 * q, s);
+        split_store<8>(turned + 16 * q, t);
     }
 }
 

@@ -46,9 +46,24 @@ struct SplitTable {
 constexpr float kScaleX = 32768.f, kScaleA = 32768.f, kScaleB = 16384.f;
 constexpr float kNsA = 3.4445f, kNsB = -4.7750f, kNsC = 2.0315f;
 
-__device__ __forceinline__ void split_half(float v, _Float16& hi, _Float16& lo) {
-    hi = (_Float16)v;
-    lo = (_Float16)(v - (float)hi);
+// x's halves in one word: the high one below
+__device__ __forceinline__ unsigned split_pack(float v) {
+    const _Float16 hi = (_Float16)v, lo = (_Float16)(v - (float)hi);
+    return (unsigned)__builtin_bit_cast(unsigned short, hi) | (unsigned)__builtin_bit_cast(unsigned short, lo) << 16;
+}
+
+// N neighbouring elements (4 or 8) of a row: high halves to p, low halves 64 bytes behind
+template <int N>
+__device__ __forceinline__ void split_store(char* p, const unsigned* w) {
+    typedef unsigned words __attribute__((ext_vector_type(N / 2)));
+    words hi, lo;
+#pragma unroll
+    for (int e = 0; e < N / 2; ++e) {
+        hi[e] = __builtin_amdgcn_perm(w[2 * e + 1], w[2 * e], 0x05040100u);
+        lo[e] = __builtin_amdgcn_perm(w[2 * e + 1], w[2 * e], 0x07060302u);
+    }
+    *reinterpret_cast<words*>(p) = hi;
+    *reinterpret_cast<words*>(p + 64) = lo;
 }
 
 template <int N>
@@ -206,7 +221,7 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN)) void split_product(cons
     asm volatile("s_barrier" ::: "memory");              // the epilogue uses the buffers as well
 
     // block (i, j) of a wave: acc[v] = result[r][c], r = 8 (v / 4) + 4 lh + v % 4, c = l32 of the block
-    float(*blk)[33] = reinterpret_cast<float(*)[33]>(lds + wave * (32 * 33 * 4));
+    unsigned(*blk)[33] = reinterpret_cast<unsigned(*)[33]>(lds + wave * (32 * 33 * 4));
     constexpr float kOut = USE == kSplitGram   ? kScaleA / (kScaleX * kScaleX)
                            : USE == kSplitPoly ? kNsC * kScaleB / (kScaleA * kScaleA)
                            : USE == kSplitStep ? 1.f / kScaleB
@@ -218,15 +233,21 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN)) void split_product(cons
         for (int i = 0; i < TM; ++i)
 #pragma unroll
             for (int j = 0; j < TN; ++j) {
-                const int c = c0 + wn + 32 * j + l32;
+                // (all the loads of a block at once, from places clamped into the matrix: behind a branch each they came back
+                // one by one)
+                const int c = c0 + wn + 32 * j + l32, cc = min(c, pr.cols - 1), r = r0 + wm + 32 * i + 4 * lh;
+                float t[16];
+                if (pr.theta != nullptr) {
+#pragma unroll
+                    for (int v = 0; v < 16; ++v) t[v] = pr.theta[(size_t)min(r + 8 * (v >> 2) + (v & 3), pr.rows - 1) * pr.cols + cc];
+                }
 #pragma unroll
                 for (int v = 0; v < 16; ++v) {
-                    const int r = r0 + wm + 32 * i + 8 * (v >> 2) + 4 * lh + (v & 3);
-                    if (r < pr.rows && c < pr.cols) {
-                        const size_t k = (size_t)r * pr.cols + c;
+                    const int y = r + 8 * (v >> 2) + (v & 3);
+                    if (y < pr.rows && c < pr.cols) {
                         const float o = acc[i][j][v] * kOut;
-                        if (pr.theta != nullptr) pr.theta[k] = keep * pr.theta[k] - step * o;
-                        else pr.out[k] = o;
+                        if (pr.theta != nullptr) pr.theta[(size_t)y * pr.cols + c] = keep * t[v] - step * o;
+                        else pr.out[(size_t)y * pr.cols + c] = o;
                     }
                 }
             }
@@ -256,42 +277,27 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN)) void split_product(cons
                     for (int v = 0; v < 16; ++v)
                         if (8 * (v >> 2) + 4 * lh + (v & 3) == l32) o[v] += kNsA * kScaleB;
             }
+            unsigned w[16];
+#pragma unroll
+            for (int v = 0; v < 16; ++v) w[v] = split_pack(o[v]);
             // transposed: row c + l32, four consecutive columns a piece (not for diagonal blocks of a symmetric result: each
             // place is written once, by one lane)
-            char* d2 = kSym ? pr.D1 : pr.D2;
             if (!(kSym && r == c)) {
-                char* d = d2 + ((size_t)(r / 32) * pr.N + c + l32) * 128 + 8 * lh;
+                char* d = (kSym ? pr.D1 : pr.D2) + ((size_t)(r / 32) * pr.N + c + l32) * 128 + 8 * lh;
 #pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    half4 h, l;
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        _Float16 x, y;
-                        split_half(o[4 * q + e], x, y);
-                        h[e] = x;
-                        l[e] = y;
-                    }
-                    *reinterpret_cast<half4*>(d + 16 * q) = h;
-                    *reinterpret_cast<half4*>(d + 16 * q + 64) = l;
-                }
+                for (int q = 0; q < 4; ++q) split_store<4>(d + 16 * q, w + 4 * q);
             }
             // as it is: through LDS, so that a lane has 16 consecutive columns of row r + l32
 #pragma unroll
-            for (int v = 0; v < 16; ++v) blk[8 * (v >> 2) + 4 * lh + (v & 3)][l32] = o[v];
+            for (int v = 0; v < 16; ++v) blk[8 * (v >> 2) + 4 * lh + (v & 3)][l32] = w[v];
             __builtin_amdgcn_wave_barrier();
             char* d = pr.D1 + ((size_t)(c / 32) * pr.M + r + l32) * 128 + 32 * lh;
 #pragma unroll
             for (int q = 0; q < 2; ++q) {
-                half8 h, l;
+                unsigned s[8];
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    _Float16 x, y;
-                    split_half(blk[l32][16 * lh + 8 * q + e], x, y);
-                    h[e] = x;
-                    l[e] = y;
-                }
-                *reinterpret_cast<half8*>(d + 16 * q) = h;
-                *reinterpret_cast<half8*>(d + 16 * q + 64) = l;
+                for (int e = 0; e < 8; ++e) s[e] = blk[l32][16 * lh + 8 * q + e];
+                split_store<8>(d + 16 * q, s);
             }
             __builtin_amdgcn_wave_barrier();
         }
