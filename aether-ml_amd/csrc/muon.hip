@@ -107,7 +107,11 @@ __global__ __launch_bounds__(256) void muon_split(const MuonTable tb, float mu, 
         u[v] = grad[at];
         m[v] = mom != nullptr ? mom[at] : 0.f;
     }
-    const double sum = muon_block_sum((int)threadIdx.x < args->parts[k] ? args->sums[k * kMuonParts + threadIdx.x] : 0.0, red);
+    double part = 0.0;
+#pragma unroll
+    for (int i = 0; i < kMuonParts; i += 256)
+        if ((int)threadIdx.x + i < args->parts[k]) part += args->sums[k * kMuonParts + threadIdx.x + i];
+    const double sum = muon_block_sum(part, red);
     // 1 / |u| as a power of two and a factor near one: u times the power is exact, whatever its size
     int power = 0;
     const float factor = sum != 0.0 ? (float)frexp((double)kScaleX / sqrt(sum), &power) : 0.f;
@@ -138,13 +142,13 @@ __global__ __launch_bounds__(256) void muon_split(const MuonTable tb, float mu, 
 // One launch for one product of every matrix, in tiles of BM x BN.
 template <int BM, int BN, int WM, int WN, int NBUF, int USE>
 static int muon_launch(SplitTable tb, float lr, const double* state, float wd) {
-    constexpr bool kSym = USE == kSplitGram || USE == kSplitPoly;
+    constexpr bool kSym = USE == kSplitGram || USE == kSplitPoly || USE == kSplitPart;
     int64_t tiles = 0;
     for (int i = 0; i < tb.count; ++i) {
         tb.p[i].first = (int)tiles;
         tb.p[i].tm = cdiv(tb.p[i].M, BM);
         tb.p[i].tn = cdiv(tb.p[i].N, BN);
-        tiles += muon_tiles(tb.p[i].M, tb.p[i].N, BM, BN, kSym);
+        tiles += muon_tiles(tb.p[i].M, tb.p[i].N, BM, BN, kSym) * (USE == kSplitPart ? tb.p[i].runs : 1);
     }
     hipLaunchKernelGGL((split_product<BM, BN, WM, WN, NBUF, USE>), dim3((unsigned)tiles), dim3(64 * (BM / WM) * (BN / WN)), 0,
                        ctx().stream, tb, lr, state, wd);
@@ -166,6 +170,24 @@ static int muon_product(const SplitTable& tb, float lr, const double* state, flo
     else return muon_launch<256, 128, 64, 64, 3, USE>(tb, lr, state, wd);
 }
 
+// A = X X^T in runs of its columns.
+static int muon_gram_runs(SplitTable tb, int tile) {
+    int rc;
+    if (tile == 0) rc = muon_launch<64, 64, 32, 32, 4, kSplitPart>(tb, 0.f, nullptr, 0.f);
+    else if (tile == 1) rc = muon_launch<96, 96, 96, 32, 3, kSplitPart>(tb, 0.f, nullptr, 0.f);
+    else rc = muon_launch<128, 128, 64, 64, 4, kSplitPart>(tb, 0.f, nullptr, 0.f);
+    if (rc) return rc;
+    int64_t groups = 0;
+    for (int i = 0; i < tb.count; ++i) {
+        tb.p[i].first = (int)groups;
+        const int64_t side = tb.p[i].M / 32;
+        groups += side * (side + 1) / 2;
+    }
+    hipLaunchKernelGGL(split_join, dim3((unsigned)groups), dim3(512), 0, ctx().stream, tb);
+    AETH_LAUNCH_CHECK();
+    return AETH_OK;
+}
+
 // The whole update of at most kMuonMax matrices that share the workspace.
 static int muon_group(const MuonMatrix* t, int count, float lr, const double* state, float mu, int nesterov, float wd, int steps) {
     MuonTable tb = {};
@@ -185,10 +207,17 @@ static int muon_group(const MuonMatrix* t, int count, float lr, const double* st
         tb.first[i] = (int)blocks;
         blocks += cdiv(at[i].mp / 32 * (at[i].np / 32), 4);
     }
+    MuonShape shapes[kMuonMax];
+    MuonRuns runs = {};
+    for (int i = 0; i < count; ++i) shapes[i] = MuonShape{at[i].mp, at[i].mp, at[i].np};
+    const bool in_runs = muon_choose_runs(shapes, count, &runs);
+    const int64_t partial = bytes;                       // (after the matrices: a multiple of 4096 bytes from their begin)
+    if (in_runs) bytes += runs.bytes;
     void* ws;
     const int rc = workspace(bytes, &ws);
     if (rc) return rc;
     char* base = static_cast<char*>(ws);
+    int64_t part_at = partial;
     tb.sums = static_cast<double*>(ws);
     for (int i = 0; i < count; ++i) {
         char *x = base + at[i].x, *xt[2] = {base + at[i].xt0, base + at[i].xt1}, *a = base + at[i].a, *b = base + at[i].b;
@@ -203,6 +232,11 @@ static int muon_group(const MuonMatrix* t, int count, float lr, const double* st
         p.out = t[i].out;
         p.gain = t[i].gain;
         p.P = p.Q = x, p.D1 = a, p.M = p.N = mp, p.K = np;
+        if (in_runs) {
+            p.runs = (int)runs.runs[i], p.run = (int)runs.run;
+            p.part = reinterpret_cast<float*>(base + part_at);
+            part_at += (int64_t)p.runs * (mp / 32) * (mp / 32 + 1) / 2 * 4096;
+        }
         gram.p[i] = p;
         p.P = p.Q = p.A = a, p.D1 = b, p.K = mp;
         poly.p[i] = p;
@@ -221,7 +255,7 @@ static int muon_group(const MuonMatrix* t, int count, float lr, const double* st
     hipLaunchKernelGGL(muon_split, dim3((unsigned)blocks), dim3(256), 0, st, tb, mu, nesterov);
     AETH_LAUNCH_CHECK();
     for (int s = 0; s < steps; ++s) {
-        int e = muon_product<kSplitGram>(gram, lr, state, wd);
+        int e = in_runs ? muon_gram_runs(gram, runs.tile) : muon_product<kSplitGram>(gram, lr, state, wd);
         if (e == AETH_OK) e = muon_product<kSplitPoly>(poly, lr, state, wd);
         if (e == AETH_OK)
             e = s + 1 < steps ? muon_product<kSplitStep>(step[s & 1], lr, state, wd) : muon_product<kSplitApply>(apply, lr, state, wd);

@@ -16,7 +16,7 @@ namespace aeth {
 
 constexpr int kMuonMax = 32;                             // matrices of a call
 constexpr int kMuonLongest = 1 << 21;                    // rows or columns: a 256-row tile's bytes stay below 2^31
-constexpr int kMuonParts = 256;                          // partial sums of a matrix's norm
+constexpr int kMuonParts = 1024;                          // partial sums of a matrix's norm
 
 MUON_HD int64_t muon_pad(int64_t n) { return (n + 31) / 32 * 32; }
 
@@ -104,6 +104,53 @@ static inline int muon_choose(const MuonShape* p, int count, bool symmetric) {
         }
     }
     return best;
+}
+
+// Gram products of few rows and many columns: every tile's columns in `runs` runs, so that all CUs have work, and the runs' sums
+// added by a second launch.  Per product: runs and slabs a run.
+struct MuonRuns {
+    int tile;                    // of kMuonTileTable
+    int64_t runs[kMuonMax], run;
+    int64_t bytes;               // of partial sums, all products
+};
+// The second launch: us at least, us for every 32 runs (8 waves add four at a time), bytes a us of partial sums written and read.
+constexpr float kMuonJoin = 3.2f, kMuonJoinRuns = 1.0f, kMuonJoinRate = 3.0e6f;
+
+// False where one launch without runs is the faster way.
+static inline bool muon_choose_runs(const MuonShape* p, int count, MuonRuns* out) {
+    bool found = false;
+    float least = muon_cost(kMuonTileTable[muon_choose(p, count, true)], p, count, true);
+    for (int k = 0; k < 3; ++k) {
+        const MuonTile& t = kMuonTileTable[k];
+        MuonRuns r;
+        r.tile = k;
+        int64_t units = 0, longest = 0;
+        for (int i = 0; i < count; ++i) {
+            units += muon_tiles(p[i].rows, p[i].cols, t.bm, t.bn, true) * (p[i].k / 32);
+            if (p[i].k / 32 > longest) longest = p[i].k / 32;
+        }
+        for (r.run = (units + kMuonCus - 1) / kMuonCus; r.run < longest; r.run += (r.run + 3) / 4) {
+            int64_t tiles = 0, most = 0;
+            r.bytes = 0;
+            for (int i = 0; i < count; ++i) {
+                const int64_t side = p[i].rows / 32;
+                r.runs[i] = (p[i].k / 32 + r.run - 1) / r.run;
+                if (r.runs[i] > most) most = r.runs[i];
+                tiles += r.runs[i] * muon_tiles(p[i].rows, p[i].cols, t.bm, t.bn, true);
+                r.bytes += r.runs[i] * (side * (side + 1) / 2) * 4096;
+            }
+            const float share = tiles < kMuonCus ? (float)tiles / kMuonCus : 1.f;
+            const float turns = (float)((tiles + kMuonCus - 1) / kMuonCus);
+            const float c = t.start + turns * (float)r.run * (t.alone + (t.full - t.alone) * share) + kMuonJoin +
+                            kMuonJoinRuns * (float)((most + 31) / 32) + (float)r.bytes / kMuonJoinRate;
+            if (c < least) {
+                least = c;
+                *out = r;
+                found = true;
+            }
+        }
+    }
+    return found;
 }
 
 }  // namespace aeth

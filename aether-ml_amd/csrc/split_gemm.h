@@ -22,6 +22,7 @@ enum SplitUse {
     kSplitGram,          // D1 = P Q^T, symmetric
     kSplitPoly,          // D1 = a I + b A + c P Q^T, symmetric (P = Q = A)
     kSplitStep,          // D1 = P Q^T and D2 its transpose
+    kSplitPart,          // part = P Q^T over a run of the columns, symmetric; split_join adds the runs
     kSplitApply,         // theta <- keep theta - step P Q^T, or out = P Q^T; float32, [rows][cols]
 };
 
@@ -33,6 +34,8 @@ struct SplitProduct {
     int rows, cols;      // of theta
     int first;           // this product's first tile
     int tm, tn;          // tiles down and across
+    int runs, run;       // kSplitPart: runs of so many slabs
+    float* part;         // [run][32 x 32 block on or above the diagonal][1024]
     float gain;
 };
 
@@ -66,6 +69,72 @@ __device__ __forceinline__ void split_store(char* p, const unsigned* w) {
     *reinterpret_cast<words*>(p + 64) = lo;
 }
 
+// What a product's accumulators are times the stored result's scale.
+template <int USE>
+__device__ constexpr float split_scale() {
+    return USE == kSplitGram || USE == kSplitPart ? kScaleA / (kScaleX * kScaleX)
+           : USE == kSplitPoly                    ? kNsC * kScaleB / (kScaleA * kScaleA)
+           : USE == kSplitStep                    ? 1.f / kScaleB
+                                                  : 1.f / (kScaleB * kScaleX);
+}
+
+// One 32 x 32 block of the result, at row r and column c, by one wave: o[v] is row r + 8 (v / 4) + 4 (lane / 32) + v % 4, column
+// c + lane % 32, already scaled.  `blk`: LDS of the wave's own.
+template <int USE>
+__device__ __forceinline__ void split_emit(const SplitProduct& pr, float* o, int r, int c, unsigned (*blk)[33]) {
+    constexpr bool kSym = USE != kSplitStep;
+    const int lane = threadIdx.x & 63, l32 = lane & 31, lh = lane >> 5;
+    if (USE == kSplitPoly) {
+        // A[r][c] read as A[c][r]: four consecutive rows a load
+        const char* a = pr.A + ((size_t)(r / 32) * pr.M + c + l32) * 128 + 8 * lh;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const half4 h = *reinterpret_cast<const half4*>(a + 16 * q), l = *reinterpret_cast<const half4*>(a + 16 * q + 64);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[4 * q + e] += ((float)h[e] + (float)l[e]) * (kNsB * kScaleB / kScaleA);
+        }
+        if (r == c)
+#pragma unroll
+            for (int v = 0; v < 16; ++v)
+                if (8 * (v >> 2) + 4 * lh + (v & 3) == l32) o[v] += kNsA * kScaleB;
+    }
+    unsigned w[16];
+#pragma unroll
+    for (int v = 0; v < 16; ++v) w[v] = split_pack(o[v]);
+    // transposed: row c + l32, four consecutive columns a piece (not for diagonal blocks of a symmetric result: each place is
+    // written once, by one lane)
+    if (!(kSym && r == c)) {
+        char* d = (kSym ? pr.D1 : pr.D2) + ((size_t)(r / 32) * pr.N + c + l32) * 128 + 8 * lh;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) split_store<4>(d + 16 * q, w + 4 * q);
+    }
+    // as it is: through LDS, so that a lane has 16 consecutive columns of row r + l32
+#pragma unroll
+    for (int v = 0; v < 16; ++v) blk[8 * (v >> 2) + 4 * lh + (v & 3)][l32] = w[v];
+    __builtin_amdgcn_wave_barrier();
+    char* d = pr.D1 + ((size_t)(c / 32) * pr.M + r + l32) * 128 + 32 * lh;
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+        unsigned s[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s[e] = blk[l32][16 * lh + 8 * q + e];
+        split_store<8>(d + 16 * q, s);
+    }
+    __builtin_amdgcn_wave_barrier();
+}
+
+// The parameters of the product that tile (or workgroup) `tile` of the launch belongs to, by scalar loads from the kernel's
+// arguments, of which the table is the first (an index into the struct itself would copy it to memory).
+__device__ __forceinline__ SplitProduct split_find(const SplitTable& tb, int tile) {
+    typedef const SplitTable __attribute__((address_space(4)))* table_ptr;
+    const table_ptr args = (table_ptr)__builtin_amdgcn_kernarg_segment_ptr();
+    int at = 0;
+    while (at + 1 < tb.count && tile >= args->p[at + 1].first) ++at;
+    SplitProduct pr = tb.p[0];
+    __builtin_memcpy(&pr, (const void*)(args->p + at), sizeof(pr));
+    return pr;
+}
+
 template <int N>
 __device__ __forceinline__ void wait_loads() {           // at most N of this wave's loads are still on their way; its LDS reads are done
     static_assert(N < 64, "vmcnt has six bits");
@@ -85,19 +154,20 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN)) void split_product(cons
     static_assert(AL * 8 * WAVES == BM && BL * 8 * WAVES == BN, "whole loads a wave");
     constexpr int BUF = (BM + BN) * 128;
     static_assert(NBUF * BUF >= WAVES * 32 * 33 * 4, "the epilogue's blocks fit");
-    constexpr bool kSym = USE == kSplitGram || USE == kSplitPoly;
+    constexpr bool kSym = USE == kSplitGram || USE == kSplitPoly || USE == kSplitPart;
     __shared__ __attribute__((aligned(1024))) char lds[NBUF * BUF];
 
     const int tile = xcd_contiguous_id(blockIdx.x, gridDim.x);
-    // the product's numbers by scalar loads from the kernel's arguments (an index into the struct itself would copy it to memory)
-    typedef const SplitTable __attribute__((address_space(4)))* table_ptr;
-    const table_ptr args = (table_ptr)__builtin_amdgcn_kernarg_segment_ptr();
-    int at = 0;
-    while (at + 1 < tb.count && tile >= args->p[at + 1].first) ++at;
-    SplitProduct pr = tb.p[0];
-    __builtin_memcpy(&pr, (const void*)(args->p + at), sizeof(pr));
+    const SplitProduct pr = split_find(tb, tile);
     int ti, tj;
-    if (kSym) {
+    int begin = 0, slabs = pr.K / 32;
+    if (USE == kSplitPart) {
+        // run by run: neighbours in time read the same columns
+        const int triangle = pr.tn * (pr.tn + 1) / 2, run = (tile - pr.first) / triangle;
+        muon_triangle(tile - pr.first - run * triangle, &ti, &tj);
+        begin = run * pr.run;
+        slabs = min(slabs - begin, pr.run);
+    } else if (kSym) {
         muon_triangle(tile - pr.first, &ti, &tj);
     } else {
         // bands of four tile rows, walked column by column: neighbours in time share operands in their XCD's L2
@@ -106,11 +176,11 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN)) void split_product(cons
         tj = in / height;
         ti = band * 4 + in - tj * height;
     }
-    const int K = pr.K, slabs = K / 32;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int l32 = lane & 31, lh = lane >> 5;
     const int r0 = ti * BM, c0 = tj * BN;
-    const char *sp = pr.P + (size_t)r0 * 128, *sq = pr.Q + (size_t)c0 * 128;         // the next slab's rows
+    // the next slab's rows
+    const char *sp = pr.P + ((size_t)begin * pr.M + r0) * 128, *sq = pr.Q + ((size_t)begin * pr.N + c0) * 128;
     const unsigned np = (unsigned)min(pr.M - r0, BM) * 128u, nq = (unsigned)min(pr.N - c0, BN) * 128u;
     const size_t dp = (size_t)pr.M * 128, dq = (size_t)pr.N * 128;
     unsigned vp[AL], vq[BL];                             // (rows behind the matrix are behind the descriptor's end: they read as zeros)
@@ -222,10 +292,7 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN)) void split_product(cons
 
     // block (i, j) of a wave: acc[v] = result[r][c], r = 8 (v / 4) + 4 lh + v % 4, c = l32 of the block
     unsigned(*blk)[33] = reinterpret_cast<unsigned(*)[33]>(lds + wave * (32 * 33 * 4));
-    constexpr float kOut = USE == kSplitGram   ? kScaleA / (kScaleX * kScaleX)
-                           : USE == kSplitPoly ? kNsC * kScaleB / (kScaleA * kScaleA)
-                           : USE == kSplitStep ? 1.f / kScaleB
-                                               : 1.f / (kScaleB * kScaleX);
+    constexpr float kOut = split_scale<USE>();
     if (USE == kSplitApply) {
         if (state != nullptr) lr = (float)state[3];
         const float keep = 1.0f - lr * wd, step = lr * pr.gain;
@@ -260,47 +327,51 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN)) void split_product(cons
             const int r = r0 + wm + 32 * i, c = c0 + wn + 32 * j;
             if (r >= pr.M || c >= pr.N) continue;        // (whole blocks: both are multiples of 32)
             if (kSym && r > c) continue;                 // (below the diagonal of a diagonal tile: written from above it)
-            float o[16];
+            if constexpr (USE == kSplitPart) {
+                const size_t side = pr.M / 32, x = c / 32, block = x * (x + 1) / 2 + r / 32;
+                float* d = pr.part + ((size_t)(begin / pr.run) * (side * (side + 1) / 2) + block) * 1024 + lane * 4;
 #pragma unroll
-            for (int v = 0; v < 16; ++v) o[v] = acc[i][j][v] * kOut;
-            if (USE == kSplitPoly) {
-                // A[r][c] read as A[c][r]: four consecutive rows a load
-                const char* a = pr.A + ((size_t)(r / 32) * pr.M + c + l32) * 128 + 8 * lh;
+                for (int q = 0; q < 4; ++q)
+                    *reinterpret_cast<f4*>(d + 256 * q) = f4{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+            } else if constexpr (USE != kSplitApply) {
+                float o[16];
 #pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const half4 h = *reinterpret_cast<const half4*>(a + 16 * q), l = *reinterpret_cast<const half4*>(a + 16 * q + 64);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) o[4 * q + e] += ((float)h[e] + (float)l[e]) * (kNsB * kScaleB / kScaleA);
-                }
-                if (r == c)
-#pragma unroll
-                    for (int v = 0; v < 16; ++v)
-                        if (8 * (v >> 2) + 4 * lh + (v & 3) == l32) o[v] += kNsA * kScaleB;
+                for (int v = 0; v < 16; ++v) o[v] = acc[i][j][v] * kOut;
+                split_emit<USE>(pr, o, r, c, blk);
             }
-            unsigned w[16];
-#pragma unroll
-            for (int v = 0; v < 16; ++v) w[v] = split_pack(o[v]);
-            // transposed: row c + l32, four consecutive columns a piece (not for diagonal blocks of a symmetric result: each
-            // place is written once, by one lane)
-            if (!(kSym && r == c)) {
-                char* d = (kSym ? pr.D1 : pr.D2) + ((size_t)(r / 32) * pr.N + c + l32) * 128 + 8 * lh;
-#pragma unroll
-                for (int q = 0; q < 4; ++q) split_store<4>(d + 16 * q, w + 4 * q);
-            }
-            // as it is: through LDS, so that a lane has 16 consecutive columns of row r + l32
-#pragma unroll
-            for (int v = 0; v < 16; ++v) blk[8 * (v >> 2) + 4 * lh + (v & 3)][l32] = w[v];
-            __builtin_amdgcn_wave_barrier();
-            char* d = pr.D1 + ((size_t)(c / 32) * pr.M + r + l32) * 128 + 32 * lh;
-#pragma unroll
-            for (int q = 0; q < 2; ++q) {
-                unsigned s[8];
-#pragma unroll
-                for (int e = 0; e < 8; ++e) s[e] = blk[l32][16 * lh + 8 * q + e];
-                split_store<8>(d + 16 * q, s);
-            }
-            __builtin_amdgcn_wave_barrier();
         }
+}
+
+// D1 = the sum of kSplitPart's runs: a 32 x 32 block a workgroup, every eighth run a wave, the waves' sums added in their order.
+__global__ __launch_bounds__(512) void split_join(const SplitTable tb) {
+    __shared__ f4 sums[8][4][64];
+    __shared__ unsigned blk[32][33];
+    const SplitProduct pr = split_find(tb, blockIdx.x);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const int side = pr.M / 32, count = side * (side + 1) / 2, t = (int)blockIdx.x - pr.first;
+    const float* p = pr.part + (size_t)t * 1024 + lane * 4;
+    f4 sum[4] = {};
+    const int runs = pr.runs;
+#pragma unroll 4
+    for (int k = wave; k < runs; k += 8)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) sum[q] += *reinterpret_cast<const f4*>(p + (size_t)k * count * 1024 + 256 * q);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) sums[wave][q][lane] = sum[q];
+    __syncthreads();
+    if (wave != 0) return;
+    float o[16];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        f4 s = sums[0][q][lane];
+#pragma unroll
+        for (int w = 1; w < 8; ++w) s += sums[w][q][lane];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[4 * q + e] = s[e] * split_scale<kSplitGram>();
+    }
+    int i, j;
+    muon_triangle(t, &i, &j);
+    split_emit<kSplitGram>(pr, o, 32 * i, 32 * j, blk);
 }
 
 }  // namespace aeth
