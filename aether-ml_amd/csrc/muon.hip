@@ -150,32 +150,38 @@ static int muon_launch(SplitTable tb, float lr, const double* state, float wd) {
         tb.p[i].tn = cdiv(tb.p[i].N, BN);
         tiles += muon_tiles(tb.p[i].M, tb.p[i].N, BM, BN, kSym) * (USE == kSplitPart ? tb.p[i].runs : 1);
     }
-    hipLaunchKernelGGL((split_product<BM, BN, WM, WN, NBUF, USE>), dim3((unsigned)tiles), dim3(64 * (BM / WM) * (BN / WN)), 0,
-                       ctx().stream, tb, lr, state, wd);
+    if constexpr (BM == 32)
+        hipLaunchKernelGGL((split_block<USE>), dim3((unsigned)tiles), dim3(256), 0, ctx().stream, tb, lr, state, wd);
+    else
+        hipLaunchKernelGGL((split_product<BM, BN, WM, WN, NBUF, USE>), dim3((unsigned)tiles), dim3(64 * (BM / WM) * (BN / WN)), 0,
+                           ctx().stream, tb, lr, state, wd);
     AETH_LAUNCH_CHECK();
+    return AETH_OK;
+}
+
+// (`tile`: kMuonTileTable's order)
+template <int USE>
+static int muon_launch_tile(int tile, const SplitTable& tb, float lr, const double* state, float wd) {
+    constexpr bool kSym = USE == kSplitGram || USE == kSplitPoly;
+    if (tile == 0) return muon_launch<32, 32, 32, 32, 3, USE>(tb, lr, state, wd);
+    if (tile == 1) return muon_launch<64, 64, 32, 32, 4, USE>(tb, lr, state, wd);
+    if (tile == 2) return muon_launch<96, 96, 96, 32, 3, USE>(tb, lr, state, wd);
+    if (USE == kSplitPart || tile == 3) return muon_launch<128, 128, 64, 64, 4, USE>(tb, lr, state, wd);
+    if constexpr (kSym) return muon_launch<192, 192, 96, 96, 3, USE>(tb, lr, state, wd);
+    else if constexpr (USE != kSplitPart) return muon_launch<256, 128, 64, 64, 3, USE>(tb, lr, state, wd);
     return AETH_OK;
 }
 
 template <int USE>
 static int muon_product(const SplitTable& tb, float lr, const double* state, float wd) {
-    // (kMuonTileTable's order)
-    constexpr bool kSym = USE == kSplitGram || USE == kSplitPoly;
     MuonShape shapes[kMuonMax];
     for (int i = 0; i < tb.count; ++i) shapes[i] = MuonShape{tb.p[i].M, tb.p[i].N, tb.p[i].K};
-    const int tile = muon_choose(shapes, tb.count, kSym);
-    if (tile == 0) return muon_launch<64, 64, 32, 32, 4, USE>(tb, lr, state, wd);
-    if (tile == 1) return muon_launch<96, 96, 96, 32, 3, USE>(tb, lr, state, wd);
-    if (tile == 2) return muon_launch<128, 128, 64, 64, 4, USE>(tb, lr, state, wd);
-    if constexpr (kSym) return muon_launch<192, 192, 96, 96, 3, USE>(tb, lr, state, wd);
-    else return muon_launch<256, 128, 64, 64, 3, USE>(tb, lr, state, wd);
+    return muon_launch_tile<USE>(muon_choose(shapes, tb.count, USE == kSplitGram || USE == kSplitPoly), tb, lr, state, wd);
 }
 
 // A = X X^T in runs of its columns.
 static int muon_gram_runs(SplitTable tb, int tile) {
-    int rc;
-    if (tile == 0) rc = muon_launch<64, 64, 32, 32, 4, kSplitPart>(tb, 0.f, nullptr, 0.f);
-    else if (tile == 1) rc = muon_launch<96, 96, 96, 32, 3, kSplitPart>(tb, 0.f, nullptr, 0.f);
-    else rc = muon_launch<128, 128, 64, 64, 4, kSplitPart>(tb, 0.f, nullptr, 0.f);
+    const int rc = muon_launch_tile<kSplitPart>(tile, tb, 0.f, nullptr, 0.f);
     if (rc) return rc;
     int64_t groups = 0;
     for (int i = 0; i < tb.count; ++i) {

@@ -54,22 +54,24 @@ static inline int64_t muon_tiles(int64_t rows, int64_t cols, int bm, int bn, boo
     return symmetric ? tm * (tm + 1) / 2 : tm * tn;
 }
 
-// The tile shapes a product can be cut into, with what a tile costs: `start` us a launch, then us a slab of 32 columns on a CU
-// whose neighbours are idle (`alone`) and with a tile on every CU (`full`: the tiles then share the L2 caches' bandwidth and the
-// power that the matrix units may draw).  Measured on square and wide products of 64 to 4096 rows; a CU takes what its tiles
+// The tile shapes a product can be cut into, with what a tile costs: `start` us a launch, `again` us for every further tile of a
+// CU (its first loads and its epilogue, as far as no other tile hides them), then us a slab of 32 columns on a CU whose neighbours
+// are idle (`alone`) and with a tile on every CU (`full`: the tiles then share the L2 caches' bandwidth and the power that the
+// matrix units may draw).  Measured on square and wide products of 64 to 4096 rows; a CU takes what its tiles
 // cost one after the other, whether they are on it together or not.
 struct MuonTile {
     int bm, bn;
     bool symmetric, general;     // offered for symmetric results, for others
-    float start, alone, full;
+    float start, again, alone, full;
 };
-constexpr int kMuonTiles = 5;
+constexpr int kMuonTiles = 6;
 static const MuonTile kMuonTileTable[kMuonTiles] = {
-    {64, 64, true, true, 3.5f, 0.24f, 0.25f},
-    {96, 96, true, true, 5.0f, 0.41f, 0.50f},
-    {128, 128, true, true, 6.0f, 0.53f, 0.80f},
-    {192, 192, true, false, 8.0f, 1.05f, 1.45f},
-    {256, 128, false, true, 7.0f, 0.95f, 1.17f},
+    {32, 32, true, true, 3.0f, 2.5f, 0.10f, 0.12f},
+    {64, 64, true, true, 3.5f, 0.5f, 0.24f, 0.25f},
+    {96, 96, true, true, 5.0f, 1.0f, 0.41f, 0.50f},
+    {128, 128, true, true, 5.0f, 1.0f, 0.53f, 0.80f},
+    {192, 192, true, false, 8.0f, 2.0f, 1.05f, 1.45f},
+    {256, 128, false, true, 7.0f, 2.0f, 0.95f, 1.17f},
 };
 constexpr int kMuonCus = 256;
 
@@ -89,7 +91,8 @@ static inline float muon_cost(const MuonTile& t, const MuonShape* p, int count, 
         if (mine > longest) longest = mine;
     }
     const float even = (float)slabs / kMuonCus, share = tiles < kMuonCus ? (float)tiles / kMuonCus : 1.f;
-    return t.start + (longest > even ? longest : even) * (t.alone + (t.full - t.alone) * share);
+    const float more = (float)((tiles + kMuonCus - 1) / kMuonCus - 1);
+    return t.start + t.again * more + (longest > even ? longest : even) * (t.alone + (t.full - t.alone) * share);
 }
 
 static inline int muon_choose(const MuonShape* p, int count, bool symmetric) {
@@ -120,7 +123,7 @@ constexpr float kMuonJoin = 3.2f, kMuonJoinRuns = 1.0f, kMuonJoinRate = 3.0e6f;
 static inline bool muon_choose_runs(const MuonShape* p, int count, MuonRuns* out) {
     bool found = false;
     float least = muon_cost(kMuonTileTable[muon_choose(p, count, true)], p, count, true);
-    for (int k = 0; k < 3; ++k) {
+    for (int k = 0; k < 4; ++k) {
         const MuonTile& t = kMuonTileTable[k];
         MuonRuns r;
         r.tile = k;
@@ -141,7 +144,7 @@ static inline bool muon_choose_runs(const MuonShape* p, int count, MuonRuns* out
             }
             const float share = tiles < kMuonCus ? (float)tiles / kMuonCus : 1.f;
             const float turns = (float)((tiles + kMuonCus - 1) / kMuonCus);
-            const float c = t.start + turns * (float)r.run * (t.alone + (t.full - t.alone) * share) + kMuonJoin +
+            const float c = t.start + t.again * (turns - 1.f) + turns * (float)r.run * (t.alone + (t.full - t.alone) * share) + kMuonJoin +
                             kMuonJoinRuns * (float)((most + 31) / 32) + (float)r.bytes / kMuonJoinRate;
             if (c < least) {
                 least = c;

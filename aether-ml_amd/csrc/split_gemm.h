@@ -138,7 +138,70 @@ __device__ __forceinline__ SplitProduct split_find(const SplitTable& tb, int til
 template <int N>
 __device__ __forceinline__ void wait_loads() {           // at most N of this wave's loads are still on their way; its LDS reads are done
     static_assert(N < 64, "vmcnt has six bits");
+    asm volatile("" ::: "memory");                       // (the compiler keeps its reads of the LDS on their side)
     __builtin_amdgcn_s_waitcnt((N & 15) | (7 << 4) | (0 << 8) | ((N >> 4) << 14));
+    asm volatile("" ::: "memory");
+}
+
+// The tile of the result that number `t` of a product's tiles is, and the slabs it adds up.
+struct SplitTile {
+    int i, j, begin, slabs;
+};
+template <int USE>
+__device__ __forceinline__ SplitTile split_tile(const SplitProduct& pr, int t) {
+    SplitTile at{0, 0, 0, pr.K / 32};
+    if (USE == kSplitPart) {
+        // run by run: neighbours in time read the same columns
+        const int triangle = pr.tn * (pr.tn + 1) / 2, run = t / triangle;
+        muon_triangle(t - run * triangle, &at.i, &at.j);
+        at.begin = run * pr.run;
+        at.slabs = min(at.slabs - at.begin, pr.run);
+    } else if (USE == kSplitGram || USE == kSplitPoly) {
+        muon_triangle(t, &at.i, &at.j);
+    } else {
+        // bands of four tile rows, walked column by column: neighbours in time share operands in their XCD's L2
+        const int band = t / (4 * pr.tn), in = t - band * 4 * pr.tn;
+        const int height = min(4, pr.tm - band * 4);
+        at.j = in / height;
+        at.i = band * 4 + in - at.j * height;
+    }
+    return at;
+}
+
+// One 32 x 32 block of a product's accumulators to where the product's use wants it; the block is inside the padded result.
+template <int USE>
+__device__ __forceinline__ void split_finish(const SplitProduct& pr, const f16v& acc, int r, int c, const SplitTile& at,
+                                             unsigned (*blk)[33], float keep, float step) {
+    const int lane = threadIdx.x & 63, l32 = lane & 31, lh = lane >> 5;
+    constexpr float kOut = split_scale<USE>();
+    if constexpr (USE == kSplitApply) {
+        // (all the loads at once, from places clamped into the matrix: behind a branch each they came back one by one)
+        const int x = c + l32, cc = min(x, pr.cols - 1), y0 = r + 4 * lh;
+        float t[16];
+        if (pr.theta != nullptr) {
+#pragma unroll
+            for (int v = 0; v < 16; ++v) t[v] = pr.theta[(size_t)min(y0 + 8 * (v >> 2) + (v & 3), pr.rows - 1) * pr.cols + cc];
+        }
+#pragma unroll
+        for (int v = 0; v < 16; ++v) {
+            const int y = y0 + 8 * (v >> 2) + (v & 3);
+            if (y < pr.rows && x < pr.cols) {
+                const float o = acc[v] * kOut;
+                if (pr.theta != nullptr) pr.theta[(size_t)y * pr.cols + x] = keep * t[v] - step * o;
+                else pr.out[(size_t)y * pr.cols + x] = o;
+            }
+        }
+    } else if constexpr (USE == kSplitPart) {
+        const size_t side = pr.M / 32, x = c / 32, block = x * (x + 1) / 2 + r / 32;
+        float* d = pr.part + ((size_t)(at.begin / pr.run) * (side * (side + 1) / 2) + block) * 1024 + lane * 4;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) *reinterpret_cast<f4*>(d + 256 * q) = f4{acc[4 * q], acc[4 * q + 1], acc[4 * q + 2], acc[4 * q + 3]};
+    } else {
+        float o[16];
+#pragma unroll
+        for (int v = 0; v < 16; ++v) o[v] = acc[v] * kOut;
+        split_emit<USE>(pr, o, r, c, blk);
+    }
 }
 
 // A matrix lies slab by slab: slab s holds columns 32 s .. 32 s + 31 of all R rows, row r's 128 bytes (64 of high halves, 64 of low)
@@ -159,28 +222,13 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN)) void split_product(cons
 
     const int tile = xcd_contiguous_id(blockIdx.x, gridDim.x);
     const SplitProduct pr = split_find(tb, tile);
-    int ti, tj;
-    int begin = 0, slabs = pr.K / 32;
-    if (USE == kSplitPart) {
-        // run by run: neighbours in time read the same columns
-        const int triangle = pr.tn * (pr.tn + 1) / 2, run = (tile - pr.first) / triangle;
-        muon_triangle(tile - pr.first - run * triangle, &ti, &tj);
-        begin = run * pr.run;
-        slabs = min(slabs - begin, pr.run);
-    } else if (kSym) {
-        muon_triangle(tile - pr.first, &ti, &tj);
-    } else {
-        // bands of four tile rows, walked column by column: neighbours in time share operands in their XCD's L2
-        const int t = tile - pr.first, band = t / (4 * pr.tn), in = t - band * 4 * pr.tn;
-        const int height = min(4, pr.tm - band * 4);
-        tj = in / height;
-        ti = band * 4 + in - tj * height;
-    }
+    const SplitTile at = split_tile<USE>(pr, tile - pr.first);
+    const int slabs = at.slabs;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int l32 = lane & 31, lh = lane >> 5;
-    const int r0 = ti * BM, c0 = tj * BN;
+    const int r0 = at.i * BM, c0 = at.j * BN;
     // the next slab's rows
-    const char *sp = pr.P + ((size_t)begin * pr.M + r0) * 128, *sq = pr.Q + ((size_t)begin * pr.N + c0) * 128;
+    const char *sp = pr.P + ((size_t)at.begin * pr.M + r0) * 128, *sq = pr.Q + ((size_t)at.begin * pr.N + c0) * 128;
     const unsigned np = (unsigned)min(pr.M - r0, BM) * 128u, nq = (unsigned)min(pr.N - c0, BN) * 128u;
     const size_t dp = (size_t)pr.M * 128, dq = (size_t)pr.N * 128;
     unsigned vp[AL], vq[BL];                             // (rows behind the matrix are behind the descriptor's end: they read as zeros)
@@ -292,34 +340,8 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN)) void split_product(cons
 
     // block (i, j) of a wave: acc[v] = result[r][c], r = 8 (v / 4) + 4 lh + v % 4, c = l32 of the block
     unsigned(*blk)[33] = reinterpret_cast<unsigned(*)[33]>(lds + wave * (32 * 33 * 4));
-    constexpr float kOut = split_scale<USE>();
-    if (USE == kSplitApply) {
-        if (state != nullptr) lr = (float)state[3];
-        const float keep = 1.0f - lr * wd, step = lr * pr.gain;
-#pragma unroll
-        for (int i = 0; i < TM; ++i)
-#pragma unroll
-            for (int j = 0; j < TN; ++j) {
-                // (all the loads of a block at once, from places clamped into the matrix: behind a branch each they came back
-                // one by one)
-                const int c = c0 + wn + 32 * j + l32, cc = min(c, pr.cols - 1), r = r0 + wm + 32 * i + 4 * lh;
-                float t[16];
-                if (pr.theta != nullptr) {
-#pragma unroll
-                    for (int v = 0; v < 16; ++v) t[v] = pr.theta[(size_t)min(r + 8 * (v >> 2) + (v & 3), pr.rows - 1) * pr.cols + cc];
-                }
-#pragma unroll
-                for (int v = 0; v < 16; ++v) {
-                    const int y = r + 8 * (v >> 2) + (v & 3);
-                    if (y < pr.rows && c < pr.cols) {
-                        const float o = acc[i][j][v] * kOut;
-                        if (pr.theta != nullptr) pr.theta[(size_t)y * pr.cols + c] = keep * t[v] - step * o;
-                        else pr.out[(size_t)y * pr.cols + c] = o;
-                    }
-                }
-            }
-        return;
-    }
+    if (state != nullptr) lr = (float)state[3];
+    const float keep = 1.0f - lr * wd, step = lr * pr.gain;
 #pragma unroll
     for (int i = 0; i < TM; ++i)
 #pragma unroll
@@ -327,19 +349,87 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN)) void split_product(cons
             const int r = r0 + wm + 32 * i, c = c0 + wn + 32 * j;
             if (r >= pr.M || c >= pr.N) continue;        // (whole blocks: both are multiples of 32)
             if (kSym && r > c) continue;                 // (below the diagonal of a diagonal tile: written from above it)
-            if constexpr (USE == kSplitPart) {
-                const size_t side = pr.M / 32, x = c / 32, block = x * (x + 1) / 2 + r / 32;
-                float* d = pr.part + ((size_t)(begin / pr.run) * (side * (side + 1) / 2) + block) * 1024 + lane * 4;
-#pragma unroll
-                for (int q = 0; q < 4; ++q)
-                    *reinterpret_cast<f4*>(d + 256 * q) = f4{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
-            } else if constexpr (USE != kSplitApply) {
-                float o[16];
-#pragma unroll
-                for (int v = 0; v < 16; ++v) o[v] = acc[i][j][v] * kOut;
-                split_emit<USE>(pr, o, r, c, blk);
-            }
+            split_finish<USE>(pr, acc[i][j], r, c, at, blk, keep, step);
         }
+}
+
+// The same for products so small that a launch's time is what its loads and its epilogue take one after the other: a 32 x 32
+// block a workgroup, every fourth slab a wave, which loads and reads its own ring without a barrier; the waves' sums are added in
+// their order.  256 x 256 x 256: 4.5 us where 64 x 64 tiles take 7.1.
+template <int USE>
+__global__ __launch_bounds__(256) void split_block(const SplitTable tb, float lr, const double* __restrict__ state, float wd) {
+    constexpr int NBUF = 3, BUF = 64 * 128;
+    __shared__ __attribute__((aligned(1024))) char lds[4 * NBUF * BUF];
+    const int tile = xcd_contiguous_id(blockIdx.x, gridDim.x);
+    const SplitProduct pr = split_find(tb, tile);
+    const SplitTile at = split_tile<USE>(pr, tile - pr.first);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const int l32 = lane & 31, lh = lane >> 5, r0 = at.i * 32, c0 = at.j * 32;
+    const char *sp = pr.P + ((size_t)(at.begin + wave) * pr.M + r0) * 128, *sq = pr.Q + ((size_t)(at.begin + wave) * pr.N + c0) * 128;
+    const size_t dp = (size_t)pr.M * 512, dq = (size_t)pr.N * 512;
+    const int slabs = (at.slabs - wave + 3) / 4;         // this wave's (none for a wave behind the last slab)
+    unsigned off[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const unsigned r = (unsigned)i * 8 + (lane >> 3);
+        off[i] = r * 128u + (((unsigned)lane & 7u) ^ ((r >> 1) & 7u)) * 16u;
+    }
+    char* ring = lds + wave * (NBUF * BUF);
+    const unsigned ring0 = lds_address(ring);
+    const auto fetch = [&](int buf) {
+        const u32x4 rp = raw_rsrc(sp, 32 * 128), rq = raw_rsrc(sq, 32 * 128);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) lds_direct_load16(rp, ring0 + (unsigned)buf * BUF + i * 1024u, off[i]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) lds_direct_load16(rq, ring0 + (unsigned)buf * BUF + 4096u + i * 1024u, off[i]);
+        sp += dp;
+        sq += dq;
+    };
+    f16v acc;
+#pragma unroll
+    for (int v = 0; v < 16; ++v) acc[v] = 0.f;
+    const unsigned f0 = (unsigned)l32 * 128u + (unsigned)(lh ^ ((l32 >> 1) & 7)) * 16u;
+    const auto multiply = [&](int buf) {
+        const char* b = ring + buf * BUF;
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            const half8 ah = *reinterpret_cast<const half8*>(b + (f0 ^ (t * 32u))), al = *reinterpret_cast<const half8*>(b + (f0 ^ (t * 32u + 64u)));
+            const half8 bh = *reinterpret_cast<const half8*>(b + 4096 + (f0 ^ (t * 32u))), bl = *reinterpret_cast<const half8*>(b + 4096 + (f0 ^ (t * 32u + 64u)));
+            acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah, bl, acc, 0, 0, 0);
+            acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(al, bh, acc, 0, 0, 0);
+            acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah, bh, acc, 0, 0, 0);
+        }
+    };
+#pragma unroll
+    for (int d = 0; d < NBUF - 1; ++d)
+        if (d < slabs) fetch(d);
+    int buf = 0, next = NBUF - 1;
+    for (int s = 0; s < slabs; ++s) {
+        // slab s has landed, and what was read of the slab before is in registers: its buffer takes the slab after next
+        if (s + 1 < slabs) wait_loads<8 * (NBUF - 2)>();
+        else wait_loads<0>();
+        if (s + NBUF - 1 < slabs) fetch(next);
+        multiply(buf);
+        buf = buf + 1 == NBUF ? 0 : buf + 1;
+        next = next + 1 == NBUF ? 0 : next + 1;
+    }
+    // (every wave's loads have landed and its reads are done where it writes its sums: over its own ring)
+    wait_loads<0>();
+    f4* sums = reinterpret_cast<f4*>(ring);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) sums[64 * q + lane] = f4{acc[4 * q], acc[4 * q + 1], acc[4 * q + 2], acc[4 * q + 3]};
+    __syncthreads();
+    if (wave != 0) return;
+#pragma unroll
+    for (int w = 1; w < 4; ++w)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const f4 s = reinterpret_cast<const f4*>(lds + w * (NBUF * BUF))[64 * q + lane];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[4 * q + e] += s[e];
+        }
+    if (state != nullptr) lr = (float)state[3];
+    split_finish<USE>(pr, acc, r0, c0, at, reinterpret_cast<unsigned(*)[33]>(ring + 4096), 1.0f - lr * wd, lr * pr.gain);
 }
 
 // D1 = the sum of kSplitPart's runs: a 32 x 32 block a workgroup, every eighth run a wave, the waves' sums added in their order.
