@@ -139,6 +139,296 @@ __global__ __launch_bounds__(256) void muon_split(const MuonTable tb, float mu, 
     }
 }
 
+// ---- small matrices: the whole update in one workgroup -------------------------------------------------------------------
+// For matrices of at most 64 rows (the shorter side) and few columns, whose chain of seventeen launches of 4 us each is all that
+// the update costs.  X stays in the registers of 8 waves as packed halves: wave w has the 32-column blocks w, w + 8, ..., a lane
+// one column j of a block and of each 32-row block the 16 rows i that an MFMA's result has in a lane.  So the result of a step,
+// B X with a column a lane, is the next step's operand as it is, with B's columns stored in the order in which a lane has its
+// rows (muon_slot); X X^T needs a row a lane, which a wave turns round through LDS of its own.  The waves' parts of A are added
+// in their order, A^2 is 1 or 3 blocks, and the weights take the last step's result from the accumulators.
+// Bound: latency, 3 us a step on 64 x 64 and 7 on 64 x 576 (its MFMAs 2.5), and what one CU loads and stores.
+constexpr int kWholeWaves = 8, kWholePitch = 72;         // halves of a row of A and B: 16-byte reads of 8 rows in different banks
+
+// Where column k of B stands in its row: a lane's 8 values of a 16-column step are rows 4 h + e and 8 + 4 h + e.
+__device__ __forceinline__ int muon_slot(int k) { return (k & ~15) | (k & 4) << 1 | (k & 8) >> 1 | (k & 3); }
+
+__device__ __forceinline__ void whole_split(const float* v, half4& hi, half4& lo) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const _Float16 h = (_Float16)v[e];
+        hi[e] = h;
+        lo[e] = (_Float16)(v[e] - (float)h);
+    }
+}
+
+__device__ __forceinline__ void whole_halves(const unsigned* w, half8& hi, half8& lo) {
+    typedef unsigned u4 __attribute__((ext_vector_type(4)));
+    u4 h, l;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        h[e] = __builtin_amdgcn_perm(w[2 * e + 1], w[2 * e], 0x05040100u);
+        l[e] = __builtin_amdgcn_perm(w[2 * e + 1], w[2 * e], 0x07060302u);
+    }
+    hi = __builtin_bit_cast(half8, h);
+    lo = __builtin_bit_cast(half8, l);
+}
+
+__device__ __forceinline__ f16v whole_mfma(const half8& ah, const half8& al, const half8& bh, const half8& bl, f16v acc) {
+    acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah, bl, acc, 0, 0, 0);
+    acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(al, bh, acc, 0, 0, 0);
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(ah, bh, acc, 0, 0, 0);
+}
+
+// MB 32-row blocks, CB column blocks a wave; kUpdate: a step of weights with momentum, else the orthogonalisation alone.
+template <int MB, int CB, bool kUpdate>
+__global__ __launch_bounds__(64 * kWholeWaves) void muon_whole(const MuonTable tb, float mu, int nesterov, float lr,
+                                                              const double* __restrict__ state, float wd, int steps) {
+    constexpr int NP = MB * (MB + 1) / 2;                // blocks of A on and above the diagonal
+    constexpr int REGION = (NP > 2 ? NP * 4096 : 9216);  // a wave's: X turned round (32 MB rows of 36 words), or its part of A
+    static_assert(REGION >= 32 * MB * 36 * 4 && REGION >= NP * 4096, "both fit");
+    __shared__ __attribute__((aligned(16))) char regions[kWholeWaves][REGION];
+    __shared__ __attribute__((aligned(16))) _Float16 a_hi[32 * MB][kWholePitch], a_lo[32 * MB][kWholePitch];
+    __shared__ __attribute__((aligned(16))) _Float16 b_hi[32 * MB][kWholePitch], b_lo[32 * MB][kWholePitch];
+    __shared__ double red[kWholeWaves];
+    const muon_table_ptr args = (muon_table_ptr)__builtin_amdgcn_kernarg_segment_ptr();
+    const int k = blockIdx.x;
+    const float* __restrict__ grad = args->t[k].grad;
+    float* mom = args->t[k].mom;
+    float* theta = args->t[k].theta;
+    float* out = args->t[k].out;
+    const int rows = args->t[k].rows, cols = args->t[k].cols;
+    const bool tall = rows > cols;
+    const int m = tall ? cols : rows, n = tall ? rows : cols, blocks = (n + 31) / 32, busy = min(blocks, kWholeWaves);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, l32 = lane & 31, lh = lane >> 5;
+    char* region = regions[wave];
+
+    // Element (i, j) of X is at si i + sj j of the matrix's memory: a part of the lane's own and a part that is the same for all.
+    // Places behind the matrix's end are cut off by the descriptors, other places that are no element are masked.
+    const int bytes = rows * cols * 4;
+    const auto rsrc = [&](const float* q) { return __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(q), 0, bytes, 0x00020000); };
+    const auto row = [&](int ib, int v) { return 32 * ib + 8 * (v >> 2) + 4 * lh + (v & 3); };
+    const auto column = [&](int cb) { return 32 * (wave + kWholeWaves * cb) + l32; };
+    const auto inside = [&](int cb, int ib, int v) { return row(ib, v) < m && column(cb) < n; };
+    // byte offset of a block's element; the strides pass through the asm so that the compiler works offsets out where they are used
+    // rather than keep one for every element from phase to phase
+    const auto offsets = [&](int cb, int ib, auto use) {
+        int si = tall ? 4 : 4 * cols, sj = tall ? 4 * cols : 4;
+        asm volatile("" : "+s"(si), "+s"(sj));
+        const int at = si * (32 * ib + 4 * lh) + sj * column(cb);
+        use([&](int v) { return at + si * (8 * (v >> 2) + (v & 3)); });
+    };
+    typedef unsigned u4 __attribute__((ext_vector_type(4)));
+    // a lane's 16 elements of a block; of a tall matrix four neighbours at a time
+    const auto load = [&](const __amdgpu_buffer_rsrc_t& q, int cb, int ib, unsigned* d) {
+        offsets(cb, ib, [&](auto at) {
+            if (tall) {
+#pragma unroll
+                for (int v = 0; v < 16; v += 4) {
+                    const u4 t = __builtin_bit_cast(u4, __builtin_amdgcn_raw_buffer_load_b128(q, at(v), 0, 0));
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) d[v + e] = t[e];
+                }
+            } else {
+#pragma unroll
+                for (int v = 0; v < 16; ++v) d[v] = __builtin_amdgcn_raw_buffer_load_b32(q, at(v), 0, 0);
+            }
+        });
+    };
+    const auto store = [&](const __amdgpu_buffer_rsrc_t& q, int cb, int ib, const unsigned* d) {
+        offsets(cb, ib, [&](auto at) {
+            if (tall && m % 4 == 0) {                    // (groups of four rows are in or out as one)
+#pragma unroll
+                for (int v = 0; v < 16; v += 4)
+                    __builtin_amdgcn_raw_buffer_store_b128(u4{d[v], d[v + 1], d[v + 2], d[v + 3]}, q, inside(cb, ib, v) ? at(v) : -1, 0, 0);
+            } else {
+#pragma unroll
+                for (int v = 0; v < 16; ++v) __builtin_amdgcn_raw_buffer_store_b32(d[v], q, inside(cb, ib, v) ? at(v) : -1, 0, 0);
+            }
+        });
+    };
+
+    unsigned w[CB][MB][16];                              // X: first u, float32, then packed halves
+    const __amdgpu_buffer_rsrc_t gr = rsrc(grad), mr = rsrc(mom);
+#pragma unroll
+    for (int cb = 0; cb < CB; ++cb)
+#pragma unroll
+        for (int ib = 0; ib < MB; ++ib) load(gr, cb, ib, w[cb][ib]);
+    unsigned old[2][16];                                 // the momentum, a block ahead
+    if (kUpdate) load(mr, 0, 0, old[0]);
+    double sum = 0.0;
+#pragma unroll
+    for (int b = 0; b < CB * MB; ++b) {
+        const int cb = b / MB, ib = b % MB;
+        if (kUpdate && b + 1 < CB * MB) load(mr, (b + 1) / MB, (b + 1) % MB, old[(b + 1) & 1]);
+        unsigned now[16];
+#pragma unroll
+        for (int v = 0; v < 16; ++v) {
+            float u = __uint_as_float(w[cb][ib][v]);
+            if (kUpdate) {
+                const float x = fmaf(mu, __uint_as_float(old[b & 1][v]), u);
+                now[v] = __float_as_uint(x);
+                u = muon_update(u, x, mu, nesterov);
+            }
+            u = inside(cb, ib, v) ? u : 0.f;
+            sum += (double)u * (double)u;
+            w[cb][ib][v] = __float_as_uint(u);
+        }
+        if (kUpdate) store(mr, cb, ib, now);
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
+    if (lane == 0) red[wave] = sum;
+    __syncthreads();
+    sum = 0.0;
+#pragma unroll
+    for (int i = 0; i < kWholeWaves; ++i) sum += red[i];
+    int power = 0;
+    const float factor = sum != 0.0 ? (float)frexp((double)kScaleX / sqrt(sum), &power) : 0.f;
+#pragma unroll
+    for (int cb = 0; cb < CB; ++cb)
+#pragma unroll
+        for (int ib = 0; ib < MB; ++ib)
+#pragma unroll
+            for (int v = 0; v < 16; ++v) w[cb][ib][v] = split_pack(ldexpf(__uint_as_float(w[cb][ib][v]), power) * factor);
+
+    if (state != nullptr) lr = (float)state[3];
+    const float keep = 1.0f - lr * wd, step = lr * args->t[k].gain;
+    for (int s = 0; s < steps; ++s) {
+        {   // A = X X^T: this wave's columns
+            f16v acc[NP];
+#pragma unroll
+            for (int p = 0; p < NP; ++p)
+#pragma unroll
+                for (int v = 0; v < 16; ++v) acc[p][v] = 0.f;
+            unsigned(*turned)[36] = reinterpret_cast<unsigned(*)[36]>(region);
+#pragma unroll
+            for (int cb = 0; cb < CB; ++cb) {
+                if (wave + kWholeWaves * cb >= blocks) continue;
+#pragma unroll
+                for (int ib = 0; ib < MB; ++ib)
+#pragma unroll
+                    for (int v = 0; v < 16; ++v) turned[row(ib, v)][l32] = w[cb][ib][v];
+                __builtin_amdgcn_wave_barrier();
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    half8 h[MB], l[MB];
+#pragma unroll
+                    for (int ib = 0; ib < MB; ++ib) {
+                        const u4* q = reinterpret_cast<const u4*>(&turned[32 * ib + l32][16 * t + 8 * lh]);
+                        const u4 x = q[0], y = q[1];
+                        const unsigned z[8] = {x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
+                        whole_halves(z, h[ib], l[ib]);
+                    }
+                    acc[0] = whole_mfma(h[0], l[0], h[0], l[0], acc[0]);
+                    if constexpr (MB == 2) {
+                        acc[1] = whole_mfma(h[0], l[0], h[1], l[1], acc[1]);
+                        acc[2] = whole_mfma(h[1], l[1], h[1], l[1], acc[2]);
+                    }
+                }
+                __builtin_amdgcn_wave_barrier();
+            }
+            f4* part = reinterpret_cast<f4*>(region);
+#pragma unroll
+            for (int p = 0; p < NP; ++p)
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                    part[(p * 4 + q) * 64 + lane] = f4{acc[p][4 * q], acc[p][4 * q + 1], acc[p][4 * q + 2], acc[p][4 * q + 3]};
+        }
+        __syncthreads();
+        for (int e = threadIdx.x; e < NP * 256; e += 64 * kWholeWaves) {
+            f4 a = reinterpret_cast<const f4*>(regions[0])[e];
+            for (int i = 1; i < busy; ++i) a += reinterpret_cast<const f4*>(regions[i])[e];
+            const int p = e >> 8, q = (e >> 6) & 3, ln = e & 63;
+            const int ib = p == 2 ? 1 : 0, jb = p == 0 ? 0 : 1;         // (0, 0), (0, 1), (1, 1)
+            const int r = 32 * ib + 8 * q + 4 * (ln >> 5), c = 32 * jb + (ln & 31);
+            half4 hi, lo;
+            const float x[4] = {a[0] * split_scale<kSplitGram>(), a[1] * split_scale<kSplitGram>(), a[2] * split_scale<kSplitGram>(),
+                                a[3] * split_scale<kSplitGram>()};
+            whole_split(x, hi, lo);
+            *reinterpret_cast<half4*>(&a_hi[c][r]) = hi;
+            *reinterpret_cast<half4*>(&a_lo[c][r]) = lo;
+            if (ib != jb)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    a_hi[r + i][c] = hi[i];
+                    a_lo[r + i][c] = lo[i];
+                }
+        }
+        __syncthreads();
+        if (wave < MB * MB) {                            // B = a I + b A + c A^2, a block a wave
+            const int ib = wave / MB, jb = wave % MB;
+            f16v acc, low;                               // high.high; the two with a low half
+#pragma unroll
+            for (int v = 0; v < 16; ++v) acc[v] = low[v] = 0.f;
+#pragma unroll
+            for (int t = 0; t < 2 * MB; ++t) {
+                const int x = 16 * t + 8 * lh;
+                const half8 ah = *reinterpret_cast<const half8*>(&a_hi[32 * ib + l32][x]), al = *reinterpret_cast<const half8*>(&a_lo[32 * ib + l32][x]);
+                const half8 bh = *reinterpret_cast<const half8*>(&a_hi[32 * jb + l32][x]), bl = *reinterpret_cast<const half8*>(&a_lo[32 * jb + l32][x]);
+                low = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah, bl, low, 0, 0, 0);
+                acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah, bh, acc, 0, 0, 0);
+                low = __builtin_amdgcn_mfma_f32_32x32x16_f16(al, bh, low, 0, 0, 0);
+            }
+            const int c = 32 * jb + l32;
+#pragma unroll
+            for (int v = 0; v < 16; v += 4) {
+                const int r = row(ib, v);
+                const half4 ah = *reinterpret_cast<const half4*>(&a_hi[c][r]), al = *reinterpret_cast<const half4*>(&a_lo[c][r]);
+                half4 hi, lo;
+                float b[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    b[e] = (acc[v + e] + low[v + e]) * split_scale<kSplitPoly>() + ((float)ah[e] + (float)al[e]) * (kNsB * kScaleB / kScaleA);
+                    if (r + e == c) b[e] += kNsA * kScaleB;
+                }
+                whole_split(b, hi, lo);
+                *reinterpret_cast<half4*>(&b_hi[c][muon_slot(r)]) = hi;
+                *reinterpret_cast<half4*>(&b_lo[c][muon_slot(r)]) = lo;
+            }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int cb = 0; cb < CB; ++cb) {                // X = B X
+            if (wave + kWholeWaves * cb >= blocks) continue;
+            f16v acc[MB];
+#pragma unroll
+            for (int ib = 0; ib < MB; ++ib)
+#pragma unroll
+                for (int v = 0; v < 16; ++v) acc[ib][v] = 0.f;
+#pragma unroll
+            for (int t = 0; t < 2 * MB; ++t) {
+                half8 xh, xl;
+                whole_halves(&w[cb][t >> 1][8 * (t & 1)], xh, xl);
+#pragma unroll
+                for (int ib = 0; ib < MB; ++ib) {
+                    const half8 bh = *reinterpret_cast<const half8*>(&b_hi[32 * ib + l32][16 * t + 8 * lh]);
+                    const half8 bl = *reinterpret_cast<const half8*>(&b_lo[32 * ib + l32][16 * t + 8 * lh]);
+                    acc[ib] = whole_mfma(bh, bl, xh, xl, acc[ib]);
+                }
+            }
+            if (s + 1 < steps) {
+#pragma unroll
+                for (int ib = 0; ib < MB; ++ib)
+#pragma unroll
+                    for (int v = 0; v < 16; ++v) w[cb][ib][v] = split_pack(acc[ib][v] * split_scale<kSplitStep>());
+                continue;
+            }
+#pragma unroll
+            for (int ib = 0; ib < MB; ++ib) {
+                const __amdgpu_buffer_rsrc_t d = rsrc(kUpdate ? theta : out);
+                unsigned t[16];
+                if (kUpdate) load(d, cb, ib, t);
+#pragma unroll
+                for (int v = 0; v < 16; ++v) {
+                    const float o = acc[ib][v] * split_scale<kSplitApply>();
+                    t[v] = __float_as_uint(kUpdate ? keep * __uint_as_float(t[v]) - step * o : o);
+                }
+                store(d, cb, ib, t);
+            }
+        }
+    }
+}
+
 // One launch for one product of every matrix, in tiles of BM x BN.
 template <int BM, int BN, int WM, int WN, int NBUF, int USE>
 static int muon_launch(SplitTable tb, float lr, const double* state, float wd) {
@@ -270,10 +560,47 @@ static int muon_group(const MuonMatrix* t, int count, float lr, const double* st
     return AETH_OK;
 }
 
+// The column blocks a wave of muon_whole would have, 0 where a matrix is too large for it.  Its registers hold six blocks of 32 x 32 a
+// wave, and that is also where the launches of all CUs catch up: five steps on 64 rows take 22 us at 64 columns, 29 at 256, 55 at
+// 576 and 74 at 1024 in one workgroup, 71 to 76 in launches.
+static int muon_whole_blocks(const MuonMatrix* t, int count, int* row_blocks) {
+    int m = 0, n = 0;
+    for (int i = 0; i < count; ++i) {
+        const int lo = t[i].rows < t[i].cols ? t[i].rows : t[i].cols, hi = t[i].rows < t[i].cols ? t[i].cols : t[i].rows;
+        if (lo > m) m = lo;
+        if (hi > n) n = hi;
+    }
+    *row_blocks = cdiv(m, 32);
+    const int blocks = cdiv(cdiv(n, 32), kWholeWaves);
+    return *row_blocks <= 2 && blocks * *row_blocks <= 6 ? blocks : 0;
+}
+
+static int muon_small(const MuonMatrix* t, int count, int row_blocks, int blocks, float lr, const double* state, float mu,
+                      int nesterov, float wd, int steps) {
+    typedef void (*Whole)(const MuonTable, float, int, float, const double*, float, int);
+    static const Whole one[2][4] = {{muon_whole<1, 1, false>, muon_whole<1, 2, false>, muon_whole<1, 4, false>, muon_whole<1, 6, false>},
+                                    {muon_whole<1, 1, true>, muon_whole<1, 2, true>, muon_whole<1, 4, true>, muon_whole<1, 6, true>}};
+    static const Whole two[2][3] = {{muon_whole<2, 1, false>, muon_whole<2, 2, false>, muon_whole<2, 3, false>},
+                                    {muon_whole<2, 1, true>, muon_whole<2, 2, true>, muon_whole<2, 3, true>}};
+    MuonTable tb = {};
+    tb.count = count;
+    for (int i = 0; i < count; ++i) tb.t[i] = t[i];
+    const int c = blocks <= 1 ? 0 : blocks <= 2 ? 1 : blocks <= 4 ? 2 : 3;
+    const int update = t[0].mom != nullptr;
+    hipLaunchKernelGGL(row_blocks == 1 ? one[update][c] : two[update][c], dim3(count), dim3(64 * kWholeWaves), 0, ctx().stream, tb, mu, nesterov, lr,
+                       state, wd, steps);
+    AETH_LAUNCH_CHECK();
+    return AETH_OK;
+}
+
 // Matrices whose buffers together pass this go out in several groups, one after the other.
 constexpr int64_t kMuonWorkspace = (int64_t)4 << 30;
 
 static int muon_run(MuonMatrix* t, int count, float lr, const double* state, float mu, int nesterov, float wd, int steps) {
+    if (count == 0) return AETH_OK;
+    int row_blocks;
+    const int blocks = muon_whole_blocks(t, count, &row_blocks);
+    if (blocks > 0) return muon_small(t, count, row_blocks, blocks, lr, state, mu, nesterov, wd, steps);
     for (int i = 0; i < count;) {
         int64_t bytes = 0;
         int k = 0;

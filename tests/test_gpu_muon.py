@@ -48,7 +48,10 @@ SHAPES = [(1, 1), (1, 7), (9, 1), (2, 2), (2, 3), (5, 4), (15, 17), (16, 16), (2
           (63, 65), (64, 64), (64, 576), (576, 64), (65, 64), (10, 300), (300, 10), (96, 96), (100, 1000), (127, 129),
           (128, 128), (128, 576), (129, 128), (130, 1030), (160, 161), (191, 193), (192, 192), (255, 257), (256, 256),
           (256, 2048), (2048, 256), (257, 400), (320, 500), (1, 5000), (3, 4097), (4500, 33), (384, 384), (500, 640), (513, 700),
-          (640, 512), (1000, 150), (1024, 512), (1025, 1030), (1300, 1100)]
+          (640, 512), (1000, 150), (1024, 512), (1025, 1030), (1300, 1100),
+          # on both sides of what one workgroup takes, by column blocks a wave
+          (32, 256), (20, 257), (20, 520), (1030, 20), (32, 1536), (1537, 32), (31, 1100), (64, 256), (33, 257), (520, 50), (64, 768),
+          (768, 33), (64, 769), (769, 64), (61, 700)]
 
 
 @pytest.mark.parametrize("r,c", SHAPES)
@@ -149,7 +152,8 @@ CNN3 = [(27, 32), (288, 64), (576, 128), (2048, 256)]
 
 @pytest.mark.parametrize("shapes", [[(1, 1)], [(64, 64)], [(256, 10)], [(10, 256)], [(300, 500)], [(1100, 600)], CNN3,
                                     [(64, 64), (64, 64), (64, 64)], [(5, 9), (700, 700), (1, 3), (130, 64), (64, 130)],
-                                    [(20 + 3 * i, 90 - 2 * i) for i in range(32)]])
+                                    [(20 + 3 * i, 90 - 2 * i) for i in range(32)], [(64, 7), (3, 60), (300, 20), (40, 41)],
+                                    [(33 + i, 30 + 8 * i) for i in range(32)]])
 @pytest.mark.parametrize("nesterov", [0, 1])
 def test_update(shapes, nesterov):
     tensors = [_triple(r, c, seed=10 * i) for i, (r, c) in enumerate(shapes)]
