@@ -2,6 +2,7 @@
 checks of the reference that the GPU tests compare with."""
 import ctypes as C
 import os
+import subprocess
 
 import numpy as np
 import pytest
@@ -124,3 +125,15 @@ def test_the_reference_sets_singular_values_near_one():
     for _ in range(5):
         p = R.COEF[0] * p + R.COEF[1] * p ** 3 + R.COEF[2] * p ** 5
     assert np.allclose(o, (u * p) @ v, atol=1e-12)
+
+
+def test_tiles_runs_and_buffers_cover_every_product(tmp_path):
+    """aether-ml_amd/csrc/muon_plan.h: tile orders, the choice of tiles and runs, the workspace (tests/cpu/muon_plan_check.cpp
+    walks them on the host)."""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    exe = str(tmp_path / "muon_plan_check")
+    subprocess.run(["g++", "-std=c++17", "-O2", "-Wall", "-Werror", "-I", os.path.join(root, "aether-ml_amd", "csrc"),
+                    os.path.join(root, "tests", "cpu", "muon_plan_check.cpp"), "-o", exe], check=True)
+    r = subprocess.run([exe], capture_output=True, text=True)
+    assert r.returncode == 0, r.stdout + r.stderr
+    assert [line.split()[1] for line in r.stdout.splitlines()] == ["triangles", "choices", "layouts"]
