@@ -430,7 +430,7 @@ __global__ __launch_bounds__(64 * kWholeWaves) void muon_whole(const MuonTable t
 }
 
 // One launch for one product of every matrix, in tiles of BM x BN.
-template <int BM, int BN, int WM, int WN, int NBUF, int USE>
+template <int BM, int BN, int WM, int WN, int NBUF, int BLOCK, int USE>
 static int muon_launch(SplitTable tb, float lr, const double* state, float wd) {
     constexpr bool kSym = USE == kSplitGram || USE == kSplitPoly || USE == kSplitPart;
     int64_t tiles = 0;
@@ -443,23 +443,27 @@ static int muon_launch(SplitTable tb, float lr, const double* state, float wd) {
     if constexpr (BM == 32)
         hipLaunchKernelGGL((split_block<USE>), dim3((unsigned)tiles), dim3(256), 0, ctx().stream, tb, lr, state, wd);
     else
-        hipLaunchKernelGGL((split_product<BM, BN, WM, WN, NBUF, USE>), dim3((unsigned)tiles), dim3(64 * (BM / WM) * (BN / WN)), 0,
+        hipLaunchKernelGGL((split_product<BM, BN, WM, WN, NBUF, BLOCK, USE>), dim3((unsigned)tiles), dim3(64 * (BM / WM) * (BN / WN)), 0,
                            ctx().stream, tb, lr, state, wd);
     AETH_LAUNCH_CHECK();
     return AETH_OK;
 }
 
-// (`tile`: kMuonTileTable's order)
 template <int USE>
 static int muon_launch_tile(int tile, const SplitTable& tb, float lr, const double* state, float wd) {
-    constexpr bool kSym = USE == kSplitGram || USE == kSplitPoly;
-    if (tile == 0) return muon_launch<32, 32, 32, 32, 3, USE>(tb, lr, state, wd);
-    if (tile == 1) return muon_launch<64, 64, 32, 32, 4, USE>(tb, lr, state, wd);
-    if (tile == 2) return muon_launch<96, 96, 96, 32, 3, USE>(tb, lr, state, wd);
-    if (USE == kSplitPart || tile == 3) return muon_launch<128, 128, 64, 64, 4, USE>(tb, lr, state, wd);
-    if constexpr (kSym) return muon_launch<192, 192, 96, 96, 3, USE>(tb, lr, state, wd);
-    else if constexpr (USE != kSplitPart) return muon_launch<256, 128, 64, 64, 3, USE>(tb, lr, state, wd);
-    return AETH_OK;
+    if (tile == kTile32) return muon_launch<32, 32, 32, 32, 3, 32, USE>(tb, lr, state, wd);
+    if (tile == kTile64) return muon_launch<64, 64, 32, 32, 4, 32, USE>(tb, lr, state, wd);
+    if constexpr (USE != kSplitPart) {
+        if (tile == kTile96) return muon_launch<96, 96, 48, 48, 3, 16, USE>(tb, lr, state, wd);
+        if (tile == kTile160) return muon_launch<160, 160, 80, 80, 3, 16, USE>(tb, lr, state, wd);
+        if (tile == kTile192) return muon_launch<192, 192, 96, 96, 3, 16, USE>(tb, lr, state, wd);
+        if constexpr (USE == kSplitGram || USE == kSplitPoly) {
+            if (tile == kTile48) return muon_launch<48, 48, 48, 16, 4, 16, USE>(tb, lr, state, wd);
+        } else {
+            if (tile == kTile256x128) return muon_launch<256, 128, 64, 64, 3, 32, USE>(tb, lr, state, wd);
+        }
+    }
+    return muon_launch<128, 128, 64, 64, 4, 32, USE>(tb, lr, state, wd);
 }
 
 template <int USE>

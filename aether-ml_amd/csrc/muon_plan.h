@@ -57,27 +57,40 @@ static inline int64_t muon_tiles(int64_t rows, int64_t cols, int bm, int bn, boo
 // The tile shapes a product can be cut into, with what a tile costs: `start` us a launch, `again` us for every further tile of a
 // CU (its first loads and its epilogue, as far as no other tile hides them), then us a slab of 32 columns on a CU whose neighbours
 // are idle (`alone`) and with a tile on every CU (`full`: the tiles then share the L2 caches' bandwidth and the power that the
-// matrix units may draw).  Measured on square and wide products of 64 to 4096 rows; a CU takes what its tiles
-// cost one after the other, whether they are on it together or not.
+// matrix units may draw).  CUs with one tile more than others hold the launch up by `slack` of that tile (several small tiles are
+// on a CU at once).  Fitted to square and wide products of 64 to 4096 rows, and the tile with the least cost is taken: 3000 x 3000
+// gram 99 us in tiles of 160 x 160 (120 in 96, 121 in 192, 132 in 64), step 140 in 192 x 192 (169 in 96); 1000 x 1537 gram 14.3 in
+// 48 x 48 (15.5 in 64); 4096 x 4096 gram 190 in 192 x 192 (240 in 160), step 350 in 256 x 128 (373 in 192 x 192).
 struct MuonTile {
     int bm, bn;
-    bool symmetric, general;     // offered for symmetric results, for others
-    float start, again, alone, full;
+    bool symmetric, general, runs;     // offered for symmetric results, for others, for gram products in runs
+    float start, again, slack, alone, full;
 };
-constexpr int kMuonTiles = 6;
+enum { kTile32, kTile48, kTile64, kTile96, kTile128, kTile160, kTile192, kTile256x128, kMuonTiles };
 static const MuonTile kMuonTileTable[kMuonTiles] = {
-    {32, 32, true, true, 3.0f, 2.5f, 0.10f, 0.12f},
-    {64, 64, true, true, 3.5f, 0.5f, 0.24f, 0.25f},
-    {96, 96, true, true, 5.0f, 1.0f, 0.41f, 0.50f},
-    {128, 128, true, true, 5.0f, 1.0f, 0.53f, 0.80f},
-    {192, 192, true, false, 8.0f, 2.0f, 1.05f, 1.45f},
-    {256, 128, false, true, 7.0f, 2.0f, 0.95f, 1.17f},
+    {32, 32, true, true, true, 3.3f, 2.0f, 0.2f, 0.11f, 0.12f},
+    {48, 48, true, false, false, 5.0f, 0.5f, 0.6f, 0.17f, 0.20f},
+    {64, 64, true, true, true, 4.5f, 0.5f, 0.5f, 0.21f, 0.25f},
+    {96, 96, true, true, false, 8.0f, 1.0f, 0.6f, 0.33f, 0.48f},
+    {128, 128, true, true, true, 6.0f, 1.0f, 1.0f, 0.53f, 0.78f},
+    {160, 160, true, true, false, 14.0f, 2.0f, 1.0f, 0.75f, 0.96f},
+    {192, 192, true, true, false, 17.0f, 2.0f, 1.0f, 1.00f, 1.34f},
+    {256, 128, false, true, false, 8.0f, 2.0f, 1.0f, 0.95f, 1.30f},
 };
 constexpr int kMuonCus = 256;
 
 struct MuonShape {
     int64_t rows, cols, k;       // padded
 };
+
+// Tiles that the busiest CU is held up by.
+static inline float muon_turns(const MuonTile& t, int64_t tiles) {
+    const float even = (float)tiles / kMuonCus, most = (float)((tiles + kMuonCus - 1) / kMuonCus);
+    return even <= 1.f ? 1.f : even + (most - even) * t.slack;
+}
+static inline float muon_slab(const MuonTile& t, int64_t tiles) {
+    return t.alone + (t.full - t.alone) * (tiles < kMuonCus ? (float)tiles / kMuonCus : 1.f);
+}
 
 // What a launch of these products costs with one tile shape, in us.
 static inline float muon_cost(const MuonTile& t, const MuonShape* p, int count, bool symmetric) {
@@ -87,12 +100,11 @@ static inline float muon_cost(const MuonTile& t, const MuonShape* p, int count, 
         const int64_t n = muon_tiles(p[i].rows, p[i].cols, t.bm, t.bn, symmetric);
         tiles += n;
         slabs += n * (p[i].k / 32);
-        const float mine = (float)((n + kMuonCus - 1) / kMuonCus) * (float)(p[i].k / 32);
+        const float mine = muon_turns(t, n) * (float)(p[i].k / 32);
         if (mine > longest) longest = mine;
     }
-    const float even = (float)slabs / kMuonCus, share = tiles < kMuonCus ? (float)tiles / kMuonCus : 1.f;
-    const float more = (float)((tiles + kMuonCus - 1) / kMuonCus - 1);
-    return t.start + t.again * more + (longest > even ? longest : even) * (t.alone + (t.full - t.alone) * share);
+    const float even = (float)slabs / kMuonCus;
+    return t.start + t.again * (muon_turns(t, tiles) - 1.f) + (longest > even ? longest : even) * muon_slab(t, tiles);
 }
 
 static inline int muon_choose(const MuonShape* p, int count, bool symmetric) {
@@ -122,10 +134,12 @@ constexpr float kMuonJoin = 3.2f, kMuonJoinRuns = 1.0f, kMuonJoinRate = 3.0e6f;
 // False where one launch without runs is the faster way.
 static inline bool muon_choose_runs(const MuonShape* p, int count, MuonRuns* out) {
     bool found = false;
+    *out = MuonRuns{};
     float least = muon_cost(kMuonTileTable[muon_choose(p, count, true)], p, count, true);
-    for (int k = 0; k < 4; ++k) {
+    for (int k = 0; k < kMuonTiles; ++k) {
         const MuonTile& t = kMuonTileTable[k];
-        MuonRuns r;
+        if (!t.runs) continue;
+        MuonRuns r = {};
         r.tile = k;
         int64_t units = 0, longest = 0;
         for (int i = 0; i < count; ++i) {
@@ -142,9 +156,8 @@ static inline bool muon_choose_runs(const MuonShape* p, int count, MuonRuns* out
                 tiles += r.runs[i] * muon_tiles(p[i].rows, p[i].cols, t.bm, t.bn, true);
                 r.bytes += r.runs[i] * (side * (side + 1) / 2) * 4096;
             }
-            const float share = tiles < kMuonCus ? (float)tiles / kMuonCus : 1.f;
-            const float turns = (float)((tiles + kMuonCus - 1) / kMuonCus);
-            const float c = t.start + t.again * (turns - 1.f) + turns * (float)r.run * (t.alone + (t.full - t.alone) * share) + kMuonJoin +
+            const float turns = muon_turns(t, tiles);
+            const float c = t.start + t.again * (turns - 1.f) + turns * (float)r.run * muon_slab(t, tiles) + kMuonJoin +
                             kMuonJoinRuns * (float)((most + 31) / 32) + (float)r.bytes / kMuonJoinRate;
             if (c < least) {
                 least = c;

@@ -204,15 +204,86 @@ __device__ __forceinline__ void split_finish(const SplitProduct& pr, const f16v&
     }
 }
 
+// The same for a 16 x 16 block: acc[e] is row r + 4 (lane / 16) + e, column c + lane % 16.
+template <int USE>
+__device__ __forceinline__ void split_finish(const SplitProduct& pr, const f4& acc, int r, int c, const SplitTile& at,
+                                             unsigned (*blk)[33], float keep, float step) {
+    static_assert(USE != kSplitPart, "partial sums come in blocks of 32 x 32");
+    constexpr bool kSym = USE != kSplitStep;
+    const int lane = threadIdx.x & 63, l16 = lane & 15, lq = lane >> 4;
+    constexpr float kOut = split_scale<USE>();
+    if constexpr (USE == kSplitApply) {
+        const int x = c + l16, cc = min(x, pr.cols - 1), y0 = r + 4 * lq;
+        float t[4];
+        if (pr.theta != nullptr) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) t[e] = pr.theta[(size_t)min(y0 + e, pr.rows - 1) * pr.cols + cc];
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (y0 + e < pr.rows && x < pr.cols) {
+                const float o = acc[e] * kOut;
+                if (pr.theta != nullptr) pr.theta[(size_t)(y0 + e) * pr.cols + x] = keep * t[e] - step * o;
+                else pr.out[(size_t)(y0 + e) * pr.cols + x] = o;
+            }
+    } else {
+        const size_t turned = ((size_t)(r / 32) * pr.N + c + l16) * 128 + 2 * (r & 31) + 8 * lq;
+        float o[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] = acc[e] * kOut;
+        if (USE == kSplitPoly) {
+            const half4 h = *reinterpret_cast<const half4*>(pr.A + turned), l = *reinterpret_cast<const half4*>(pr.A + turned + 64);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                o[e] += ((float)h[e] + (float)l[e]) * (kNsB * kScaleB / kScaleA);
+                if (r == c && 4 * lq + e == l16) o[e] += kNsA * kScaleB;
+            }
+        }
+        unsigned w[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[e] = split_pack(o[e]);
+        if (!(kSym && r == c)) split_store<4>((kSym ? pr.D1 : pr.D2) + turned, w);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) blk[4 * lq + e][l16] = w[e];
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[e] = blk[l16][4 * lq + e];
+        split_store<4>(pr.D1 + ((size_t)(c / 32) * pr.M + r + l16) * 128 + 2 * (c & 31) + 8 * lq, w);
+        __builtin_amdgcn_wave_barrier();
+    }
+}
+
+__device__ __forceinline__ f16v split_mfma(const half8& a, const half8& b, const f16v& c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f4 split_mfma(const half8& a, const half8& b, const f4& c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+template <int BLOCK>
+struct SplitAcc;
+template <>
+struct SplitAcc<32> {
+    typedef f16v type;
+};
+template <>
+struct SplitAcc<16> {
+    typedef f4 type;
+};
+
 // A matrix lies slab by slab: slab s holds columns 32 s .. 32 s + 31 of all R rows, row r's 128 bytes (64 of high halves, 64 of low)
 // at (s R + r) * 128, so that what a tile reads at a time is one contiguous piece and no offset grows with the matrix.
 // One workgroup: BM x BN of the result, waves of WM x WN, slabs through a ring of NBUF LDS buffers, loaded straight into LDS
 // NBUF - 1 slabs ahead.  16-byte chunk c of row r lies at c ^ ((r >> 1) & 7): the 16 rows that a fragment read takes at a time
 // then lie in different banks.
-template <int BM, int BN, int WM, int WN, int NBUF, int USE>
+// BLOCK: the MFMA's result, 32 x 32 (16 columns a step) or 16 x 16 (32 columns, a whole slab).  The small one is for waves of 16, 48
+// or 80 rows or columns, and for 96 x 96: there it keeps one step's operands fewer (2048 x 2048 in 96 x 96 tiles: 42 us with four
+// waves of 48 x 48, 44 with three of 96 x 32; 4096 x 4096 in 192 x 192: 190 us, with 32 x 32 blocks 198).
+// Bound: with a tile on every CU, the power the matrix units draw (4096 x 4096: 1.1 PFLOP/s of float16, what a library's float16
+// product of that size reaches); below that what a CU can have in flight from the L2 caches, 85 GB/s.
+template <int BM, int BN, int WM, int WN, int NBUF, int BLOCK, int USE>
 __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN)) void split_product(const SplitTable tb, float lr,
                                                                            const double* __restrict__ state, float wd) {
-    constexpr int WAVES = (BM / WM) * (BN / WN), TM = WM / 32, TN = WN / 32;
+    constexpr int WAVES = (BM / WM) * (BN / WN), TM = WM / BLOCK, TN = WN / BLOCK, STEPS = BLOCK / 16;
     constexpr int AL = BM / 8 / WAVES, BL = BN / 8 / WAVES;
     static_assert(AL * 8 * WAVES == BM && BL * 8 * WAVES == BN, "whole loads a wave");
     constexpr int BUF = (BM + BN) * 128;
@@ -225,7 +296,6 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN)) void split_product(cons
     const SplitTile at = split_tile<USE>(pr, tile - pr.first);
     const int slabs = at.slabs;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-    const int l32 = lane & 31, lh = lane >> 5;
     const int r0 = at.i * BM, c0 = at.j * BN;
     // the next slab's rows
     const char *sp = pr.P + ((size_t)at.begin * pr.M + r0) * 128, *sq = pr.Q + ((size_t)at.begin * pr.N + c0) * 128;
@@ -254,48 +324,49 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN)) void split_product(cons
         sq += dq;
     };
 
-    f16v acc[TM][TN];
+    typename SplitAcc<BLOCK>::type acc[TM][TN];
 #pragma unroll
     for (int i = 0; i < TM; ++i)
 #pragma unroll
         for (int j = 0; j < TN; ++j)
 #pragma unroll
-            for (int v = 0; v < 16; ++v) acc[i][j][v] = 0.f;
+            for (int v = 0; v < BLOCK * BLOCK / 64; ++v) acc[i][j][v] = 0.f;
 
     const int wm = (wave / (BN / WN)) * WM, wn = (wave % (BN / WN)) * WN;
-    const unsigned sw = (unsigned)(lh ^ ((l32 >> 1) & 7)) * 16u;
-    const unsigned fa = (unsigned)(wm + l32) * 128u + sw, fb = (unsigned)(BM + wn + l32) * 128u + sw;
-    // One slab: two steps of 16 columns, three products each.  The next slab's loads go out one by one between the MFMAs: a wave
-    // that issues them all at once waits for the load unit's queue with its MFMAs behind it (4096 x 4096, tiles of 256 x 128: 307 us
-    // a product, tiles of 192 x 192 for the symmetric ones 194 us; all at once 215 us for these).
+    // a lane's operand row and its chunk of the row's columns, in the first block
+    const unsigned row = (unsigned)lane & (BLOCK - 1), sw = (((unsigned)lane / BLOCK) ^ ((row >> 1) & 7u)) * 16u;
+    const unsigned fa = (wm + row) * 128u + sw, fb = (BM + wn + row) * 128u + sw;
+    // One slab: two steps of 16 columns (one of 32), three products each.  The next slab's loads go out one by one between the
+    // MFMAs: a wave that issues them all at once waits for the load unit's queue with its MFMAs behind it (4096 x 4096, tiles of
+    // 192 x 192: 195 us a product, all at once 215).
     const auto multiply = [&](int buf, int into, auto loads) {
         const char* b = lds + buf * BUF;
-        half8 f[2][2 * TM + 2 * TN];                     // high and low halves of both operands' rows, for either step
+        half8 f[STEPS][2 * TM + 2 * TN];                 // high and low halves of both operands' rows, for every step
         const auto read = [&](int t) {
 #pragma unroll
             for (int i = 0; i < TM; ++i) {
-                f[t][i] = *reinterpret_cast<const half8*>(b + ((fa ^ (t * 32u)) + i * 4096u));
-                f[t][TM + i] = *reinterpret_cast<const half8*>(b + ((fa ^ (t * 32u + 64u)) + i * 4096u));
+                f[t][i] = *reinterpret_cast<const half8*>(b + ((fa ^ (t * 32u)) + i * (BLOCK * 128u)));
+                f[t][TM + i] = *reinterpret_cast<const half8*>(b + ((fa ^ (t * 32u + 64u)) + i * (BLOCK * 128u)));
             }
 #pragma unroll
             for (int j = 0; j < TN; ++j) {
-                f[t][2 * TM + j] = *reinterpret_cast<const half8*>(b + ((fb ^ (t * 32u)) + j * 4096u));
-                f[t][2 * TM + TN + j] = *reinterpret_cast<const half8*>(b + ((fb ^ (t * 32u + 64u)) + j * 4096u));
+                f[t][2 * TM + j] = *reinterpret_cast<const half8*>(b + ((fb ^ (t * 32u)) + j * (BLOCK * 128u)));
+                f[t][2 * TM + TN + j] = *reinterpret_cast<const half8*>(b + ((fb ^ (t * 32u + 64u)) + j * (BLOCK * 128u)));
             }
         };
         read(0);
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
+        for (int t = 0; t < STEPS; ++t) {
 #pragma unroll
             for (int g = 0; g < 3; ++g) {                // high.low, low.high, high.high
-                if (t == 0 && g == 1) read(1);
+                if (STEPS == 2 && t == 0 && g == 1) read(1);
 #pragma unroll
                 for (int i = 0; i < TM; ++i) {
                     const half8 x = f[t][(g == 1 ? TM : 0) + i];
 #pragma unroll
                     for (int j = 0; j < TN; ++j)
-                        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, f[t][2 * TM + (g == 0 ? TN : 0) + j], acc[i][j], 0, 0, 0);
-                    constexpr int GROUPS = 6 * TM;
+                        acc[i][j] = split_mfma(x, f[t][2 * TM + (g == 0 ? TN : 0) + j], acc[i][j]);
+                    constexpr int GROUPS = 3 * STEPS * TM;
                     const int u = (t * 3 + g) * TM + i;
                     if (decltype(loads)::value) {
 #pragma unroll
@@ -346,7 +417,7 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN)) void split_product(cons
     for (int i = 0; i < TM; ++i)
 #pragma unroll
         for (int j = 0; j < TN; ++j) {
-            const int r = r0 + wm + 32 * i, c = c0 + wn + 32 * j;
+            const int r = r0 + wm + BLOCK * i, c = c0 + wn + BLOCK * j;
             if (r >= pr.M || c >= pr.N) continue;        // (whole blocks: both are multiples of 32)
             if (kSym && r > c) continue;                 // (below the diagonal of a diagonal tile: written from above it)
             split_finish<USE>(pr, acc[i][j], r, c, at, blk, keep, step);

@@ -57,7 +57,7 @@ static int choices() {
         MuonRuns r;
         if (muon_choose_runs(g, count, &r)) {
             // the tiles that kSplitPart is built for; runs that cover all slabs, none empty
-            CHECK(r.tile >= 0 && r.tile < 4 && r.run >= 1);
+            CHECK(r.tile >= 0 && r.tile < kMuonTiles && kMuonTileTable[r.tile].runs && r.run >= 1);
             int64_t bytes = 0;
             for (int i = 0; i < count; ++i) {
                 const int64_t slabs = g[i].k / 32, side = g[i].rows / 32;
