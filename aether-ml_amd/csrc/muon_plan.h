@@ -68,11 +68,11 @@ struct MuonTile {
 };
 enum { kTile32, kTile48, kTile64, kTile96, kTile128, kTile160, kTile192, kTile256x128, kMuonTiles };
 static const MuonTile kMuonTileTable[kMuonTiles] = {
-    {32, 32, true, true, true, 3.3f, 2.0f, 0.2f, 0.11f, 0.12f},
+    {32, 32, true, true, true, 3.3f, 4.0f, 0.2f, 0.11f, 0.12f},
     {48, 48, true, false, false, 5.0f, 0.5f, 0.6f, 0.17f, 0.20f},
     {64, 64, true, true, true, 4.5f, 0.5f, 0.5f, 0.21f, 0.25f},
     {96, 96, true, true, false, 8.0f, 1.0f, 0.6f, 0.33f, 0.48f},
-    {128, 128, true, true, true, 6.0f, 1.0f, 1.0f, 0.53f, 0.78f},
+    {128, 128, true, true, true, 6.0f, 1.0f, 1.0f, 0.50f, 0.74f},
     {160, 160, true, true, false, 14.0f, 2.0f, 1.0f, 0.75f, 0.96f},
     {192, 192, true, true, false, 17.0f, 2.0f, 1.0f, 1.00f, 1.34f},
     {256, 128, false, true, false, 8.0f, 2.0f, 1.0f, 0.95f, 1.30f},
@@ -129,7 +129,7 @@ struct MuonRuns {
     int64_t bytes;               // of partial sums, all products
 };
 // The second launch: us at least, us for every 32 runs (8 waves add four at a time), bytes a us of partial sums written and read.
-constexpr float kMuonJoin = 3.2f, kMuonJoinRuns = 1.0f, kMuonJoinRate = 3.0e6f;
+constexpr float kMuonJoin = 2.6f, kMuonJoinRuns = 1.0f, kMuonJoinRate = 3.5e6f;
 
 // False where one launch without runs is the faster way.
 static inline bool muon_choose_runs(const MuonShape* p, int count, MuonRuns* out) {
