@@ -449,21 +449,24 @@ __global__ __launch_bounds__(kLnLong) void ln_bwd_rows(const LnBwdArgs p) {
 __global__ __launch_bounds__(256) void ln_bwd_columns(const LnBwdArgs p, int run) {
     __shared__ float red[2][4][64];
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, C = p.C;
-    const int64_t c = (int64_t)blockIdx.x * 64 + lane;
     const int beg = blockIdx.y * run, end = min(p.rows, beg + run);
-    float a = 0.f, b = 0.f;
-    if (c < C)
-        for (int r = beg + w; r < end; r += 4) {
-            const float g = p.dy[(size_t)r * C + c];
-            a += g * ((p.x[(size_t)r * C + c] - p.mean[r]) * p.invstd[r]);
-            b += g;
-        }
-    red[0][w][lane] = a;
-    red[1][w][lane] = b;
-    __syncthreads();
-    if (w < 2 && c < C)
-        p.part[((size_t)blockIdx.y * 2 + w) * C + c] =
-            (red[w][0][lane] + red[w][1][lane]) + (red[w][2][lane] + red[w][3][lane]);
+    for (int64_t at = (int64_t)blockIdx.x * 64; at < C; at += (int64_t)gridDim.x * 64) {
+        const int64_t c = at + lane;
+        float a = 0.f, b = 0.f;
+        if (c < C)
+            for (int r = beg + w; r < end; r += 4) {
+                const float g = p.dy[(size_t)r * C + c];
+                a += g * ((p.x[(size_t)r * C + c] - p.mean[r]) * p.invstd[r]);
+                b += g;
+            }
+        __syncthreads();                                 // (the last group's sums have been read)
+        red[0][w][lane] = a;
+        red[1][w][lane] = b;
+        __syncthreads();
+        if (w < 2 && c < C)
+            p.part[((size_t)blockIdx.y * 2 + w) * C + c] =
+                (red[w][0][lane] + red[w][1][lane]) + (red[w][2][lane] + red[w][3][lane]);
+    }
 }
 
 // dgamma | dbeta = the partial rows part[block][2C] added up: 32 columns (128 bytes of a row) a workgroup, 128 lanes of blocks
@@ -472,45 +475,67 @@ __global__ __launch_bounds__(1024) void ln_bwd_finish(const float* __restrict__ 
                                                       float* __restrict__ dgamma, float* __restrict__ dbeta) {
     __shared__ float red[128][33];
     const int unit = threadIdx.x & 7, w = threadIdx.x >> 3;
-    const int64_t c = ((int64_t)blockIdx.x * 8 + unit) * 4, C2 = 2 * (int64_t)C;
-    float a[4] = {0.f, 0.f, 0.f, 0.f};
-    if (c + 4 <= C2) {
-        for (int i0 = w; i0 < blocks; i0 += 512) {
-            ln_f4 v[4];
+    const int64_t C2 = 2 * (int64_t)C;
+    for (int64_t at = (int64_t)blockIdx.x * 32; at < C2; at += (int64_t)gridDim.x * 32) {
+        const int64_t c = at + unit * 4;
+        float a[4] = {0.f, 0.f, 0.f, 0.f};
+        if (c + 4 <= C2) {
+            for (int i0 = w; i0 < blocks; i0 += 512) {
+                ln_f4 v[4];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const int i = i0 + 128 * k;
-                v[k] = i < blocks ? *reinterpret_cast<const ln_f4*>(part + i * C2 + c) : ln_f4{0.f, 0.f, 0.f, 0.f};
+                for (int k = 0; k < 4; ++k) {
+                    const int i = i0 + 128 * k;
+                    v[k] = i < blocks ? *reinterpret_cast<const ln_f4*>(part + i * C2 + c) : ln_f4{0.f, 0.f, 0.f, 0.f};
+                }
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) a[e] += v[k][e];
             }
+        } else {                                         // (the last two columns of an odd C)
+            for (int i = w; i < blocks; i += 128)
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) a[e] += v[k][e];
+                for (int e = 0; e < 4; ++e) a[e] += c + e < C2 ? part[i * C2 + c + e] : 0.f;
         }
-    } else {                                             // (the last two columns of an odd C)
-        for (int i = w; i < blocks; i += 128)
+        __syncthreads();                                 // (the last group's sums have been read)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) a[e] += c + e < C2 ? part[i * C2 + c + e] : 0.f;
-    }
+        for (int e = 0; e < 4; ++e) red[w][unit * 4 + e] = a[e];
+        __syncthreads();
+        const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) red[w][unit * 4 + e] = a[e];
-    __syncthreads();
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        const int col = wave * 2 + h;
-        const int64_t k = (int64_t)blockIdx.x * 32 + col;
-        const float v = ln_group_sum<64>(red[lane][col] + red[lane + 64][col]);
-        if (lane == 0 && k < C2) {
-            if (k < C) dgamma[k] = v;
-            else dbeta[k - C] = v;
+        for (int h = 0; h < 2; ++h) {
+            const int col = wave * 2 + h;
+            const int64_t k = at + col;
+            const float v = ln_group_sum<64>(red[lane][col] + red[lane + 64][col]);
+            if (lane == 0 && k < C2) {
+                if (k < C) dgamma[k] = v;
+                else dbeta[k - C] = v;
+            }
         }
     }
 }
 
-static bool ln_apart(const void* a, const void* b, int64_t na, int64_t nb) {
-    const char *p = (const char*)a, *q = (const char*)b;
-    return p == nullptr || q == nullptr || p + na <= q || q + nb <= p;
+// A launch's threads along one axis stay below 2^32.
+constexpr int kLnMostGroups = 1 << 20;
+
+// Tensors of a call; no output may overlap another output or an input.
+struct LnSpan {
+    const void* p;
+    int64_t bytes;
+};
+template <int W, int R>
+static bool ln_apart(const LnSpan (&written)[W], const LnSpan (&read)[R]) {
+    const auto apart = [](const LnSpan& a, const LnSpan& b) {
+        const char *p = (const char*)a.p, *q = (const char*)b.p;
+        return p == nullptr || q == nullptr || a.bytes == 0 || b.bytes == 0 || p + a.bytes <= q || q + b.bytes <= p;
+    };
+    for (int i = 0; i < W; ++i) {
+        for (int j = 0; j < i; ++j)
+            if (!apart(written[i], written[j])) return false;
+        for (int j = 0; j < R; ++j)
+            if (!apart(written[i], read[j])) return false;
+    }
+    return true;
 }
 
 // How a row is laid over lanes: the way with the fewest idle places, and of those the one with the most lanes (802816 x 64 backward:
@@ -615,7 +640,10 @@ static int ln_fwd_impl(const float* x, const float* gamma, const float* beta, fl
     AETH_CHECK_ARG((save_mean == nullptr) == (save_invstd == nullptr));
     AETH_CHECK_ARG(rows == 0 || (x && gamma && beta && y));
     const int64_t n = (int64_t)rows * C;
-    AETH_CHECK_ARG(ln_apart(x, y, 4 * n, 4 * n) && ln_apart(x, y16, 4 * n, 2 * n) && ln_apart(y, y16, 4 * n, 2 * n));
+    const int64_t r4 = 4 * (int64_t)rows, c4 = rows ? 4 * (int64_t)C : 0;
+    const LnSpan written[] = {{y, 4 * n}, {y16, 2 * n}, {save_mean, r4}, {save_invstd, r4}};
+    const LnSpan read[] = {{x, 4 * n}, {gamma, c4}, {beta, c4}};
+    AETH_CHECK_ARG(ln_apart(written, read));
     AETH_REQUIRE_INIT();
     if (rows == 0) return AETH_OK;
     const LnShape s = ln_fwd_shape(C);
@@ -634,8 +662,10 @@ static int ln_bwd_impl(const float* x, const float* dy, const float* gamma, cons
     AETH_CHECK_ARG(rows >= 0 && C > 0 && (int64_t)rows * C < ((int64_t)1 << 31));
     AETH_CHECK_ARG(dgamma && dbeta && (rows == 0 || (x && dy && gamma && mean && invstd && dx)));
     const int64_t n = (int64_t)rows * C;
-    AETH_CHECK_ARG(ln_apart(x, dx, 4 * n, 4 * n) && ln_apart(dy, dx, 4 * n, 4 * n));
-    AETH_CHECK_ARG(ln_apart(x, dx16, 4 * n, 2 * n) && ln_apart(dy, dx16, 4 * n, 2 * n) && ln_apart(dx, dx16, 4 * n, 2 * n));
+    const int64_t r4 = 4 * (int64_t)rows, c4 = 4 * (int64_t)C;
+    const LnSpan written[] = {{dx, 4 * n}, {dx16, 2 * n}, {dgamma, c4}, {dbeta, c4}};
+    const LnSpan read[] = {{x, 4 * n}, {dy, 4 * n}, {gamma, rows ? c4 : 0}, {mean, r4}, {invstd, r4}};
+    AETH_CHECK_ARG(ln_apart(written, read));
     AETH_REQUIRE_INIT();
     hipStream_t st = ctx().stream;
     int blocks = 0;
@@ -661,11 +691,14 @@ static int ln_bwd_impl(const float* x, const float* dy, const float* gamma, cons
         hipLaunchKernelGGL(ln_bwd_kernel(s), dim3(s.lanes < 0 ? (rows < 4096 ? rows : 4096) : blocks), dim3(threads), 0, st, p);
         AETH_LAUNCH_CHECK();
         if (s.lanes < 0) {
-            hipLaunchKernelGGL(ln_bwd_columns, dim3(cdiv(C, 64), blocks), dim3(256), 0, st, p, run);
+            const int groups = cdiv(C, 64);
+            hipLaunchKernelGGL(ln_bwd_columns, dim3(groups < kLnMostGroups ? groups : kLnMostGroups, blocks), dim3(256), 0, st, p, run);
             AETH_LAUNCH_CHECK();
         }
     }
-    hipLaunchKernelGGL(ln_bwd_finish, dim3(cdiv(2 * (int64_t)C, 32)), dim3(1024), 0, st, (const float*)ws, blocks, C, dgamma, dbeta);
+    const int groups = cdiv(2 * (int64_t)C, 32);
+    hipLaunchKernelGGL(ln_bwd_finish, dim3(groups < kLnMostGroups ? groups : kLnMostGroups), dim3(1024), 0, st, (const float*)ws, blocks,
+                       C, dgamma, dbeta);
     AETH_LAUNCH_CHECK();
     return AETH_OK;
 }

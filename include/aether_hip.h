@@ -203,8 +203,8 @@ int aeth_bn_bwd_f32(const float* x, const float* dy, const float* gamma,
  * ln_bwd : with xhat = (x - mean) invstd and g = dy gamma: dx = invstd (g - sum_c g / C - xhat sum_c g xhat / C),
  *          dgamma = sum_rows dy xhat, dbeta = sum_rows dy, each element written.  Deterministic.
  * rows may be 0 (dgamma = dbeta = 0).  A NaN or an infinity stays in its row (and, backward, in its columns' dgamma /
- * dbeta).  Outputs may not overlap inputs.  The _twin_ forms also leave a bfloat16 copy of y / dx, as the other producers do
- * (aeth_relu_fwd_twin_f32 below). */
+ * dbeta).  No output may overlap another tensor of the call.  The _twin_ forms also leave a bfloat16 copy of y / dx, as the
+ * other producers do (aeth_relu_fwd_twin_f32 below). */
 int aeth_ln_fwd_f32(const float* x, const float* gamma, const float* beta,
                     float* save_mean /* may be NULL */, float* save_invstd /* NULL with save_mean */, float* y,
                     int rows, int C, float eps);

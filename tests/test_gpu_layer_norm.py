@@ -157,6 +157,19 @@ def test_bad_values_stay_in_their_row(c):
     assert np.all(np.isnan(dg)) and np.array_equal(db, want[2])
 
 
+def test_a_row_of_more_columns_than_a_launch_has_threads_for():
+    c = (1 << 26) + 77
+    x, dy = (np.resize(a, (1, c)) for a in _inputs(1, 1 << 18)[::3])
+    gamma, beta = (np.resize(a, c) for a in _inputs(1, 100003)[1:3])
+    (y, mean, inv), (e_y, e_mean, e_inv) = R.forward(x, gamma, beta, 1e-5)
+    got = _forward(x, gamma, beta)
+    assert R.worst(got[0], y, e_y) <= 1 and R.worst(got[1], mean, e_mean) <= 1 and R.worst(got[2], inv, e_inv) <= 1
+    want, bounds = R.backward(x, dy, gamma, got[1], got[2])
+    back = _backward(x, dy, gamma, got[1], got[2])
+    for g, w, b, name in zip(back, want, bounds, ("dx", "dgamma", "dbeta")):
+        assert R.worst(g, w, b) <= 1, name
+
+
 def test_no_rows():
     x, gamma, beta, _ = _inputs(1, 12)
     empty = np.zeros((0, 12), np.float32)

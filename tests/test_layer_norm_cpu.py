@@ -56,6 +56,12 @@ def test_refusals(lib, name):
         refused(**{"_%d" % at[Y16]: Y + 64})
     if DY in at:
         refused(**{"_%d" % at[Y]: DY})
+    outputs = [i for i, a in enumerate(good) if a in ((Y, Y16, M, S) if 1e-5 in at else (Y, Y16, DG, DB))]
+    for i in outputs:                        # no output over any other tensor, whole or at one element
+        for j in pointers:
+            if i != j:
+                refused(**{"_%d" % i: good[j]})
+                refused(**{"_%d" % i: good[j] + 2})
     if 1e-5 in at:
         refused(**{"_%d" % at[1e-5]: -1e-3})
         refused(**{"_%d" % at[1e-5]: float("nan")})
