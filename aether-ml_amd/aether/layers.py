@@ -978,6 +978,14 @@ class Optimizer_Adam:
             self._state_iterations = self.iterations
         return self._state
 
+    def recorded_settings(self, layers):
+        """What a recorded update holds besides its tensors: with other values it has to be recorded anew."""
+        return self._base_rate(), self.decay, self.epsilon
+
+    def _base_rate(self):
+        """What a step without decay would take (pre_update_parameters leaves the current rate alone then)."""
+        return float(self.learning_rate if self.decay else self.current_learning_rate)
+
     def record_update(self, layers):
         """Queue one whole optimizer step (pre_update, every layer, post_update) in a form
         that can be replayed: learning rate and bias corrections come from device_state()."""
@@ -992,7 +1000,7 @@ class Optimizer_Adam:
         state = self._state
         self._recorded_params = [t[0] for t in batch]
         b1, b2 = float(np.float32(self.beta_1)), float(np.float32(self.beta_2))
-        _ck(_L().aeth_adam_state_step(state.ptr, float(self.learning_rate), float(self.decay), b1, b2))
+        _ck(_L().aeth_adam_state_step(state.ptr, self._base_rate(), float(self.decay), b1, b2))
         while batch:
             part, batch = batch[:32], batch[32:]
             n = len(part)
@@ -1114,6 +1122,12 @@ class Optimizer_Muon:
             self._state_iterations = self.iterations
         return self._state
 
+    def recorded_settings(self, layers):
+        return (self._base_rate(), self.decay, self.momentum, bool(self.nesterov), self.weight_decay, self.ns_steps,
+                self.adam.recorded_settings(layers), tuple(self.takes(layer) for layer in layers))
+
+    _base_rate = Optimizer_Adam._base_rate
+
     def record_update(self, layers):
         """Queue one whole optimizer step in a form that can be replayed (see Optimizer_Adam.record_update)."""
         matrices, others = [], []
@@ -1124,7 +1138,7 @@ class Optimizer_Muon:
                 others.append((layer.weights, layer.dweights, layer.weight_momentums, layer.weight_cache))
             others.append((layer.biases, layer.dbiases, layer.bias_momentums, layer.bias_cache))
         self._recorded_params = [t[0] for t in matrices]
-        _ck(_L().aeth_adam_state_step(self._state.ptr, float(self.learning_rate), float(self.decay), 1.0, 1.0))
+        _ck(_L().aeth_adam_state_step(self._state.ptr, self._base_rate(), float(self.decay), 1.0, 1.0))
         while matrices:
             part, matrices = matrices[:32], matrices[32:]
             _ck(_L().aeth_muon_multi_dev_f32(*self._matrices(part), self.momentum, int(bool(self.nesterov)),

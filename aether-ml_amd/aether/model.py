@@ -243,9 +243,12 @@ class Model:
             recs[key] = {"graph": None}
             return None
         # a recording holds the optimizer's update and reads and writes the parameter buffers it was made with:
-        # another optimizer, or parameters set anew since then (set_parameters, load_parameters), make it stale
+        # another optimizer or other settings of it, or parameters set anew since then (set_parameters, load_parameters),
+        # make it stale
         params = [(id(l), l.weights.ptr, l.biases.ptr) for l in self.trainable_layers]
-        if rec["graph"] is not None and (rec.get("params") != params or rec.get("optimizer") is not self.optimizer):
+        settings = self.optimizer.recorded_settings(self.trainable_layers)
+        if rec["graph"] is not None and (rec.get("params") != params or rec.get("optimizer") is not self.optimizer
+                                         or rec.get("settings") != settings):
             _lib.check(lib.aeth_graph_destroy(rec["graph"]))
             recs[key] = rec = {"graph": None}
         if rec["graph"] is None:
@@ -273,6 +276,7 @@ class Model:
             rec["graph"] = handle
             rec["params"] = params
             rec["optimizer"] = self.optimizer
+            rec["settings"] = settings
             # what the layers point at after this step (output, dinputs, dweights, ...):
             # replays fill the same buffers, so the attributes are put back after steps
             # that ran in between (an evaluation, a step of another shape)

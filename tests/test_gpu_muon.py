@@ -345,6 +345,29 @@ def test_another_optimizer_makes_a_recording_stale():
     assert all(np.array_equal(a, b) for a, b in zip(*runs))
 
 
+@pytest.mark.parametrize("change", ["momentum", "nesterov", "ns_steps", "weight_decay", "current_learning_rate", "adam", "muon"])
+def test_other_settings_make_a_recording_stale(change):
+    import aether
+    steps = _batches(6)
+    runs = []
+    for record in (False, True):
+        model = _network(aether.Optimizer_Muon(), norm=False)
+        model.record_steps(record)
+        for k, (x, y) in enumerate(steps):
+            if k == 4:
+                if change == "adam":
+                    model.optimizer.adam.current_learning_rate = 3e-3
+                elif change == "muon":
+                    model.trainable_layers[0].muon = False
+                else:
+                    value = dict(momentum=.5, nesterov=False, ns_steps=3, weight_decay=.1, current_learning_rate=.1)[change]
+                    setattr(model.optimizer, change, value)
+            model.train_step(x, y)
+        runs.append(_host(model))
+        model.record_steps(False)
+    assert all(np.array_equal(a, b) for a, b in zip(*runs))
+
+
 def test_which_layers_are_matrices():
     import aether
     model = _network(aether.Optimizer_Muon())
