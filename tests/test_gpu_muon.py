@@ -62,6 +62,13 @@ def test_orthogonalisation(r, c):
     assert np.array_equal(_ortho(g), o)                    # the same bits again
 
 
+# every tile of the larger products, ragged: their choice goes by the sizes
+@pytest.mark.parametrize("r,c", [(810, 750), (1000, 4100), (1500, 1600), (2112, 2050), (2500, 6001), (3000, 3001), (4100, 3990),
+                                 (4095, 4096)])
+def test_large_matrices(r, c):
+    _check(_gradient(r, c))
+
+
 @pytest.mark.parametrize("steps", [1, 2, 3, 7, 12])
 def test_steps(steps):
     for r, c in ((40, 70), (150, 90), (300, 260)):
