@@ -124,18 +124,20 @@ __global__ __launch_bounds__(256) void muon_split(const MuonTable tb, float mu, 
         blk[2 * v + lh][l32] = split_pack(in ? ldexpf(w, power) * factor : 0.f);
     }
     __builtin_amdgcn_wave_barrier();
-    char* same = args->same[k] + ((size_t)(c / 32) * rp + r + l32) * 128 + 32 * lh;
-    char* turned = args->turned[k] + ((size_t)(r / 32) * cp + c + l32) * 128 + 32 * lh;
+    // four lanes a row: a store covers whole pieces of 64 bytes
+    const int row = lane >> 2, col = 8 * (lane & 3);
+    char* same = args->same[k] + ((size_t)(c / 32) * rp + r + row) * 128 + 2 * col;
+    char* turned = args->turned[k] + ((size_t)(r / 32) * cp + c + row) * 128 + 2 * col;
 #pragma unroll
-    for (int q = 0; q < 2; ++q) {
+    for (int h = 0; h < 2; ++h) {
         unsigned s[8], t[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            s[e] = blk[l32][16 * lh + 8 * q + e];
-            t[e] = blk[16 * lh + 8 * q + e][l32];
+            s[e] = blk[16 * h + row][col + e];
+            t[e] = blk[col + e][16 * h + row];
         }
-        split_store<8>(same + 16 * q, s);
-        split_store<8>(turned + 16 * q, t);
+        split_store<8>(same + 2048 * h, s);
+        split_store<8>(turned + 2048 * h, t);
     }
 }
 
@@ -457,9 +459,7 @@ static int muon_launch_tile(int tile, const SplitTable& tb, float lr, const doub
         if (tile == kTile96) return muon_launch<96, 96, 48, 48, 3, 16, USE>(tb, lr, state, wd);
         if (tile == kTile160) return muon_launch<160, 160, 80, 80, 3, 16, USE>(tb, lr, state, wd);
         if (tile == kTile192) return muon_launch<192, 192, 96, 96, 3, 16, USE>(tb, lr, state, wd);
-        if constexpr (USE == kSplitGram || USE == kSplitPoly) {
-            if (tile == kTile48) return muon_launch<48, 48, 48, 16, 4, 16, USE>(tb, lr, state, wd);
-        } else {
+        if constexpr (USE == kSplitStep || USE == kSplitApply) {
             if (tile == kTile256x128) return muon_launch<256, 128, 64, 64, 3, 32, USE>(tb, lr, state, wd);
         }
     }

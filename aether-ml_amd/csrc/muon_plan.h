@@ -58,24 +58,23 @@ static inline int64_t muon_tiles(int64_t rows, int64_t cols, int bm, int bn, boo
 // CU (its first loads and its epilogue, as far as no other tile hides them), then us a slab of 32 columns on a CU whose neighbours
 // are idle (`alone`) and with a tile on every CU (`full`: the tiles then share the L2 caches' bandwidth and the power that the
 // matrix units may draw).  CUs with one tile more than others hold the launch up by `slack` of that tile (several small tiles are
-// on a CU at once).  Fitted to square and wide products of 64 to 4096 rows, and the tile with the least cost is taken: 3000 x 3000
-// gram 99 us in tiles of 160 x 160 (120 in 96, 121 in 192, 132 in 64), step 140 in 192 x 192 (169 in 96); 1000 x 1537 gram 14.3 in
-// 48 x 48 (15.5 in 64); 4096 x 4096 gram 190 in 192 x 192 (240 in 160), step 350 in 256 x 128 (373 in 192 x 192).
+// on a CU at once).  Fitted to square and wide products of 64 to 4096 rows; the tile with the least cost is taken: 3000 x 3000
+// gram 94 us in tiles of 160 x 160 (120 in 96, 121 in 192, 132 in 64), step 136 in 192 x 192 (169 in 96); 4096 x 4096 gram 180 in
+// 192 x 192 (240 in 160), step 330 in 256 x 128 (373 in 192 x 192).
 struct MuonTile {
     int bm, bn;
     bool symmetric, general, runs;     // offered for symmetric results, for others, for gram products in runs
     float start, again, slack, alone, full;
 };
-enum { kTile32, kTile48, kTile64, kTile96, kTile128, kTile160, kTile192, kTile256x128, kMuonTiles };
+enum { kTile32, kTile64, kTile96, kTile128, kTile160, kTile192, kTile256x128, kMuonTiles };
 static const MuonTile kMuonTileTable[kMuonTiles] = {
     {32, 32, true, true, true, 3.3f, 4.0f, 0.2f, 0.11f, 0.12f},
-    {48, 48, true, false, false, 5.0f, 0.5f, 0.6f, 0.17f, 0.20f},
     {64, 64, true, true, true, 4.5f, 0.5f, 0.5f, 0.21f, 0.25f},
-    {96, 96, true, true, false, 8.0f, 1.0f, 0.6f, 0.33f, 0.48f},
+    {96, 96, true, true, false, 6.0f, 1.0f, 0.6f, 0.33f, 0.48f},
     {128, 128, true, true, true, 6.0f, 1.0f, 1.0f, 0.50f, 0.74f},
-    {160, 160, true, true, false, 14.0f, 2.0f, 1.0f, 0.75f, 0.96f},
-    {192, 192, true, true, false, 17.0f, 2.0f, 1.0f, 1.00f, 1.34f},
-    {256, 128, false, true, false, 8.0f, 2.0f, 1.0f, 0.95f, 1.30f},
+    {160, 160, true, true, false, 10.0f, 2.0f, 1.0f, 0.75f, 0.96f},
+    {192, 192, true, true, false, 10.0f, 2.0f, 1.0f, 1.00f, 1.34f},
+    {256, 128, false, true, false, 5.0f, 2.0f, 1.0f, 0.95f, 1.27f},
 };
 constexpr int kMuonCus = 256;
 

@@ -78,49 +78,44 @@ __device__ constexpr float split_scale() {
                                                   : 1.f / (kScaleB * kScaleX);
 }
 
-// One 32 x 32 block of the result, at row r and column c, by one wave: o[v] is row r + 8 (v / 4) + 4 (lane / 32) + v % 4, column
-// c + lane % 32, already scaled.  `blk`: LDS of the wave's own.
+// Half of a 32 x 32 block of a result (16 of its rows, or with `turned` of its columns) to its place in the result, or in the
+// transposed one: four lanes a row, eight elements each, so that a store covers whole pieces of 64 bytes.  t: the block in LDS,
+// [row][S], as halves (split_pack) or, for the polynomial, as float32 sums to which b A + a I is added here.  A and the result are
+// symmetric: either way round the same bits are added.
 template <int USE>
-__device__ __forceinline__ void split_emit(const SplitProduct& pr, float* o, int r, int c, unsigned (*blk)[33]) {
-    constexpr bool kSym = USE != kSplitStep;
-    const int lane = threadIdx.x & 63, l32 = lane & 31, lh = lane >> 5;
-    if (USE == kSplitPoly) {
-        // A[r][c] read as A[c][r]: four consecutive rows a load
-        const char* a = pr.A + ((size_t)(r / 32) * pr.M + c + l32) * 128 + 8 * lh;
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            const half4 h = *reinterpret_cast<const half4*>(a + 16 * q), l = *reinterpret_cast<const half4*>(a + 16 * q + 64);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) o[4 * q + e] += ((float)h[e] + (float)l[e]) * (kNsB * kScaleB / kScaleA);
+struct SplitRows {
+    size_t at;                                           // of the lane's eight high halves
+    half8 high, low;                                     // of A
+    __device__ __forceinline__ SplitRows(const SplitProduct& pr, int r, int c, bool turned, int h) {
+        const int lane = threadIdx.x & 63, row = 16 * h + (lane >> 2);
+        at = (turned ? (size_t)(r / 32) * pr.N + c + row : (size_t)(c / 32) * pr.M + r + row) * 128 + 16 * (lane & 3);
+        if (USE == kSplitPoly) {
+            high = *reinterpret_cast<const half8*>(pr.A + at);
+            low = *reinterpret_cast<const half8*>(pr.A + at + 64);
         }
-        if (r == c)
-#pragma unroll
-            for (int v = 0; v < 16; ++v)
-                if (8 * (v >> 2) + 4 * lh + (v & 3) == l32) o[v] += kNsA * kScaleB;
     }
-    unsigned w[16];
+    template <int S>
+    __device__ __forceinline__ void store(const SplitProduct& pr, const unsigned* t, int r, int c, bool turned, int h) const {
+        const int lane = threadIdx.x & 63, row = 16 * h + (lane >> 2), col = 8 * (lane & 3);
+        unsigned w[8];
 #pragma unroll
-    for (int v = 0; v < 16; ++v) w[v] = split_pack(o[v]);
-    // transposed: row c + l32, four consecutive columns a piece (not for diagonal blocks of a symmetric result: each place is
-    // written once, by one lane)
-    if (!(kSym && r == c)) {
-        char* d = (kSym ? pr.D1 : pr.D2) + ((size_t)(r / 32) * pr.N + c + l32) * 128 + 8 * lh;
+        for (int e = 0; e < 8; ++e) w[e] = turned ? t[(col + e) * S + row] : t[row * S + col + e];
+        if (USE == kSplitPoly)
 #pragma unroll
-        for (int q = 0; q < 4; ++q) split_store<4>(d + 16 * q, w + 4 * q);
+            for (int e = 0; e < 8; ++e) {
+                float o = __builtin_bit_cast(float, w[e]) + ((float)high[e] + (float)low[e]) * (kNsB * kScaleB / kScaleA);
+                if (r == c && row == col + e) o += kNsA * kScaleB;
+                w[e] = split_pack(o);
+            }
+        split_store<8>((turned && USE == kSplitStep ? pr.D2 : pr.D1) + at, w);
     }
-    // as it is: through LDS, so that a lane has 16 consecutive columns of row r + l32
-#pragma unroll
-    for (int v = 0; v < 16; ++v) blk[8 * (v >> 2) + 4 * lh + (v & 3)][l32] = w[v];
-    __builtin_amdgcn_wave_barrier();
-    char* d = pr.D1 + ((size_t)(c / 32) * pr.M + r + l32) * 128 + 32 * lh;
-#pragma unroll
-    for (int q = 0; q < 2; ++q) {
-        unsigned s[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) s[e] = blk[l32][16 * lh + 8 * q + e];
-        split_store<8>(d + 16 * q, s);
-    }
-    __builtin_amdgcn_wave_barrier();
+};
+
+// What lies in LDS of a sum.
+template <int USE>
+__device__ __forceinline__ unsigned split_word(float sum) {
+    const float o = sum * split_scale<USE>();
+    return USE == kSplitPoly ? __builtin_bit_cast(unsigned, o) : split_pack(o);
 }
 
 // The parameters of the product that tile (or workgroup) `tile` of the launch belongs to, by scalar loads from the kernel's
@@ -168,12 +163,12 @@ __device__ __forceinline__ SplitTile split_tile(const SplitProduct& pr, int t) {
     return at;
 }
 
-// One 32 x 32 block of a product's accumulators to where the product's use wants it; the block is inside the padded result.
+// One block of a product's accumulators to where a product with float32 results wants it; the block is inside the padded result.
+// 32 x 32: acc[v] is row r + 8 (v / 4) + 4 (lane / 32) + v % 4, column c + lane % 32.
 template <int USE>
-__device__ __forceinline__ void split_finish(const SplitProduct& pr, const f16v& acc, int r, int c, const SplitTile& at,
-                                             unsigned (*blk)[33], float keep, float step) {
+__device__ __forceinline__ void split_finish(const SplitProduct& pr, const f16v& acc, int r, int c, const SplitTile& at, float keep,
+                                             float step) {
     const int lane = threadIdx.x & 63, l32 = lane & 31, lh = lane >> 5;
-    constexpr float kOut = split_scale<USE>();
     if constexpr (USE == kSplitApply) {
         // (all the loads at once, from places clamped into the matrix: behind a branch each they came back one by one)
         const int x = c + l32, cc = min(x, pr.cols - 1), y0 = r + 4 * lh;
@@ -186,71 +181,38 @@ __device__ __forceinline__ void split_finish(const SplitProduct& pr, const f16v&
         for (int v = 0; v < 16; ++v) {
             const int y = y0 + 8 * (v >> 2) + (v & 3);
             if (y < pr.rows && x < pr.cols) {
-                const float o = acc[v] * kOut;
+                const float o = acc[v] * split_scale<USE>();
                 if (pr.theta != nullptr) pr.theta[(size_t)y * pr.cols + x] = keep * t[v] - step * o;
                 else pr.out[(size_t)y * pr.cols + x] = o;
             }
         }
-    } else if constexpr (USE == kSplitPart) {
+    } else {
+        static_assert(USE == kSplitPart, "the others go through LDS");
         const size_t side = pr.M / 32, x = c / 32, block = x * (x + 1) / 2 + r / 32;
         float* d = pr.part + ((size_t)(at.begin / pr.run) * (side * (side + 1) / 2) + block) * 1024 + lane * 4;
 #pragma unroll
         for (int q = 0; q < 4; ++q) *reinterpret_cast<f4*>(d + 256 * q) = f4{acc[4 * q], acc[4 * q + 1], acc[4 * q + 2], acc[4 * q + 3]};
-    } else {
-        float o[16];
-#pragma unroll
-        for (int v = 0; v < 16; ++v) o[v] = acc[v] * kOut;
-        split_emit<USE>(pr, o, r, c, blk);
     }
 }
 
-// The same for a 16 x 16 block: acc[e] is row r + 4 (lane / 16) + e, column c + lane % 16.
+// 16 x 16: acc[e] is row r + 4 (lane / 16) + e, column c + lane % 16.
 template <int USE>
-__device__ __forceinline__ void split_finish(const SplitProduct& pr, const f4& acc, int r, int c, const SplitTile& at,
-                                             unsigned (*blk)[33], float keep, float step) {
-    static_assert(USE != kSplitPart, "partial sums come in blocks of 32 x 32");
-    constexpr bool kSym = USE != kSplitStep;
-    const int lane = threadIdx.x & 63, l16 = lane & 15, lq = lane >> 4;
-    constexpr float kOut = split_scale<USE>();
-    if constexpr (USE == kSplitApply) {
-        const int x = c + l16, cc = min(x, pr.cols - 1), y0 = r + 4 * lq;
-        float t[4];
-        if (pr.theta != nullptr) {
+__device__ __forceinline__ void split_finish(const SplitProduct& pr, const f4& acc, int r, int c, const SplitTile&, float keep,
+                                             float step) {
+    static_assert(USE == kSplitApply, "partial sums come in blocks of 32 x 32, the others go through LDS");
+    const int lane = threadIdx.x & 63, x = c + (lane & 15), cc = min(x, pr.cols - 1), y0 = r + 4 * (lane >> 4);
+    float t[4];
+    if (pr.theta != nullptr) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) t[e] = pr.theta[(size_t)min(y0 + e, pr.rows - 1) * pr.cols + cc];
-        }
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-            if (y0 + e < pr.rows && x < pr.cols) {
-                const float o = acc[e] * kOut;
-                if (pr.theta != nullptr) pr.theta[(size_t)(y0 + e) * pr.cols + x] = keep * t[e] - step * o;
-                else pr.out[(size_t)(y0 + e) * pr.cols + x] = o;
-            }
-    } else {
-        const size_t turned = ((size_t)(r / 32) * pr.N + c + l16) * 128 + 2 * (r & 31) + 8 * lq;
-        float o[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[e] = acc[e] * kOut;
-        if (USE == kSplitPoly) {
-            const half4 h = *reinterpret_cast<const half4*>(pr.A + turned), l = *reinterpret_cast<const half4*>(pr.A + turned + 64);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                o[e] += ((float)h[e] + (float)l[e]) * (kNsB * kScaleB / kScaleA);
-                if (r == c && 4 * lq + e == l16) o[e] += kNsA * kScaleB;
-            }
-        }
-        unsigned w[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) w[e] = split_pack(o[e]);
-        if (!(kSym && r == c)) split_store<4>((kSym ? pr.D1 : pr.D2) + turned, w);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) blk[4 * lq + e][l16] = w[e];
-        __builtin_amdgcn_wave_barrier();
-#pragma unroll
-        for (int e = 0; e < 4; ++e) w[e] = blk[l16][4 * lq + e];
-        split_store<4>(pr.D1 + ((size_t)(c / 32) * pr.M + r + l16) * 128 + 2 * (c & 31) + 8 * lq, w);
-        __builtin_amdgcn_wave_barrier();
+        for (int e = 0; e < 4; ++e) t[e] = pr.theta[(size_t)min(y0 + e, pr.rows - 1) * pr.cols + cc];
     }
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        if (y0 + e < pr.rows && x < pr.cols) {
+            const float o = acc[e] * split_scale<USE>();
+            if (pr.theta != nullptr) pr.theta[(size_t)(y0 + e) * pr.cols + x] = keep * t[e] - step * o;
+            else pr.out[(size_t)(y0 + e) * pr.cols + x] = o;
+        }
 }
 
 __device__ __forceinline__ f16v split_mfma(const half8& a, const half8& b, const f16v& c) {
@@ -275,11 +237,12 @@ struct SplitAcc<16> {
 // One workgroup: BM x BN of the result, waves of WM x WN, slabs through a ring of NBUF LDS buffers, loaded straight into LDS
 // NBUF - 1 slabs ahead.  16-byte chunk c of row r lies at c ^ ((r >> 1) & 7): the 16 rows that a fragment read takes at a time
 // then lie in different banks.
-// BLOCK: the MFMA's result, 32 x 32 (16 columns a step) or 16 x 16 (32 columns, a whole slab).  The small one is for waves of 16, 48
-// or 80 rows or columns, and for 96 x 96: there it keeps one step's operands fewer (2048 x 2048 in 96 x 96 tiles: 42 us with four
-// waves of 48 x 48, 44 with three of 96 x 32; 4096 x 4096 in 192 x 192: 190 us, with 32 x 32 blocks 198).
-// Bound: with a tile on every CU, the power the matrix units draw (4096 x 4096: 1.1 PFLOP/s of float16, what a library's float16
-// product of that size reaches); below that what a CU can have in flight from the L2 caches, 85 GB/s.
+// BLOCK: the MFMA's result, 32 x 32 (16 columns a step) or 16 x 16 (32 columns, a whole slab).  The small one is for waves of 48 or 80
+// rows and columns, and for 96 x 96: there it keeps one step's operands fewer (2048 x 2048 in 96 x 96 tiles: 42 us with four waves
+// of 48 x 48, 44 with three of 96 x 32; 4096 x 4096 in 192 x 192: 190 us, with 32 x 32 blocks 198; before the results went through
+// LDS).
+// Bound: with a tile on every CU, the power the matrix units draw (4096 x 4096: 1.15-1.25 PFLOP/s of float16, what a library's
+// float16 product of that size reaches); below that what a CU can have in flight from the L2 caches, 85 GB/s.
 template <int BM, int BN, int WM, int WN, int NBUF, int BLOCK, int USE>
 __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN)) void split_product(const SplitTable tb, float lr,
                                                                            const double* __restrict__ state, float wd) {
@@ -287,9 +250,10 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN)) void split_product(cons
     constexpr int AL = BM / 8 / WAVES, BL = BN / 8 / WAVES;
     static_assert(AL * 8 * WAVES == BM && BL * 8 * WAVES == BN, "whole loads a wave");
     constexpr int BUF = (BM + BN) * 128;
-    static_assert(NBUF * BUF >= WAVES * 32 * 33 * 4, "the epilogue's blocks fit");
     constexpr bool kSym = USE == kSplitGram || USE == kSplitPoly || USE == kSplitPart;
-    __shared__ __attribute__((aligned(1024))) char lds[NBUF * BUF];
+    constexpr bool kTurned = USE == kSplitGram || USE == kSplitPoly || USE == kSplitStep;
+    constexpr int S = BN + 1, STAGE = kTurned ? BM * S * 4 : 0;
+    __shared__ __attribute__((aligned(1024))) char lds[NBUF * BUF > STAGE ? NBUF * BUF : STAGE];
 
     const int tile = xcd_contiguous_id(blockIdx.x, gridDim.x);
     const SplitProduct pr = split_find(tb, tile);
@@ -409,19 +373,43 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN)) void split_product(cons
     wait_loads<0>();
     asm volatile("s_barrier" ::: "memory");              // the epilogue uses the buffers as well
 
-    // block (i, j) of a wave: acc[v] = result[r][c], r = 8 (v / 4) + 4 lh + v % 4, c = l32 of the block
-    unsigned(*blk)[33] = reinterpret_cast<unsigned(*)[33]>(lds + wave * (32 * 33 * 4));
-    if (state != nullptr) lr = (float)state[3];
-    const float keep = 1.0f - lr * wd, step = lr * pr.gain;
+    if constexpr (kTurned) {
+        // The tile goes through LDS, where every wave reads whole blocks of 32 x 32 either way round (from the accumulators, in
+        // pieces of 8 or 16 bytes a row: 4096 x 4096 step 345 us instead of 330, 1024 x 4096 33 instead of 30).
+        unsigned* t = reinterpret_cast<unsigned*>(lds);
+        unsigned* mine = t + (wm + lane / BLOCK * 4) * S + wn + (lane & (BLOCK - 1));
 #pragma unroll
-    for (int i = 0; i < TM; ++i)
+        for (int i = 0; i < TM; ++i)
 #pragma unroll
-        for (int j = 0; j < TN; ++j) {
-            const int r = r0 + wm + BLOCK * i, c = c0 + wn + BLOCK * j;
+            for (int j = 0; j < TN; ++j)
+#pragma unroll
+                for (int v = 0; v < BLOCK * BLOCK / 64; ++v)
+                    mine[(BLOCK * i + 8 * (v >> 2) + (v & 3)) * S + BLOCK * j] = split_word<USE>(acc[i][j][v]);
+        __syncthreads();
+        for (int b = wave; b < (BM / 32) * (BN / 32); b += WAVES) {
+            const int i = b / (BN / 32), j = b % (BN / 32), r = r0 + 32 * i, c = c0 + 32 * j;
             if (r >= pr.M || c >= pr.N) continue;        // (whole blocks: both are multiples of 32)
             if (kSym && r > c) continue;                 // (below the diagonal of a diagonal tile: written from above it)
-            split_finish<USE>(pr, acc[i][j], r, c, at, blk, keep, step);
+            const unsigned* block = t + 32 * i * S + 32 * j;
+            const SplitRows<USE> top(pr, r, c, false, 0), bottom(pr, r, c, false, 1), left(pr, r, c, true, 0), right(pr, r, c, true, 1);
+            top.template store<S>(pr, block, r, c, false, 0);
+            bottom.template store<S>(pr, block, r, c, false, 1);
+            if (kSym && r == c) continue;                // (a diagonal block: each place is written once)
+            left.template store<S>(pr, block, r, c, true, 0);
+            right.template store<S>(pr, block, r, c, true, 1);
         }
+    } else {
+        if (state != nullptr) lr = (float)state[3];
+        const float keep = 1.0f - lr * wd, step = lr * pr.gain;
+#pragma unroll
+        for (int i = 0; i < TM; ++i)
+#pragma unroll
+            for (int j = 0; j < TN; ++j) {
+                const int r = r0 + wm + BLOCK * i, c = c0 + wn + BLOCK * j;
+                if (r >= pr.M || c >= pr.N || (kSym && r > c)) continue;
+                split_finish<USE>(pr, acc[i][j], r, c, at, keep, step);
+            }
+    }
 }
 
 // The same for products so small that a launch's time is what its loads and its epilogue take one after the other: a 32 x 32
@@ -487,26 +475,45 @@ __global__ __launch_bounds__(256) void split_block(const SplitTable tb, float lr
     // (every wave's loads have landed and its reads are done where it writes its sums: over its own ring)
     wait_loads<0>();
     f4* sums = reinterpret_cast<f4*>(ring);
+    constexpr bool kTurned = USE == kSplitGram || USE == kSplitPoly || USE == kSplitStep;
+    if constexpr (kTurned) {
+        // a quarter of the rows is added up by each wave, and each stores half of the block one way round
+        const bool turned = wave >= 2;
+        const SplitRows<USE> rows(pr, r0, c0, turned, wave & 1);
 #pragma unroll
-    for (int q = 0; q < 4; ++q) sums[64 * q + lane] = f4{acc[4 * q], acc[4 * q + 1], acc[4 * q + 2], acc[4 * q + 3]};
-    __syncthreads();
-    if (wave != 0) return;
+        for (int q = 0; q < 4; ++q) sums[64 * q + lane] = f4{acc[4 * q], acc[4 * q + 1], acc[4 * q + 2], acc[4 * q + 3]};
+        __syncthreads();
+        f4 sum = reinterpret_cast<const f4*>(lds)[64 * wave + lane];
 #pragma unroll
-    for (int w = 1; w < 4; ++w)
+        for (int w = 1; w < 4; ++w) sum += reinterpret_cast<const f4*>(lds + w * (NBUF * BUF))[64 * wave + lane];
+        unsigned* t = reinterpret_cast<unsigned*>(lds + 4096);                       // (behind the first wave's sums)
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            const f4 s = reinterpret_cast<const f4*>(lds + w * (NBUF * BUF))[64 * q + lane];
+        for (int e = 0; e < 4; ++e) t[(8 * wave + 4 * lh + e) * 33 + l32] = split_word<USE>(sum[e]);
+        __syncthreads();
+        if (USE != kSplitStep && r0 == c0 && turned) return;
+        rows.template store<33>(pr, t, r0, c0, turned, wave & 1);
+    } else {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) acc[4 * q + e] += s[e];
-        }
-    if (state != nullptr) lr = (float)state[3];
-    split_finish<USE>(pr, acc, r0, c0, at, reinterpret_cast<unsigned(*)[33]>(ring + 4096), 1.0f - lr * wd, lr * pr.gain);
+        for (int q = 0; q < 4; ++q) sums[64 * q + lane] = f4{acc[4 * q], acc[4 * q + 1], acc[4 * q + 2], acc[4 * q + 3]};
+        __syncthreads();
+        if (wave != 0) return;
+#pragma unroll
+        for (int w = 1; w < 4; ++w)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const f4 s = reinterpret_cast<const f4*>(lds + w * (NBUF * BUF))[64 * q + lane];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[4 * q + e] += s[e];
+            }
+        if (state != nullptr) lr = (float)state[3];
+        split_finish<USE>(pr, acc, r0, c0, at, 1.0f - lr * wd, lr * pr.gain);
+    }
 }
 
 // D1 = the sum of kSplitPart's runs: a 32 x 32 block a workgroup, every eighth run a wave, the waves' sums added in their order.
 __global__ __launch_bounds__(512) void split_join(const SplitTable tb) {
     __shared__ f4 sums[8][4][64];
-    __shared__ unsigned blk[32][33];
+    __shared__ unsigned block[32 * 33];
     const SplitProduct pr = split_find(tb, blockIdx.x);
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int side = pr.M / 32, count = side * (side + 1) / 2, t = (int)blockIdx.x - pr.first;
@@ -520,19 +527,19 @@ __global__ __launch_bounds__(512) void split_join(const SplitTable tb) {
 #pragma unroll
     for (int q = 0; q < 4; ++q) sums[wave][q][lane] = sum[q];
     __syncthreads();
-    if (wave != 0) return;
-    float o[16];
+    if (wave < 4) {
+        f4 v = sums[0][wave][lane];
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-        f4 s = sums[0][q][lane];
+        for (int w = 1; w < 8; ++w) v += sums[w][wave][lane];
 #pragma unroll
-        for (int w = 1; w < 8; ++w) s += sums[w][q][lane];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[4 * q + e] = s[e] * split_scale<kSplitGram>();
+        for (int e = 0; e < 4; ++e) block[(8 * wave + 4 * (lane >> 5) + e) * 33 + (lane & 31)] = split_word<kSplitGram>(v[e]);
     }
+    __syncthreads();
     int i, j;
     muon_triangle(t, &i, &j);
-    split_emit<kSplitGram>(pr, o, 32 * i, 32 * j, blk);
+    const bool turned = wave >= 2;
+    if (wave >= 4 || (turned && i == j)) return;
+    SplitRows<kSplitGram>(pr, 32 * i, 32 * j, turned, wave & 1).store<33>(pr, block, 32 * i, 32 * j, turned, wave & 1);
 }
 
 }  // namespace aeth
