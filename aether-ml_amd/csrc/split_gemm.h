@@ -160,67 +160,12 @@ __device__ __forceinline__ SplitTile split_tile(const SplitProduct& pr, int t) {
         at.j = in / height;
         at.i = band * 4 + in - at.j * height;
     }
+    // (the divisions are done in vector registers; what follows from them are the loads' scalar descriptors)
+    at.i = __builtin_amdgcn_readfirstlane(at.i);
+    at.j = __builtin_amdgcn_readfirstlane(at.j);
     return at;
 }
 
-// One block of a product's accumulators to where a product with float32 results wants it; the block is inside the padded result.
-// 32 x 32: acc[v] is row r + 8 (v / 4) + 4 (lane / 32) + v % 4, column c + lane % 32.
-template <int USE>
-__device__ __forceinline__ void split_finish(const SplitProduct& pr, const f16v& acc, int r, int c, const SplitTile& at, float keep,
-                                             float step) {
-    const int lane = threadIdx.x & 63, l32 = lane & 31, lh = lane >> 5;
-    if constexpr (USE == kSplitApply) {
-        // (all the loads at once, from places clamped into the matrix: behind a branch each they came back one by one)
-        const int x = c + l32, cc = min(x, pr.cols - 1), y0 = r + 4 * lh;
-        float t[16];
-        if (pr.theta != nullptr) {
-#pragma unroll
-            for (int v = 0; v < 16; ++v) t[v] = pr.theta[(size_t)min(y0 + 8 * (v >> 2) + (v & 3), pr.rows - 1) * pr.cols + cc];
-        }
-#pragma unroll
-        for (int v = 0; v < 16; ++v) {
-            const int y = y0 + 8 * (v >> 2) + (v & 3);
-            if (y < pr.rows && x < pr.cols) {
-                const float o = acc[v] * split_scale<USE>();
-                if (pr.theta != nullptr) pr.theta[(size_t)y * pr.cols + x] = keep * t[v] - step * o;
-                else pr.out[(size_t)y * pr.cols + x] = o;
-            }
-        }
-    } else {
-        static_assert(USE == kSplitPart, "the others go through LDS");
-        const size_t side = pr.M / 32, x = c / 32, block = x * (x + 1) / 2 + r / 32;
-        float* d = pr.part + ((size_t)(at.begin / pr.run) * (side * (side + 1) / 2) + block) * 1024 + lane * 4;
-#pragma unroll
-        for (int q = 0; q < 4; ++q) *reinterpret_cast<f4*>(d + 256 * q) = f4{acc[4 * q], acc[4 * q + 1], acc[4 * q + 2], acc[4 * q + 3]};
-    }
-}
-
-// 16 x 16: acc[e] is row r + 4 (lane / 16) + e, column c + lane % 16.
-template <int USE>
-__device__ __forceinline__ void split_finish(const SplitProduct& pr, const f4& acc, int r, int c, const SplitTile&, float keep,
-                                             float step) {
-    static_assert(USE == kSplitApply, "partial sums come in blocks of 32 x 32, the others go through LDS");
-    const int lane = threadIdx.x & 63, x = c + (lane & 15), cc = min(x, pr.cols - 1), y0 = r + 4 * (lane >> 4);
-    float t[4];
-    if (pr.theta != nullptr) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) t[e] = pr.theta[(size_t)min(y0 + e, pr.rows - 1) * pr.cols + cc];
-    }
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-        if (y0 + e < pr.rows && x < pr.cols) {
-            const float o = acc[e] * split_scale<USE>();
-            if (pr.theta != nullptr) pr.theta[(size_t)(y0 + e) * pr.cols + x] = keep * t[e] - step * o;
-            else pr.out[(size_t)(y0 + e) * pr.cols + x] = o;
-        }
-}
-
-__device__ __forceinline__ f16v split_mfma(const half8& a, const half8& b, const f16v& c) {
-    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
-}
-__device__ __forceinline__ f4 split_mfma(const half8& a, const half8& b, const f4& c) {
-    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
-}
 template <int BLOCK>
 struct SplitAcc;
 template <>
@@ -231,6 +176,44 @@ template <>
 struct SplitAcc<16> {
     typedef f4 type;
 };
+
+// theta <- keep theta - step D (or out = D) for one block of a product's accumulators: acc[v] is row r + 8 (v / 4) + 4 (lane / 32) +
+// v % 4 and column c + lane % 32 of a 32 x 32 block, row r + 4 (lane / 16) + v and column c + lane % 16 of a 16 x 16 one.
+// All the loads go out at once, from places clamped into the matrix: behind a branch each they came back one by one.
+template <int BLOCK>
+__device__ __forceinline__ void split_apply(const SplitProduct& pr, const typename SplitAcc<BLOCK>::type& acc, int r, int c, float keep,
+                                            float step) {
+    constexpr int N = BLOCK * BLOCK / 64;
+    const int lane = threadIdx.x & 63, x = c + (lane & (BLOCK - 1)), cc = min(x, pr.cols - 1), y0 = r + lane / BLOCK * 4;
+    float t[N];
+    if (pr.theta != nullptr) {
+#pragma unroll
+        for (int v = 0; v < N; ++v) t[v] = pr.theta[(size_t)min(y0 + 8 * (v >> 2) + (v & 3), pr.rows - 1) * pr.cols + cc];
+    }
+#pragma unroll
+    for (int v = 0; v < N; ++v) {
+        const int y = y0 + 8 * (v >> 2) + (v & 3);
+        if (y < pr.rows && x < pr.cols) {
+            const float o = acc[v] * split_scale<kSplitApply>();
+            if (pr.theta != nullptr) pr.theta[(size_t)y * pr.cols + x] = keep * t[v] - step * o;
+            else pr.out[(size_t)y * pr.cols + x] = o;
+        }
+    }
+}
+
+// The partial sums of a 32 x 32 block, as the matrix instruction leaves them: quarter q of them (lane's sums 4 q .. 4 q + 3).
+__device__ __forceinline__ void split_part(const SplitProduct& pr, const f4& sums, int q, int r, int c, const SplitTile& at) {
+    const size_t side = pr.M / 32, x = c / 32, block = x * (x + 1) / 2 + r / 32;
+    float* d = pr.part + ((size_t)(at.begin / pr.run) * (side * (side + 1) / 2) + block) * 1024;
+    *reinterpret_cast<f4*>(d + 256 * q + 4 * (threadIdx.x & 63)) = sums;
+}
+
+__device__ __forceinline__ f16v split_mfma(const half8& a, const half8& b, const f16v& c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f4 split_mfma(const half8& a, const half8& b, const f4& c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
 
 // A matrix lies slab by slab: slab s holds columns 32 s .. 32 s + 31 of all R rows, row r's 128 bytes (64 of high halves, 64 of low)
 // at (s R + r) * 128, so that what a tile reads at a time is one contiguous piece and no offset grows with the matrix.
@@ -251,8 +234,8 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN)) void split_product(cons
     static_assert(AL * 8 * WAVES == BM && BL * 8 * WAVES == BN, "whole loads a wave");
     constexpr int BUF = (BM + BN) * 128;
     constexpr bool kSym = USE == kSplitGram || USE == kSplitPoly || USE == kSplitPart;
-    constexpr bool kTurned = USE == kSplitGram || USE == kSplitPoly || USE == kSplitStep;
-    constexpr int S = BN + 1, STAGE = kTurned ? BM * S * 4 : 0;
+    constexpr bool kStaged = USE != kSplitPart && USE != kSplitApply;
+    constexpr int S = BN + 1, STAGE = kStaged ? BM * S * 4 : 0;
     __shared__ __attribute__((aligned(1024))) char lds[NBUF * BUF > STAGE ? NBUF * BUF : STAGE];
 
     const int tile = xcd_contiguous_id(blockIdx.x, gridDim.x);
@@ -373,32 +356,7 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN)) void split_product(cons
     wait_loads<0>();
     asm volatile("s_barrier" ::: "memory");              // the epilogue uses the buffers as well
 
-    if constexpr (kTurned) {
-        // The tile goes through LDS, where every wave reads whole blocks of 32 x 32 either way round (from the accumulators, in
-        // pieces of 8 or 16 bytes a row: 4096 x 4096 step 345 us instead of 330, 1024 x 4096 33 instead of 30).
-        unsigned* t = reinterpret_cast<unsigned*>(lds);
-        unsigned* mine = t + (wm + lane / BLOCK * 4) * S + wn + (lane & (BLOCK - 1));
-#pragma unroll
-        for (int i = 0; i < TM; ++i)
-#pragma unroll
-            for (int j = 0; j < TN; ++j)
-#pragma unroll
-                for (int v = 0; v < BLOCK * BLOCK / 64; ++v)
-                    mine[(BLOCK * i + 8 * (v >> 2) + (v & 3)) * S + BLOCK * j] = split_word<USE>(acc[i][j][v]);
-        __syncthreads();
-        for (int b = wave; b < (BM / 32) * (BN / 32); b += WAVES) {
-            const int i = b / (BN / 32), j = b % (BN / 32), r = r0 + 32 * i, c = c0 + 32 * j;
-            if (r >= pr.M || c >= pr.N) continue;        // (whole blocks: both are multiples of 32)
-            if (kSym && r > c) continue;                 // (below the diagonal of a diagonal tile: written from above it)
-            const unsigned* block = t + 32 * i * S + 32 * j;
-            const SplitRows<USE> top(pr, r, c, false, 0), bottom(pr, r, c, false, 1), left(pr, r, c, true, 0), right(pr, r, c, true, 1);
-            top.template store<S>(pr, block, r, c, false, 0);
-            bottom.template store<S>(pr, block, r, c, false, 1);
-            if (kSym && r == c) continue;                // (a diagonal block: each place is written once)
-            left.template store<S>(pr, block, r, c, true, 0);
-            right.template store<S>(pr, block, r, c, true, 1);
-        }
-    } else {
+    if constexpr (!kStaged) {
         if (state != nullptr) lr = (float)state[3];
         const float keep = 1.0f - lr * wd, step = lr * pr.gain;
 #pragma unroll
@@ -407,8 +365,40 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN)) void split_product(cons
             for (int j = 0; j < TN; ++j) {
                 const int r = r0 + wm + BLOCK * i, c = c0 + wn + BLOCK * j;
                 if (r >= pr.M || c >= pr.N || (kSym && r > c)) continue;
-                split_finish<USE>(pr, acc[i][j], r, c, at, keep, step);
+                if constexpr (USE == kSplitApply) {
+                    split_apply<BLOCK>(pr, acc[i][j], r, c, keep, step);
+                } else {
+#pragma unroll
+                    for (int q = 0; q < 4; ++q)
+                        split_part(pr, f4{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]}, q, r, c, at);
+                }
             }
+        return;
+    }
+    // The tile goes through LDS, where every wave reads whole blocks of 32 x 32 either way round (from the accumulators, in pieces of
+    // 8 or 16 bytes a row: 4096 x 4096 step 345 us instead of 330, 1024 x 4096 33 instead of 30; but the weights, whose rows the
+    // accumulators hold in pieces of 64 or 128 bytes, took 38 us that way instead of 32).
+    unsigned* t = reinterpret_cast<unsigned*>(lds);
+    unsigned* mine = t + (wm + lane / BLOCK * 4) * S + wn + (lane & (BLOCK - 1));
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int j = 0; j < TN; ++j)
+#pragma unroll
+            for (int v = 0; v < BLOCK * BLOCK / 64; ++v)
+                mine[(BLOCK * i + 8 * (v >> 2) + (v & 3)) * S + BLOCK * j] = split_word<USE>(acc[i][j][v]);
+    __syncthreads();
+    for (int b = wave; b < (BM / 32) * (BN / 32); b += WAVES) {
+        const int i = b / (BN / 32), j = b % (BN / 32), r = r0 + 32 * i, c = c0 + 32 * j;
+        if (r >= pr.M || c >= pr.N) continue;        // (whole blocks: both are multiples of 32)
+        if (kSym && r > c) continue;                 // (below the diagonal of a diagonal tile: written from above it)
+        const unsigned* block = t + 32 * i * S + 32 * j;
+        const SplitRows<USE> top(pr, r, c, false, 0), bottom(pr, r, c, false, 1), left(pr, r, c, true, 0), right(pr, r, c, true, 1);
+        top.template store<S>(pr, block, r, c, false, 0);
+        bottom.template store<S>(pr, block, r, c, false, 1);
+        if (kSym && r == c) continue;                // (a diagonal block: each place is written once)
+        left.template store<S>(pr, block, r, c, true, 0);
+        right.template store<S>(pr, block, r, c, true, 1);
     }
 }
 
@@ -475,38 +465,47 @@ __global__ __launch_bounds__(256) void split_block(const SplitTable tb, float lr
     // (every wave's loads have landed and its reads are done where it writes its sums: over its own ring)
     wait_loads<0>();
     f4* sums = reinterpret_cast<f4*>(ring);
-    constexpr bool kTurned = USE == kSplitGram || USE == kSplitPoly || USE == kSplitStep;
-    if constexpr (kTurned) {
-        // a quarter of the rows is added up by each wave, and each stores half of the block one way round
-        const bool turned = wave >= 2;
-        const SplitRows<USE> rows(pr, r0, c0, turned, wave & 1);
 #pragma unroll
-        for (int q = 0; q < 4; ++q) sums[64 * q + lane] = f4{acc[4 * q], acc[4 * q + 1], acc[4 * q + 2], acc[4 * q + 3]};
+    for (int q = 0; q < 4; ++q) sums[64 * q + lane] = f4{acc[4 * q], acc[4 * q + 1], acc[4 * q + 2], acc[4 * q + 3]};
+    // a quarter of the rows is added up by each wave: its sums e are row 8 wave + 4 lh + e, column l32
+    const auto add = [&] {
         __syncthreads();
         f4 sum = reinterpret_cast<const f4*>(lds)[64 * wave + lane];
 #pragma unroll
         for (int w = 1; w < 4; ++w) sum += reinterpret_cast<const f4*>(lds + w * (NBUF * BUF))[64 * wave + lane];
+        return sum;
+    };
+    if constexpr (USE == kSplitPart) {
+        split_part(pr, add(), wave, r0, c0, at);
+    } else if constexpr (USE == kSplitApply) {
+        if (state != nullptr) lr = (float)state[3];
+        const float keep = 1.0f - lr * wd, step = lr * pr.gain;
+        const int x = c0 + l32, y = r0 + 8 * wave + 4 * lh;
+        float* const theta = pr.theta;
+        float* d = pr.out;
+        if (theta != nullptr) d = theta;
+        d += x;
+        float w[4] = {0.f, 0.f, 0.f, 0.f};
+        if (theta != nullptr && x < pr.cols)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) w[e] = d[(size_t)min(y + e, pr.rows - 1) * pr.cols];
+        const f4 sum = add();
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const float o = sum[e] * split_scale<USE>();
+            if (x < pr.cols && y + e < pr.rows) d[(size_t)(y + e) * pr.cols] = theta != nullptr ? keep * w[e] - step * o : o;
+        }
+    } else {
+        // each stores half of the block one way round
+        const bool turned = wave >= 2;
+        const SplitRows<USE> rows(pr, r0, c0, turned, wave & 1);
+        const f4 sum = add();
         unsigned* t = reinterpret_cast<unsigned*>(lds + 4096);                       // (behind the first wave's sums)
 #pragma unroll
         for (int e = 0; e < 4; ++e) t[(8 * wave + 4 * lh + e) * 33 + l32] = split_word<USE>(sum[e]);
         __syncthreads();
         if (USE != kSplitStep && r0 == c0 && turned) return;
         rows.template store<33>(pr, t, r0, c0, turned, wave & 1);
-    } else {
-#pragma unroll
-        for (int q = 0; q < 4; ++q) sums[64 * q + lane] = f4{acc[4 * q], acc[4 * q + 1], acc[4 * q + 2], acc[4 * q + 3]};
-        __syncthreads();
-        if (wave != 0) return;
-#pragma unroll
-        for (int w = 1; w < 4; ++w)
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const f4 s = reinterpret_cast<const f4*>(lds + w * (NBUF * BUF))[64 * q + lane];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) acc[4 * q + e] += s[e];
-            }
-        if (state != nullptr) lr = (float)state[3];
-        split_finish<USE>(pr, acc, r0, c0, at, 1.0f - lr * wd, lr * pr.gain);
     }
 }
 
