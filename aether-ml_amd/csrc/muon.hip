@@ -136,8 +136,13 @@ __global__ __launch_bounds__(256) void muon_split(const MuonTable tb, float mu, 
             s[e] = blk[16 * h + row][col + e];
             t[e] = blk[col + e][16 * h + row];
         }
-        split_store<8>(same + 2048 * h, s);
-        split_store<8>(turned + 2048 * h, t);
+        u32x4 hi, lo;
+        split_halves(s, hi, lo);
+        *reinterpret_cast<u32x4*>(same + 2048 * h) = hi;
+        *reinterpret_cast<u32x4*>(same + 2048 * h + 64) = lo;
+        split_halves(t, hi, lo);
+        *reinterpret_cast<u32x4*>(turned + 2048 * h) = hi;
+        *reinterpret_cast<u32x4*>(turned + 2048 * h + 64) = lo;
     }
 }
 

@@ -55,18 +55,13 @@ __device__ __forceinline__ unsigned split_pack(float v) {
     return (unsigned)__builtin_bit_cast(unsigned short, hi) | (unsigned)__builtin_bit_cast(unsigned short, lo) << 16;
 }
 
-// N neighbouring elements (4 or 8) of a row: high halves to p, low halves 64 bytes behind
-template <int N>
-__device__ __forceinline__ void split_store(char* p, const unsigned* w) {
-    typedef unsigned words __attribute__((ext_vector_type(N / 2)));
-    words hi, lo;
+// Eight neighbouring elements of a row: their high halves, their low halves
+__device__ __forceinline__ void split_halves(const unsigned* w, u32x4& hi, u32x4& lo) {
 #pragma unroll
-    for (int e = 0; e < N / 2; ++e) {
+    for (int e = 0; e < 4; ++e) {
         hi[e] = __builtin_amdgcn_perm(w[2 * e + 1], w[2 * e], 0x05040100u);
         lo[e] = __builtin_amdgcn_perm(w[2 * e + 1], w[2 * e], 0x07060302u);
     }
-    *reinterpret_cast<words*>(p) = hi;
-    *reinterpret_cast<words*>(p + 64) = lo;
 }
 
 // What a product's accumulators are times the stored result's scale.
@@ -79,19 +74,21 @@ __device__ constexpr float split_scale() {
 }
 
 // Half of a 32 x 32 block of a result (16 of its rows, or with `turned` of its columns) to its place in the result, or in the
-// transposed one: four lanes a row, eight elements each, so that a store covers whole pieces of 64 bytes.  t: the block in LDS,
-// [row][S], as halves (split_pack) or, for the polynomial, as float32 sums to which b A + a I is added here.  A and the result are
-// symmetric: either way round the same bits are added.
+// transposed one: four lanes a row, eight elements each, so that a store covers whole pieces of 64 bytes.  r, c, turned, h are
+// uniform.  t: the block in LDS, [row][S], as halves (split_pack) or, for the polynomial, as float32 sums to which b A + a I is
+// added here.  A and the result are symmetric: either way round the same bits are added.
 template <int USE>
 struct SplitRows {
-    size_t at;                                           // of the lane's eight high halves
+    size_t block;                                        // of the block's 4096 bytes
+    unsigned at;                                         // in them: the lane's eight high halves
     half8 high, low;                                     // of A
     __device__ __forceinline__ SplitRows(const SplitProduct& pr, int r, int c, bool turned, int h) {
-        const int lane = threadIdx.x & 63, row = 16 * h + (lane >> 2);
-        at = (turned ? (size_t)(r / 32) * pr.N + c + row : (size_t)(c / 32) * pr.M + r + row) * 128 + 16 * (lane & 3);
+        const int lane = threadIdx.x & 63;
+        block = (turned ? (size_t)(r / 32) * pr.N + c : (size_t)(c / 32) * pr.M + r) * 128;
+        at = (16 * h + (lane >> 2)) * 128 + 16 * (lane & 3);
         if (USE == kSplitPoly) {
-            high = *reinterpret_cast<const half8*>(pr.A + at);
-            low = *reinterpret_cast<const half8*>(pr.A + at + 64);
+            high = *reinterpret_cast<const half8*>(pr.A + block + at);
+            low = *reinterpret_cast<const half8*>(pr.A + block + at + 64);
         }
     }
     template <int S>
@@ -107,7 +104,14 @@ struct SplitRows {
                 if (r == c && row == col + e) o += kNsA * kScaleB;
                 w[e] = split_pack(o);
             }
-        split_store<8>((turned && USE == kSplitStep ? pr.D2 : pr.D1) + at, w);
+        u32x4 hi, lo;
+        split_halves(w, hi, lo);
+        // Written through to memory at once (the last argument's bit 4), where the next launch's other dies read it: what stays
+        // in an L2 cache is written back between the launches (1000 x 1537 step 17.7 us, so 16.4).
+        const __amdgpu_buffer_rsrc_t d =
+            __builtin_amdgcn_make_buffer_rsrc((turned && USE == kSplitStep ? pr.D2 : pr.D1) + block, 0, 4096, 0x00020000);
+        __builtin_amdgcn_raw_buffer_store_b128(hi, d, (int)at, 0, 16);
+        __builtin_amdgcn_raw_buffer_store_b128(lo, d, (int)at + 64, 0, 16);
     }
 };
 
@@ -536,6 +540,8 @@ __global__ __launch_bounds__(512) void split_join(const SplitTable tb) {
     __syncthreads();
     int i, j;
     muon_triangle(t, &i, &j);
+    i = __builtin_amdgcn_readfirstlane(i);
+    j = __builtin_amdgcn_readfirstlane(j);
     const bool turned = wave >= 2;
     if (wave >= 4 || (turned && i == j)) return;
     SplitRows<kSplitGram>(pr, 32 * i, 32 * j, turned, wave & 1).store<33>(pr, block, 32 * i, 32 * j, turned, wave & 1);
