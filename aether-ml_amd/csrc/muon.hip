@@ -570,8 +570,8 @@ static int muon_group(const MuonMatrix* t, int count, float lr, const double* st
 }
 
 // The column blocks a wave of muon_whole would have, 0 where a matrix is too large for it.  Its registers hold six blocks of 32 x 32 a
-// wave, and that is also where the launches of all CUs catch up: five steps on 64 rows take 22 us at 64 columns, 29 at 256, 55 at
-// 576 and 74 at 1024 in one workgroup, 71 to 76 in launches.
+// wave, and that is also where the launches of all CUs catch up: an update of 64 rows takes 22 us at 64 columns, 29 at 256, 50 at
+// 576 (58 on the transpose) and 59 at 768 in one workgroup, 55 to 65 in seventeen launches as fast as the host can queue them.
 static int muon_whole_blocks(const MuonMatrix* t, int count, int* row_blocks) {
     int m = 0, n = 0;
     for (int i = 0; i < count; ++i) {

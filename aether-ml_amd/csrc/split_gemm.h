@@ -64,6 +64,9 @@ __device__ __forceinline__ void split_halves(const unsigned* w, u32x4& hi, u32x4
     }
 }
 
+// A buffer store's cache policy: through the L2 cache (device scope)
+constexpr int kThrough = 16;
+
 // What a product's accumulators are times the stored result's scale.
 template <int USE>
 __device__ constexpr float split_scale() {
@@ -106,12 +109,12 @@ struct SplitRows {
             }
         u32x4 hi, lo;
         split_halves(w, hi, lo);
-        // Written through to memory at once (the last argument's bit 4), where the next launch's other dies read it: what stays
-        // in an L2 cache is written back between the launches (1000 x 1537 step 17.7 us, so 16.4).
+        // Written through to memory at once (kThrough), where the next launch's other dies read it: what stays in an L2 cache is
+        // written back between the launches (1000 x 1537 step 17.0 us, so 16.2).
         const __amdgpu_buffer_rsrc_t d =
             __builtin_amdgcn_make_buffer_rsrc((turned && USE == kSplitStep ? pr.D2 : pr.D1) + block, 0, 4096, 0x00020000);
-        __builtin_amdgcn_raw_buffer_store_b128(hi, d, (int)at, 0, 16);
-        __builtin_amdgcn_raw_buffer_store_b128(lo, d, (int)at + 64, 0, 16);
+        __builtin_amdgcn_raw_buffer_store_b128(hi, d, (int)at, 0, kThrough);
+        __builtin_amdgcn_raw_buffer_store_b128(lo, d, (int)at + 64, 0, kThrough);
     }
 };
 
@@ -209,7 +212,8 @@ __device__ __forceinline__ void split_apply(const SplitProduct& pr, const typena
 __device__ __forceinline__ void split_part(const SplitProduct& pr, const f4& sums, int q, int r, int c, const SplitTile& at) {
     const size_t side = pr.M / 32, x = c / 32, block = x * (x + 1) / 2 + r / 32;
     float* d = pr.part + ((size_t)(at.begin / pr.run) * (side * (side + 1) / 2) + block) * 1024;
-    *reinterpret_cast<f4*>(d + 256 * q + 4 * (threadIdx.x & 63)) = sums;
+    const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc(d, 0, 4096, 0x00020000);
+    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, sums), rsrc, 1024 * q + 16 * (int)(threadIdx.x & 63), 0, kThrough);
 }
 
 __device__ __forceinline__ f16v split_mfma(const half8& a, const half8& b, const f16v& c) {
