@@ -596,8 +596,8 @@ static int muon_small(const MuonMatrix* t, int count, int row_blocks, int blocks
     for (int i = 0; i < count; ++i) tb.t[i] = t[i];
     const int c = blocks <= 1 ? 0 : blocks <= 2 ? 1 : blocks <= 4 ? 2 : 3;
     const int update = t[0].mom != nullptr;
-    hipLaunchKernelGGL(row_blocks == 1 ? one[update][c] : two[update][c], dim3(count), dim3(64 * kWholeWaves), 0, ctx().stream, tb, mu, nesterov, lr,
-                       state, wd, steps);
+    hipLaunchKernelGGL(row_blocks == 1 ? one[update][c] : two[update][c], dim3(count), dim3(64 * kWholeWaves), 0, ctx().stream, tb, mu,
+                       nesterov, lr, state, wd, steps);
     AETH_LAUNCH_CHECK();
     return AETH_OK;
 }

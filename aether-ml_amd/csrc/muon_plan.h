@@ -1,7 +1,8 @@
 // How a call's matrices are laid out and cut into tiles for the Newton-Schulz products.  Free of HIP calls, so that the host
 // can check it without a GPU.
 //
-// A matrix is held as two float16 halves (split_gemm.h) in slabs of 32 columns.  Rows and columns are padded to multiples of 32 with zeros; zeros stay zeros through all products.
+// A matrix is held as two float16 halves (split_gemm.h) in slabs of 32 columns.  Rows and columns are padded to multiples of 32 with
+// zeros; zeros stay zeros through all products.
 #pragma once
 
 #include <stdint.h>

@@ -255,7 +255,8 @@ __global__ __launch_bounds__(kLnLong) void ln_fwd_rows(const LnFwdArgs p) {
 
 // ---- backward ----------------------------------------------------------------------------------------------------------
 // Bound: HBM, 12 bytes an element (14 with the bfloat16 copy): 65536 x 1024 152 us = 5.3 TB/s, 802816 x 64 115 us = 5.4 TB/s, ragged
-// rows 4.6-5.2 TB/s; a short call (5003 x 1537, 92 MB, 23 us) pays for two launches.  x and dy are read once: the same lanes hold the row while its
+// rows 4.6-5.2 TB/s; a short call (5003 x 1537, 92 MB, 22 us) pays for two launches.  x and dy are read once: the same lanes hold the row
+// while its
 // two sums are taken, and the lane that owns a column adds its dy xhat and dy over all rows it sees.  A workgroup walks many
 // rows and leaves one partial row of dgamma and one of dbeta, part[block][2][C]; ln_bwd_finish adds those in block order.
 struct LnBwdArgs {
