@@ -69,6 +69,29 @@ def test_large_matrices(r, c):
     _check(_gradient(r, c))
 
 
+@pytest.mark.parametrize("r,tall", [(3, False), (3, True), (260, False), (260, True)])
+def test_the_longest_matrices(r, tall):
+    """2^21 columns (or rows), the buffers past 2^31 bytes at 260 rows.  n copies of a matrix H beside each other have H's
+    left singular vectors and n of the right ones' copies: their result is H's, over sqrt(n), n times.  Sums of K products
+    in float32, a rounding for 16 of them: at most 3 K / 16 2^-24 = 2.4 % of a sum for the three parts of a product; a
+    singular value's change is the same part of itself or less; an offset that wraps changes all of a result."""
+    from aether import DeviceTensor
+    lib, check = _lib()
+    h = _gradient(r, 4096, seed=9)
+    tol, exact = R.tolerance(h)
+    n = (1 << 21) // 4096
+    g = np.tile(h, (1, n))
+    gd = _dev(np.ascontiguousarray(g.T) if tall else g)
+    o = DeviceTensor.full(gd.shape, np.nan)
+    check(lib.aeth_newton_schulz_f32(gd.ptr, o.ptr, gd.shape[0], gd.shape[1], 5))
+    del g
+    o = o.get().T if tall else o.get()
+    want = (exact / np.sqrt(n)).astype(np.float32)
+    off = [np.linalg.norm(o[:, 4096 * k:4096 * (k + 1)] - want) for k in range(n)]
+    bound = (tol + 3 * (1 << 21) / 16 * 2.0 ** -24 * np.linalg.norm(exact)) / np.sqrt(n)
+    assert max(off) <= bound, (np.argmax(off), max(off), bound)
+
+
 @pytest.mark.parametrize("steps", [1, 2, 3, 7, 12])
 def test_steps(steps):
     for r, c in ((40, 70), (150, 90), (300, 260)):
