@@ -170,6 +170,43 @@ def test_a_row_of_more_columns_than_a_launch_has_threads_for():
         assert R.worst(g, w, b) <= 1, name
 
 
+@pytest.mark.parametrize("c", [64, 8192, 100000])
+def test_tensors_past_two_to_the_thirty_second_bytes(c):
+    """As many rows as the element limit allows, copies of a tile beside each other: every tile's output is the first one's,
+    also where the offset passes 2^31 and 2^32 bytes; dbeta is a sum of small integers, so exact."""
+    from aether import DeviceTensor
+    lib, check = _lib()
+    tile = (1 << 22) // c
+    rows = ((1 << 31) - 1) // c
+    x, gamma, beta, _ = _inputs(tile, c)
+    dy = np.random.RandomState(c).randint(-2, 3, (tile, c)).astype(np.float32)
+
+    def repeated(a):
+        t, one = DeviceTensor((rows, c)), _dev(a)
+        for r in range(0, rows, tile):
+            part = t[r:min(r + tile, rows)]
+            check(lib.aeth_memcpy_d2d(part.ptr, one.ptr, part.nbytes))
+        return t
+
+    xd, gd, bd = repeated(x), _dev(gamma), _dev(beta)
+    out, m, s = DeviceTensor((rows, c)), _nan(rows), _nan(rows)
+    check(lib.aeth_ln_fwd_f32(xd.ptr, gd.ptr, bd.ptr, m.ptr, s.ptr, out.ptr, rows, c, 1e-5))
+    want = _forward(x, gamma, beta)
+    places = [k * tile for k in (0, 1, (rows // tile) // 4, (rows // tile) // 2, rows // tile - 1, rows // tile)]
+    for r in places:
+        n = min(tile, rows - r)
+        assert np.array_equal(out[r:r + n].get(), want[0][:n]) and np.array_equal(m[r:r + n].get(), want[1][:n])
+    dyd, dg, db = repeated(dy), _nan(c), _nan(c)
+    check(lib.aeth_ln_bwd_f32(xd.ptr, dyd.ptr, gd.ptr, m.ptr, s.ptr, out.ptr, dg.ptr, db.ptr, rows, c))
+    back = _backward(x, dy, gamma, want[1], want[2])
+    for r in places:
+        n = min(tile, rows - r)
+        assert np.array_equal(out[r:r + n].get(), back[0][:n])
+    sums = dy.astype(np.int64).sum(0) * (rows // tile) + dy[:rows % tile].astype(np.int64).sum(0)
+    assert np.abs(sums).max() < 1 << 24
+    assert np.array_equal(db.get(), sums.astype(np.float32)) and np.all(np.isfinite(dg.get()))
+
+
 def test_no_rows():
     x, gamma, beta, _ = _inputs(1, 12)
     empty = np.zeros((0, 12), np.float32)
