@@ -220,6 +220,19 @@ def test_learning_rate_on_the_device():
     assert all(np.array_equal(p[0], q[0]) and np.array_equal(p[1], q[1]) for p, q in zip(a, b))
 
 
+def test_matrices_whose_buffers_go_out_in_groups():
+    """Buffers of more than 4 GiB together: one matrix after the other, with the bits of a call for each."""
+    cols = 1 << 20
+    tensors = []
+    for seed in (1, 2):
+        theta, grad, mom = _triple(260, 2048, seed)
+        tensors.append((np.tile(theta, (1, cols // 2048)), np.tile(grad, (1, cols // 2048)), np.tile(mom, (1, cols // 2048))))
+    both = _multi(tensors)
+    for t, got in zip(tensors, both):
+        want = _multi([t])[0]
+        assert np.array_equal(got[0], want[0]) and np.array_equal(got[1], want[1])
+
+
 def test_empty_matrices_are_skipped():
     tensors = [_triple(20, 30)]
     lib, check = _lib()
