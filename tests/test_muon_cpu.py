@@ -38,6 +38,7 @@ def _call(lib, dev=False, **changes):
     (dict(theta=None), "NULL"), (dict(grad=None), "NULL"), (dict(mom=None), "NULL"), (dict(rows=None), "NULL"),
     (dict(cols=None), "NULL"), (dict(theta=[A, None]), "NULL"), (dict(grad=[None, B]), "NULL"), (dict(mom=[D, None]), "NULL"),
     (dict(rows=[-1, 3]), "-1"), (dict(cols=[9, -200]), "-200"), (dict(rows=[1 << 16, 3], cols=[1 << 15, 3]), "65536"),
+    (dict(rows=[8, (1 << 21) + 1], cols=[9, 1]), "2097153"), (dict(rows=[8, 1], cols=[9, (1 << 21) + 1]), "2097153"),
     (dict(momentum=1.0), "momentum"), (dict(momentum=-0.1), "momentum"), (dict(momentum=float("nan")), "momentum"),
     (dict(lr=float("nan")), "learning rate"), (dict(lr=float("inf")), "learning rate"), (dict(wd=-1.0), "weight decay"),
     (dict(wd=float("nan")), "weight decay"), (dict(wd=float("inf")), "weight decay"),
@@ -55,7 +56,7 @@ def test_refusals(lib, changes, word):
 
 def test_refusals_of_the_orthogonalisation(lib):
     for args in ((None, B, 4, 5, 5), (A, None, 4, 5, 5), (A, A, 4, 5, 5), (A, A + 79 * 1, 4, 5, 5), (A + 4, A, 4, 5, 5),
-                 (A, B, -1, 5, 5), (A, B, 4, -5, 5), (A, B, 1 << 16, 1 << 15, 5), (A, B, 4, 5, 0), (A, B, 4, 5, 101)):
+                 (A, B, -1, 5, 5), (A, B, 4, -5, 5), (A, B, 1 << 16, 1 << 15, 5), (A, B, (1 << 21) + 1, 1, 5), (A, B, 1, (1 << 21) + 1, 5), (A, B, 4, 5, 0), (A, B, 4, 5, 101)):
         assert lib.aeth_newton_schulz_f32(*args) == -1, args
     assert _call(lib, dev=True, state=None) == -1
 
