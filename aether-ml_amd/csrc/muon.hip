@@ -11,6 +11,8 @@
 
 #include <math.h>
 
+#include <algorithm>
+
 namespace aeth {
 
 // One matrix of a call.  mom == NULL: grad is the update itself (orthogonalisation alone, written to out).
@@ -445,7 +447,8 @@ static int muon_launch(SplitTable tb, float lr, const double* state, float wd) {
         tb.p[i].first = (int)tiles;
         tb.p[i].tm = cdiv(tb.p[i].M, BM);
         tb.p[i].tn = cdiv(tb.p[i].N, BN);
-        tiles += muon_tiles(tb.p[i].M, tb.p[i].N, BM, BN, kSym) * (USE == kSplitPart ? tb.p[i].runs : 1);
+        tb.p[i].tiles = (int)muon_tiles(tb.p[i].M, tb.p[i].N, BM, BN, kSym) * (USE == kSplitPart ? tb.p[i].runs : 1);
+        tiles += tb.p[i].tiles;
     }
     if constexpr (BM == 32)
         hipLaunchKernelGGL((split_block<USE>), dim3((unsigned)tiles), dim3(256), 0, ctx().stream, tb, lr, state, wd);
@@ -486,7 +489,8 @@ static int muon_gram_runs(SplitTable tb, int tile) {
     for (int i = 0; i < tb.count; ++i) {
         tb.p[i].first = (int)groups;
         const int64_t side = tb.p[i].M / 32;
-        groups += side * (side + 1) / 2;
+        tb.p[i].tiles = (int)(side * (side + 1) / 2);
+        groups += tb.p[i].tiles;
     }
     hipLaunchKernelGGL(split_join, dim3((unsigned)groups), dim3(512), 0, ctx().stream, tb);
     AETH_LAUNCH_CHECK();
@@ -610,6 +614,11 @@ static int muon_run(MuonMatrix* t, int count, float lr, const double* state, flo
     int row_blocks;
     const int blocks = muon_whole_blocks(t, count, &row_blocks);
     if (blocks > 0) return muon_small(t, count, row_blocks, blocks, lr, state, mu, nesterov, wd, steps);
+    // the longest tiles first: what is left at a launch's end is short
+    std::stable_sort(t, t + count, [](const MuonMatrix& a, const MuonMatrix& b) {
+        const int n = a.rows > a.cols ? a.rows : a.cols, p = b.rows > b.cols ? b.rows : b.cols;
+        return n != p ? n > p : (a.rows < a.cols ? a.rows : a.cols) > (b.rows < b.cols ? b.rows : b.cols);
+    });
     for (int i = 0; i < count;) {
         int64_t bytes = 0;
         int k = 0;

@@ -72,10 +72,10 @@ static const MuonTile kMuonTileTable[kMuonTiles] = {
     {32, 32, true, true, true, 3.3f, 4.0f, 0.2f, 0.11f, 0.12f},
     {64, 64, true, true, true, 4.5f, 0.5f, 0.5f, 0.21f, 0.25f},
     {96, 96, true, true, false, 6.0f, 1.0f, 0.6f, 0.33f, 0.48f},
-    {128, 128, true, true, true, 6.0f, 1.0f, 1.0f, 0.50f, 0.74f},
-    {160, 160, true, true, false, 10.0f, 2.0f, 1.0f, 0.75f, 0.96f},
-    {192, 192, true, true, false, 10.0f, 2.0f, 1.0f, 1.00f, 1.34f},
-    {256, 128, false, true, false, 5.0f, 2.0f, 1.0f, 0.95f, 1.27f},
+    {128, 128, true, true, true, 6.0f, 5.0f, 1.0f, 0.50f, 0.74f},
+    {160, 160, true, true, false, 10.0f, 5.0f, 1.0f, 0.75f, 0.96f},
+    {192, 192, true, true, false, 10.0f, 5.0f, 1.0f, 1.00f, 1.34f},
+    {256, 128, false, true, false, 5.0f, 5.0f, 1.0f, 0.95f, 1.26f},
 };
 constexpr int kMuonCus = 256;
 
@@ -92,7 +92,7 @@ static inline float muon_slab(const MuonTile& t, int64_t tiles) {
     return t.alone + (t.full - t.alone) * (tiles < kMuonCus ? (float)tiles / kMuonCus : 1.f);
 }
 
-// What a launch of these products costs with one tile shape, in us.
+// What a launch of these products costs with one tile shape, in us: all tiles in turn, of average length, or one product's alone.
 static inline float muon_cost(const MuonTile& t, const MuonShape* p, int count, bool symmetric) {
     int64_t tiles = 0, slabs = 0;
     float longest = 0.f;
@@ -103,8 +103,8 @@ static inline float muon_cost(const MuonTile& t, const MuonShape* p, int count, 
         const float mine = muon_turns(t, n) * (float)(p[i].k / 32);
         if (mine > longest) longest = mine;
     }
-    const float even = (float)slabs / kMuonCus;
-    return t.start + t.again * (muon_turns(t, tiles) - 1.f) + (longest > even ? longest : even) * muon_slab(t, tiles);
+    const float turns = muon_turns(t, tiles), all = turns * (float)slabs / (float)tiles;
+    return t.start + t.again * (turns - 1.f) + (longest > all ? longest : all) * muon_slab(t, tiles);
 }
 
 static inline int muon_choose(const MuonShape* p, int count, bool symmetric) {
@@ -146,7 +146,8 @@ static inline bool muon_choose_runs(const MuonShape* p, int count, MuonRuns* out
             units += muon_tiles(p[i].rows, p[i].cols, t.bm, t.bn, true) * (p[i].k / 32);
             if (p[i].k / 32 > longest) longest = p[i].k / 32;
         }
-        for (r.run = (units + kMuonCus - 1) / kMuonCus; r.run < longest; r.run += (r.run + 3) / 4) {
+        // (from four runs a CU, where one alone would be too uneven, to one)
+        for (r.run = (units + 4 * kMuonCus - 1) / (4 * kMuonCus); r.run < longest; r.run += (r.run + 3) / 4) {
             int64_t tiles = 0, most = 0;
             r.bytes = 0;
             for (int i = 0; i < count; ++i) {

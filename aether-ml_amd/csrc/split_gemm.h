@@ -32,7 +32,7 @@ struct SplitProduct {
     float *theta, *out;
     int M, N, K;         // padded: rows of P, rows of Q, their columns
     int rows, cols;      // of theta
-    int first;           // this product's first tile
+    int first, tiles;    // this product's first tile; how many it has
     int tm, tn;          // tiles down and across
     int runs, run;       // kSplitPart: runs of so many slabs
     float* part;         // [run][32 x 32 block on or above the diagonal][1024]
@@ -43,6 +43,7 @@ struct SplitTable {
     int count;
     SplitProduct p[kMuonMax];
 };
+static_assert(sizeof(SplitTable) + 64 <= 4096, "a launch's arguments");
 
 // Scales of the stored halves: X's elements are at most 1.21 (the step's polynomial maps [0, 1.21] into itself), A = X X^T's at most
 // 1.47, the polynomial's a I + b A + c A^2 at most 3.45: all below 65504 times their scale's inverse.
@@ -125,15 +126,20 @@ __device__ __forceinline__ unsigned split_word(float sum) {
     return USE == kSplitPoly ? __builtin_bit_cast(unsigned, o) : split_pack(o);
 }
 
-// The parameters of the product that tile (or workgroup) `tile` of the launch belongs to, by scalar loads from the kernel's
-// arguments, of which the table is the first (an index into the struct itself would copy it to memory).
-__device__ __forceinline__ SplitProduct split_find(const SplitTable& tb, int tile) {
+// The parameters of the workgroup's product and the number of its tile in it, by scalar loads from the kernel's arguments, of which the
+// table is the first (an index into the struct itself would copy it to memory).  Neighbouring tiles are on one die, where they share
+// operands in its L2 cache, but product by product, so that every die has its share of the long ones: two products of 128 slabs and
+// four of 32 (272 and 544 tiles of 64 x 64) took 100 us with the launch's tiles dealt out as one row, and take 64; eight equal products
+// are 5 % slower for it.
+__device__ __forceinline__ SplitProduct split_find(const SplitTable& tb, int& tile) {
     typedef const SplitTable __attribute__((address_space(4)))* table_ptr;
     const table_ptr args = (table_ptr)__builtin_amdgcn_kernarg_segment_ptr();
+    const int group = blockIdx.x;
     int at = 0;
-    while (at + 1 < tb.count && tile >= args->p[at + 1].first) ++at;
+    while (at + 1 < tb.count && group >= args->p[at + 1].first) ++at;
     SplitProduct pr = tb.p[0];
     __builtin_memcpy(&pr, (const void*)(args->p + at), sizeof(pr));
+    tile = xcd_contiguous_id(group - pr.first, pr.tiles);
     return pr;
 }
 
@@ -246,9 +252,9 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN)) void split_product(cons
     constexpr int S = BN + 1, STAGE = kStaged ? BM * S * 4 : 0;
     __shared__ __attribute__((aligned(1024))) char lds[NBUF * BUF > STAGE ? NBUF * BUF : STAGE];
 
-    const int tile = xcd_contiguous_id(blockIdx.x, gridDim.x);
+    int tile;
     const SplitProduct pr = split_find(tb, tile);
-    const SplitTile at = split_tile<USE>(pr, tile - pr.first);
+    const SplitTile at = split_tile<USE>(pr, tile);
     const int slabs = at.slabs;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int r0 = at.i * BM, c0 = at.j * BN;
@@ -417,9 +423,9 @@ template <int USE>
 __global__ __launch_bounds__(256) void split_block(const SplitTable tb, float lr, const double* __restrict__ state, float wd) {
     constexpr int NBUF = 3, BUF = 64 * 128;
     __shared__ __attribute__((aligned(1024))) char lds[4 * NBUF * BUF];
-    const int tile = xcd_contiguous_id(blockIdx.x, gridDim.x);
+    int tile;
     const SplitProduct pr = split_find(tb, tile);
-    const SplitTile at = split_tile<USE>(pr, tile - pr.first);
+    const SplitTile at = split_tile<USE>(pr, tile);
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int l32 = lane & 31, lh = lane >> 5, r0 = at.i * 32, c0 = at.j * 32;
     const char *sp = pr.P + ((size_t)(at.begin + wave) * pr.M + r0) * 128, *sq = pr.Q + ((size_t)(at.begin + wave) * pr.N + c0) * 128;
@@ -521,9 +527,10 @@ __global__ __launch_bounds__(256) void split_block(const SplitTable tb, float lr
 __global__ __launch_bounds__(512) void split_join(const SplitTable tb) {
     __shared__ f4 sums[8][4][64];
     __shared__ unsigned block[32 * 33];
-    const SplitProduct pr = split_find(tb, blockIdx.x);
+    int t;
+    const SplitProduct pr = split_find(tb, t);
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-    const int side = pr.M / 32, count = side * (side + 1) / 2, t = (int)blockIdx.x - pr.first;
+    const int side = pr.M / 32, count = side * (side + 1) / 2;
     const float* p = pr.part + (size_t)t * 1024 + lane * 4;
     f4 sum[4] = {};
     const int runs = pr.runs;
