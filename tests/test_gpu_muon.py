@@ -199,6 +199,16 @@ def test_update(shapes, nesterov):
     assert all(np.array_equal(p[0], q[0]) and np.array_equal(p[1], q[1]) for p, q in zip(got, again))
 
 
+def test_update_of_large_and_small_matrices_together():
+    """Tiles of very different lengths in one launch, both orientations, more than the CUs at once."""
+    tensors = [_triple(r, c, seed=r + c + i) for i, (r, c) in enumerate(
+        [(500, 1200), (2000, 260), (1024, 3000), (64, 64), (3000, 1024), (700, 700), (1024, 3000), (3, 1), (1500, 1600)])]
+    for t, g in zip(tensors, _multi(tensors)):
+        want, m, bound = R.update(*t, 0.02, 0.95, 1, 0.01)
+        assert np.all(np.abs(g[1] - m) <= R.momentum_bound(t[1], t[2], 0.95))
+        assert np.linalg.norm(g[0] - want) <= bound
+
+
 def test_update_without_momentum_decay_or_gradient():
     theta, grad, mom = _triple(40, 60)
     zero = np.zeros_like(grad)
