@@ -256,9 +256,9 @@ __global__ __launch_bounds__(kLnLong) void ln_fwd_rows(const LnFwdArgs p) {
 // ---- backward ----------------------------------------------------------------------------------------------------------
 // Bound: HBM, 12 bytes an element (14 with the bfloat16 copy): 65536 x 1024 152 us = 5.3 TB/s, 802816 x 64 115 us = 5.4 TB/s, ragged
 // rows 4.6-5.2 TB/s; a short call (5003 x 1537, 92 MB, 22 us) pays for two launches.  x and dy are read once: the same lanes hold the row
-// while its
-// two sums are taken, and the lane that owns a column adds its dy xhat and dy over all rows it sees.  A workgroup walks many
+// while its two sums are taken, and the lane that owns a column adds its dy xhat and dy over all rows it sees.  A workgroup walks many
 // rows and leaves one partial row of dgamma and one of dbeta, part[block][2][C]; ln_bwd_finish adds those in block order.
+// Few rows: one launch (part == NULL), in which workgroups of their own read the columns a second time and write dgamma and dbeta.
 struct LnBwdArgs {
     const float *x, *dy, *gamma, *mean, *invstd;
     float* dx;
@@ -267,6 +267,8 @@ struct LnBwdArgs {
     float inv_c;
     float* part;
     bool stream;
+    int groups;                                          // workgroups of rows; those behind them have 32 columns each
+    float *dgamma, *dbeta;
 };
 
 // What a lane holds of a row: x and dy as loaded.
@@ -329,13 +331,34 @@ __device__ __forceinline__ void ln_bwd_row(const LnBwdArgs& p, int64_t r, const 
     }
 }
 
+// dgamma and dbeta of 32 columns, every `lanes`th row a lane, the lanes in order.
+__device__ __forceinline__ void ln_bwd_own_columns(const LnBwdArgs& p, int group, int lanes, float (*red)[32][33]) {
+    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, c = group * 32 + lane, cc = min(c, p.C - 1);
+    float a = 0.f, b = 0.f;
+#pragma unroll 8
+    for (int r = w; r < p.rows; r += lanes) {
+        const float g = p.dy[(size_t)r * p.C + cc];
+        a = fmaf(g, (p.x[(size_t)r * p.C + cc] - p.mean[r]) * p.invstd[r], a);
+        b += g;
+    }
+    red[0][w][lane] = a;
+    red[1][w][lane] = b;
+    __syncthreads();
+    if (w < 2 && c < p.C) {
+        float v = red[w][0][lane];
+        for (int i = 1; i < lanes; ++i) v += red[w][i][lane];
+        (w == 0 ? p.dgamma : p.dbeta)[c] = v;
+    }
+}
+
 // Rows of at most L V units, T / L of them at a time.  Up to V = 6 the next row's loads are on their way while this row's sums are
 // taken (beyond there are no registers for it; after the last row that row is read once more rather than have a branch around
 // the loads).
 template <int T, int L, int V, bool kTiny = false>
 __global__ __launch_bounds__(T) void ln_bwd_wave(const LnBwdArgs p) {
     constexpr bool kAhead = V <= 6;
-    __shared__ float red[T / 64][L * V * 4];
+    __shared__ float red[T / 64][L * V * 4], columns[2][32][33];
+    if ((int)blockIdx.x >= p.groups) return ln_bwd_own_columns(p, blockIdx.x - p.groups, T / 32, columns);
     const int s = threadIdx.x % L, C = p.C;
     const LnLane<V, kTiny> u(s, L, C);
     float gm[V][4], dg[V][4], db[V][4];
@@ -344,7 +367,7 @@ __global__ __launch_bounds__(T) void ln_bwd_wave(const LnBwdArgs p) {
     for (int j = 0; j < V; ++j)
 #pragma unroll
         for (int e = 0; e < 4; ++e) dg[j][e] = db[j][e] = 0.f;
-    const int step = gridDim.x * (T / L);
+    const int step = p.groups * (T / L);
     int64_t r = (int64_t)blockIdx.x * (T / L) + threadIdx.x / L;
     LnBwdRow<V> next;
     if (kAhead && r < p.rows) next.load(p, r, u);
@@ -360,6 +383,7 @@ __global__ __launch_bounds__(T) void ln_bwd_wave(const LnBwdArgs p) {
             a[1] = ln_group_sum<L>(a[1]);
         });
     }
+    if (p.part == nullptr) return;
     // the rows of a wave, then the waves in order
     float* out = p.part + (size_t)blockIdx.x * 2 * C;
 #pragma unroll
@@ -388,7 +412,8 @@ __global__ __launch_bounds__(T) void ln_bwd_wave(const LnBwdArgs p) {
 template <int T, int V>
 __global__ __launch_bounds__(T) void ln_bwd_block(const LnBwdArgs p) {
     constexpr bool kAhead = V <= 4;
-    __shared__ float red[2][2][16];
+    __shared__ float red[2][2][16], columns[2][32][33];
+    if ((int)blockIdx.x >= p.groups) return ln_bwd_own_columns(p, blockIdx.x - p.groups, blockDim.x >> 5, columns);
     LnTeam team(red);
     const int C = p.C;
     const LnLane<V> u(threadIdx.x, blockDim.x, C);
@@ -410,10 +435,11 @@ __global__ __launch_bounds__(T) void ln_bwd_block(const LnBwdArgs p) {
             ln_gains(p, u, gm);
         }
         const int64_t now = r;
-        r += gridDim.x;
+        r += p.groups;
         if (kAhead) next.load(p, r < p.rows ? r : now, u);
         ln_bwd_row(p, now, u, w, gm, dg, db, [&](float* a) { team.sum<2>(a); });
     }
+    if (p.part == nullptr) return;
     float* out = p.part + (size_t)blockIdx.x * 2 * C;
 #pragma unroll
     for (int j = 0; j < V; ++j) {
@@ -683,12 +709,21 @@ static int ln_bwd_impl(const float* x, const float* dy, const float* gamma, cons
             // 1024; 4096 x 16384: 171, 171, 170, 183); more leave more partial rows, a part of one leaves CUs idle
             cap = s.lanes < 0 ? 64 : 256 * (threads < 512 ? 512 / threads : 1);
         }
+        // One launch for few rows: 128 x 256 3.1 us instead of 5.6, 512 x 256 4.1 and 5.6, 512 x 2048 5.4 and 9.3, 128 x 8192 6.0 and 12.4,
+        // 256 x 20000 27 and 36; but a column's rows are one workgroup's: 1024 x 256 6.3 and 5.8, 512 x 8192 18 and 17
+        if (s.lanes >= 0 && rows <= (s.lanes > 0 ? 512 : 256)) {
+            const LnBwdArgs p{x, dy, gamma, mean, invstd, dx, dx16, rows, C, 1.0f / (float)C, nullptr, 4 * n >= kLnStreamBytes, turns, dgamma,
+                              dbeta};
+            hipLaunchKernelGGL(ln_bwd_kernel(s), dim3(turns + cdiv(C, 32)), dim3(threads), 0, st, p);
+            AETH_LAUNCH_CHECK();
+            return AETH_OK;
+        }
         // as many workgroups as are needed for each to take no more rows than with `cap` of them
         const int run = cdiv(turns, cap);
         blocks = cdiv(turns, run);
         const int rc = workspace((int64_t)2 * blocks * C * sizeof(float), &ws);
         if (rc) return rc;
-        const LnBwdArgs p{x, dy, gamma, mean, invstd, dx, dx16, rows, C, 1.0f / (float)C, (float*)ws, 4 * n >= kLnStreamBytes};
+        const LnBwdArgs p{x, dy, gamma, mean, invstd, dx, dx16, rows, C, 1.0f / (float)C, (float*)ws, 4 * n >= kLnStreamBytes, blocks, nullptr, nullptr};
         hipLaunchKernelGGL(ln_bwd_kernel(s), dim3(s.lanes < 0 ? (rows < 4096 ? rows : 4096) : blocks), dim3(threads), 0, st, p);
         AETH_LAUNCH_CHECK();
         if (s.lanes < 0) {
