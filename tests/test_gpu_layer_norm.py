@@ -67,7 +67,10 @@ SIZES = [(1, 1), (1, 4), (5, 1), (3, 2), (7, 3), (1, 256), (128, 256), (2, 15), 
          (31, 60), (130, 63), (257, 64), (17, 65), (19, 100), (5, 127), (66, 128), (5, 129), (12, 252), (3, 255), (3, 257),
          (7, 260), (4, 511), (6, 512), (3, 513), (5, 1000), (2, 1023), (9, 1024), (3, 1025), (2, 1537), (6, 2048), (3, 2049),
          (2, 4095), (5, 4096), (2, 4100), (2, 5001), (3, 8192), (2, 8193), (2, 8196), (2, 16384), (1, 16385), (3, 20000),
-         (1, 32768), (2, 32769), (1, 40004), (1, 70001), (3, 100000), (1000, 8), (2000, 5), (1500, 64), (1030, 100), (700, 1024)]
+         (1, 32768), (2, 32769), (1, 40004), (1, 70001), (3, 100000), (1000, 8), (2000, 5), (1500, 64), (1030, 100), (700, 1024),
+         # on both sides of the rows that the backward pass takes in one launch, every width above it
+         (512, 256), (513, 256), (513, 1), (600, 3), (530, 15), (777, 33), (640, 60), (520, 129), (530, 513), (521, 1023), (514, 1025),
+         (600, 1537), (513, 2048), (256, 2052), (257, 2052), (300, 4100), (258, 8193), (270, 16385), (257, 20000)]
 
 
 @pytest.mark.parametrize("rows,c", SIZES)
@@ -87,7 +90,8 @@ def test_forward_and_backward(rows, c):
     assert all(np.array_equal(a, b) for a, b in zip(again[:3], back[:3]))
 
 
-@pytest.mark.parametrize("rows,c", [(1, 1), (5, 3), (129, 64), (7, 100), (3, 1025), (40, 1024), (2, 20000), (1, 40001)])
+@pytest.mark.parametrize("rows,c", [(1, 1), (5, 3), (129, 64), (7, 100), (3, 1025), (40, 1024), (2, 20000), (1, 40001), (600, 100), (600, 3),
+                                    (300, 2500)])
 def test_twins_are_the_rounded_outputs(rows, c):
     x, gamma, beta, dy = _inputs(rows, c, seed=1)
     plain, twin = _forward(x, gamma, beta), _forward(x, gamma, beta, twin=True)
@@ -96,7 +100,8 @@ def test_twins_are_the_rounded_outputs(rows, c):
     assert all(np.array_equal(p, q) for p, q in zip(a[:3], b[:3])) and np.array_equal(b[3], O.bf16_bits(b[0]))
 
 
-@pytest.mark.parametrize("rows,c,skip", [(6, 64, 1), (6, 100, 2), (5, 1024, 3), (3, 4096, 1), (2, 20000, 3)])
+@pytest.mark.parametrize("rows,c,skip", [(6, 64, 1), (6, 100, 2), (5, 1024, 3), (3, 4096, 1), (2, 20000, 3), (520, 100, 2), (520, 1023, 3),
+                                         (260, 4099, 1)])
 def test_pointers_that_are_only_four_byte_aligned(rows, c, skip):
     """Views that start `skip` floats into a block: no 16-byte load is aligned, the results are those of aligned ones within
     the tolerance, and the floats in front of and behind the outputs stay."""
@@ -141,17 +146,17 @@ def test_rows_far_from_zero_and_constant_rows(c):
     assert np.array_equal(got[3], beta)
 
 
-@pytest.mark.parametrize("c", [3, 64, 1024, 33000])
-def test_bad_values_stay_in_their_row(c):
-    x, gamma, beta, dy = _inputs(6, c, seed=3)
+@pytest.mark.parametrize("rows,c", [(6, 3), (6, 64), (6, 1024), (6, 33000), (530, 3), (530, 64), (530, 1024), (270, 4000)])
+def test_bad_values_stay_in_their_row(rows, c):
+    x, gamma, beta, dy = _inputs(rows, c, seed=3)
     clean = _forward(x, gamma, beta)
     x[1, c // 2], x[4, 0] = np.nan, np.inf
     got = _forward(x, gamma, beta)
-    keep = [0, 2, 3, 5]
+    keep = [r for r in range(rows) if r not in (1, 4)]
     assert np.array_equal(got[0][keep], clean[0][keep])
     assert np.all(np.isnan(got[0][[1, 4]]))
     dx, dg, db, _ = _backward(x, dy, gamma, got[1], got[2])
-    x0, _, _, _ = _inputs(6, c, seed=3)
+    x0, _, _, _ = _inputs(rows, c, seed=3)
     want = _backward(x0, dy, gamma, clean[1], clean[2])
     assert np.array_equal(dx[keep], want[0][keep]) and np.all(np.isnan(dx[[1, 4]]))
     assert np.all(np.isnan(dg)) and np.array_equal(db, want[2])
@@ -292,13 +297,14 @@ def test_twin_for_a_bf16_convolution_and_behind_one():
     assert np.array_equal(norm.dinputs._bf16.get(), O.bf16_bits(norm.dinputs.get()))
 
 
-def test_recorded_and_replayed():
+@pytest.mark.parametrize("rows", [300, 600])
+def test_recorded_and_replayed(rows):
     """Forward and backward pass in a recording: every replay, with eager work of the same layer kind (and a larger
     workspace) between, equals the eager result bit for bit."""
     import aether
     lib, check = _lib()
     r = np.random.RandomState(7)
-    rows, c = 300, 130
+    c = 130
     gamma, beta = r.randn(c).astype(np.float32), r.randn(c).astype(np.float32)
     layer, other = aether.Layer_Norm(), aether.Layer_Norm()
     layer.set_parameters(gamma, beta)
