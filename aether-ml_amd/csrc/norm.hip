@@ -596,27 +596,24 @@ static LnShape ln_shape(int C, int most_threads, int most) {
 typedef void (*LnFwd)(const LnFwdArgs);
 typedef void (*LnBwd)(const LnBwdArgs);
 
+// Of fewer than 64 lanes ln_shape takes one unit or three (two and four are one and two of twice the lanes).
 template <int L>
 static LnFwd ln_fwd_wave_of(int v) {
-    static const LnFwd k[4] = {ln_fwd_wave<L, 1>, ln_fwd_wave<L, 2>, ln_fwd_wave<L, 3>, ln_fwd_wave<L, 4>};
-    return k[v - 1];
-}
-template <int T>
-static LnFwd ln_fwd_block_of(int v) {
-    static const LnFwd k[8] = {ln_fwd_block<T, 1>, ln_fwd_block<T, 2>, ln_fwd_block<T, 3>, ln_fwd_block<T, 4>,
-                               ln_fwd_block<T, 5>, ln_fwd_block<T, 6>, ln_fwd_block<T, 7>, ln_fwd_block<T, 8>};
-    return k[v - 1];
+    return v == 1 ? ln_fwd_wave<L, 1> : ln_fwd_wave<L, 3>;
 }
 static LnFwd ln_fwd_kernel(const LnShape& s) {
-    static const LnFwd wide[4] = {ln_fwd_wave<64, 5>, ln_fwd_wave<64, 6>, ln_fwd_wave<64, 7>, ln_fwd_wave<64, 8>};
+    static const LnFwd wave[8] = {ln_fwd_wave<64, 1>, ln_fwd_wave<64, 2>, ln_fwd_wave<64, 3>, ln_fwd_wave<64, 4>,
+                                  ln_fwd_wave<64, 5>, ln_fwd_wave<64, 6>, ln_fwd_wave<64, 7>, ln_fwd_wave<64, 8>};
+    static const LnFwd block[4] = {ln_fwd_block<512, 5>, ln_fwd_block<512, 6>, ln_fwd_block<512, 7>, ln_fwd_block<512, 8>};
+    static const LnFwd large[4] = {ln_fwd_block<1024, 5>, ln_fwd_block<1024, 6>, ln_fwd_block<1024, 7>, ln_fwd_block<1024, 8>};
     if (s.tiny) return ln_fwd_wave<4, 1, true>;
     switch (s.lanes) {
         case 4: return ln_fwd_wave_of<4>(s.v);
         case 8: return ln_fwd_wave_of<8>(s.v);
         case 16: return ln_fwd_wave_of<16>(s.v);
         case 32: return ln_fwd_wave_of<32>(s.v);
-        case 64: return s.v > 4 ? wide[s.v - 5] : ln_fwd_wave_of<64>(s.v);
-        case 0: return s.threads <= 512 ? ln_fwd_block_of<512>(s.v) : ln_fwd_block_of<1024>(s.v);
+        case 64: return wave[s.v - 1];
+        case 0: return s.v == 3 ? ln_fwd_block<512, 3> : s.threads <= 512 ? block[s.v - 5] : large[s.v - 5];
     }
     return ln_fwd_rows;
 }
@@ -624,23 +621,24 @@ static LnFwd ln_fwd_kernel(const LnShape& s) {
 constexpr int kLnBwdWaveThreads = 512;
 template <int L>
 static LnBwd ln_bwd_wave_of(int v) {
-    constexpr int T = kLnBwdWaveThreads;
-    static const LnBwd k[4] = {ln_bwd_wave<T, L, 1>, ln_bwd_wave<T, L, 2>, ln_bwd_wave<T, L, 3>, ln_bwd_wave<T, L, 4>};
-    return k[v - 1];
+    return v == 1 ? ln_bwd_wave<kLnBwdWaveThreads, L, 1> : ln_bwd_wave<kLnBwdWaveThreads, L, 3>;
 }
 static LnBwd ln_bwd_kernel(const LnShape& s) {
     constexpr int T = kLnBwdWaveThreads;
-    static const LnBwd wide[4] = {ln_bwd_wave<T, 64, 5>, ln_bwd_wave<T, 64, 6>, ln_bwd_wave<T, 64, 7>, ln_bwd_wave<T, 64, 8>};
-    static const LnBwd block[8] = {ln_bwd_block<512, 1>, ln_bwd_block<512, 2>, ln_bwd_block<512, 3>, ln_bwd_block<512, 4>,
-                                   ln_bwd_block<512, 5>, ln_bwd_block<512, 6>, ln_bwd_block<512, 7>, ln_bwd_block<512, 8>};
+    static const LnBwd wave[8] = {ln_bwd_wave<T, 64, 1>, ln_bwd_wave<T, 64, 2>, ln_bwd_wave<T, 64, 3>, ln_bwd_wave<T, 64, 4>,
+                                  ln_bwd_wave<T, 64, 5>, ln_bwd_wave<T, 64, 6>, ln_bwd_wave<T, 64, 7>, ln_bwd_wave<T, 64, 8>};
+    static const LnBwd ahead[3] = {ln_bwd_block<512, 2>, ln_bwd_block<512, 3>, ln_bwd_block<512, 4>};
+    static const LnBwd block[3] = {ln_bwd_block<512, 6>, ln_bwd_block<512, 7>, ln_bwd_block<512, 8>};
     if (s.tiny) return ln_bwd_wave<T, 4, 1, true>;
     switch (s.lanes) {
         case 4: return ln_bwd_wave_of<4>(s.v);
         case 8: return ln_bwd_wave_of<8>(s.v);
         case 16: return ln_bwd_wave_of<16>(s.v);
         case 32: return ln_bwd_wave_of<32>(s.v);
-        case 64: return s.v > 4 ? wide[s.v - 5] : ln_bwd_wave_of<64>(s.v);
-        case 0: return s.threads <= 512 ? block[s.v - 1] : s.v == 6 ? ln_bwd_block<768, 6> : ln_bwd_block<768, 7>;
+        case 64: return wave[s.v - 1];
+        case 0:
+            if (s.threads > 512) return s.v == 6 ? ln_bwd_block<768, 6> : ln_bwd_block<768, 7>;
+            return s.v <= 4 ? ahead[s.v - 2] : block[s.v - 6];
     }
     return ln_bwd_rows;
 }

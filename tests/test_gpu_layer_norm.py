@@ -70,6 +70,11 @@ SIZES = [(1, 1), (1, 4), (5, 1), (3, 2), (7, 3), (1, 256), (128, 256), (2, 15), 
          (1, 32768), (2, 32769), (1, 40004), (1, 70001), (3, 100000), (1000, 8), (2000, 5), (1500, 64), (1030, 100), (700, 1024),
          # on both sides of the rows that the backward pass takes in one launch, every width above it
          (512, 256), (513, 256), (513, 1), (600, 3), (530, 15), (777, 33), (640, 60), (520, 129), (530, 513), (521, 1023), (514, 1025),
+         # every width of a row, one launch and two
+         (2, 30), (2, 40), (600, 40), (3, 90), (600, 90), (4, 190), (600, 190), (3, 380), (520, 380), (520, 700), (520, 1250), (2, 1500),
+         (2, 1700), (2, 1900), (520, 1900), (2, 2300), (260, 2300), (2, 2500), (260, 2500), (2, 5000), (260, 6100), (2, 9000), (260, 9000),
+         (2, 12000), (260, 12000), (2, 15000), (260, 15000), (2, 17000), (260, 18000), (2, 19000), (2, 21504), (260, 21500), (2, 25000),
+         (2, 30000), (2, 23040), (600, 500), (600, 30), (600, 1500),
          (600, 1537), (513, 2048), (256, 2052), (257, 2052), (300, 4100), (258, 8193), (270, 16385), (257, 20000)]
 
 
