@@ -979,7 +979,8 @@ class Optimizer_Adam:
         return self._state
 
     def recorded_settings(self, layers):
-        """What a recorded update holds besides its tensors: with other values it has to be recorded anew."""
+        """What a recorded update holds besides its tensors: with other values it has to be recorded anew, after a normal
+        step with them."""
         return self._base_rate(), self.decay, self.epsilon
 
     def _base_rate(self):
@@ -1054,6 +1055,8 @@ class Optimizer_Muon:
     @staticmethod
     def takes(layer):
         """Whether the layer's weights are updated as a matrix."""
+        if layer.weights is None:                            # (a norm layer that has seen no input yet)
+            return False
         shape = layer.weights.shape
         wanted = getattr(layer, "muon", None)
         if wanted is None:
@@ -1081,7 +1084,7 @@ class Optimizer_Muon:
             self._flush()
 
     def has_state(self, layer):
-        if layer.weights is None or not self.takes(layer):
+        if not self.takes(layer):
             return self.adam.has_state(layer)
         return hasattr(layer, "muon_momentums") and hasattr(layer, "bias_cache")
 

@@ -235,22 +235,21 @@ class Model:
         recs = self.__dict__.setdefault("_recordings", {})
         rec = recs.get(key)
         lib = _lib.lib()
-        if rec is None or not all(self.optimizer.has_state(l) for l in self.trainable_layers):
-            # first step of this shape, or no optimizer state yet: a normal one (lazy initialisations,
-            # workspace sizes)
+        settings = self.optimizer.recorded_settings(self.trainable_layers)
+        if (rec is None or rec["optimizer"] is not self.optimizer or rec["settings"] != settings
+                or not all(self.optimizer.has_state(l) for l in self.trainable_layers)):
+            # first step of this shape, another optimizer or other settings of it, or no optimizer state yet: a normal
+            # one (lazy initialisations, workspace sizes)
             if rec is not None and rec["graph"] is not None:
                 _lib.check(lib.aeth_graph_destroy(rec["graph"]))
-            recs[key] = {"graph": None}
+            recs[key] = {"graph": None, "optimizer": self.optimizer, "settings": settings}
             return None
-        # a recording holds the optimizer's update and reads and writes the parameter buffers it was made with:
-        # another optimizer or other settings of it, or parameters set anew since then (set_parameters, load_parameters),
-        # make it stale
+        # a recording reads and writes the parameter buffers it was made with: parameters set anew since then
+        # (set_parameters, load_parameters) make it stale
         params = [(id(l), l.weights.ptr, l.biases.ptr) for l in self.trainable_layers]
-        settings = self.optimizer.recorded_settings(self.trainable_layers)
-        if rec["graph"] is not None and (rec.get("params") != params or rec.get("optimizer") is not self.optimizer
-                                         or rec.get("settings") != settings):
+        if rec["graph"] is not None and rec.get("params") != params:
             _lib.check(lib.aeth_graph_destroy(rec["graph"]))
-            recs[key] = rec = {"graph": None}
+            recs[key] = rec = {"graph": None, "optimizer": self.optimizer, "settings": settings}
         if rec["graph"] is None:
             rec["x"] = DeviceTensor(batch_X.shape, np.float32)
             rec["labels"] = DeviceTensor(labels.shape, labels.dtype)
@@ -275,8 +274,6 @@ class Model:
             _lib.check(rc)
             rec["graph"] = handle
             rec["params"] = params
-            rec["optimizer"] = self.optimizer
-            rec["settings"] = settings
             # what the layers point at after this step (output, dinputs, dweights, ...):
             # replays fill the same buffers, so the attributes are put back after steps
             # that ran in between (an evaluation, a step of another shape)

@@ -7,6 +7,7 @@
 //
 // Every singular value s of X goes to p(s) = a s + b s^3 + c s^5; from s <= 1 (the norm bounds them) all stay below 1.21 and
 // those that are not tiny end in about [0.7, 1.2]: u's singular vectors with singular values near one.
+#include "muon_f32.h"
 #include "split_gemm.h"
 
 #include <math.h>
@@ -34,6 +35,12 @@ struct MuonTable {
     double* sums;                                        // [count][kMuonParts]
 };
 typedef const MuonTable __attribute__((address_space(4)))* muon_table_ptr;
+
+// Workgroups of muon_momentum for a matrix
+static int muon_parts(const MuonMatrix& t) {
+    const int64_t size = (int64_t)t.rows * t.cols;
+    return size > 4096 * (int64_t)kMuonParts ? kMuonParts : cdiv(size, 4096);
+}
 
 __device__ __forceinline__ double muon_block_sum(double v, double* red) {
 #pragma unroll
@@ -438,6 +445,127 @@ __global__ __launch_bounds__(64 * kWholeWaves) void muon_whole(const MuonTable t
     }
 }
 
+// ---- many steps: float32 products ------------------------------------------------------------------------------------
+struct MuonScaleTable {
+    int count;
+    MuonMatrix t[kMuonMax];
+    int parts[kMuonMax];                                 // workgroups of muon_momentum
+    int first[kMuonMax];                                 // first workgroup of muon_scale
+    float* x[kMuonMax];
+    double* sums;                                        // [count][kMuonParts]
+};
+static_assert(sizeof(MuonScaleTable) + 64 <= 4096 && sizeof(MuonTable) + 64 <= 4096, "a launch's arguments");
+
+// X = u / |u| times 2^60, rows <= cols (transposed otherwise), padding 0; a 32 x 32 block of X a workgroup.
+__global__ __launch_bounds__(256) void muon_scale(const MuonScaleTable tb, float mu, int nesterov) {
+    __shared__ double red[4];
+    __shared__ float block[32][33];
+    typedef const MuonScaleTable __attribute__((address_space(4)))* table_ptr;
+    const table_ptr args = (table_ptr)__builtin_amdgcn_kernarg_segment_ptr();
+    int k = 0;
+    while (k + 1 < tb.count && (int)blockIdx.x >= args->first[k + 1]) ++k;
+    const float* __restrict__ grad = args->t[k].grad;
+    const float* __restrict__ mom = args->t[k].mom;
+    const int rows = args->t[k].rows, cols = args->t[k].cols;
+    const bool tall = rows > cols;
+    const MuonFloatLayout at = muon_float_layout(tall ? cols : rows, tall ? rows : cols, 0);
+    const int b = blockIdx.x - args->first[k], across = (int)(at.np / 32);
+    const int64_t i0 = (int64_t)(b / across) * 32, j0 = (int64_t)(b % across) * 32;         // of X
+    const int x = threadIdx.x & 31, y = threadIdx.x >> 5;
+    double part = 0.0;
+    for (int i = threadIdx.x; i < args->parts[k]; i += 256) part += args->sums[k * kMuonParts + i];
+    const double sum = muon_block_sum(part, red);
+    int power = 0;
+    const float factor = sum != 0.0 ? (float)frexp((double)kFloatScale / sqrt(sum), &power) : 0.f;
+    const int64_t r0 = tall ? j0 : i0, c0 = tall ? i0 : j0;                                  // of the matrix
+#pragma unroll
+    for (int v = y; v < 32; v += 8) {
+        float w = 0.f;
+        if (r0 + v < rows && c0 + x < cols) {
+            const int64_t e = (r0 + v) * cols + c0 + x;
+            w = mom != nullptr ? muon_update(grad[e], mom[e], mu, nesterov) : grad[e];
+            w = ldexpf(w, power) * factor;
+        }
+        block[v][x] = w;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int v = y; v < 32; v += 8) args->x[k][(i0 + v) * at.np + j0 + x] = tall ? block[x][v] : block[v][x];
+}
+
+// One launch for one product of every matrix.
+template <bool kRows, bool kApply>
+static int muon_float_product(FloatTable tb, float alpha, float beta, float lr, const double* state, float wd) {
+    int64_t tiles = 0;
+    for (int i = 0; i < tb.count; ++i) {
+        tb.p[i].first = (int)tiles;
+        tiles += (int64_t)(tb.p[i].M / 64) * (tb.p[i].N / 64);
+    }
+    hipLaunchKernelGGL((float_product<kRows, kApply>), dim3((unsigned)tiles), dim3(256), 0, ctx().stream, tb, alpha, beta, lr, state, wd);
+    AETH_LAUNCH_CHECK();
+    return AETH_OK;
+}
+
+static int muon_float_group(const MuonMatrix* t, int count, float lr, const double* state, float mu, int nesterov, float wd, int steps) {
+    MuonTable norm = {};
+    MuonScaleTable scale = {};
+    FloatTable gram = {}, poly = {}, step[2] = {};
+    MuonFloatLayout at[kMuonMax];
+    int64_t bytes = (int64_t)count * kMuonParts * sizeof(double), blocks = 0;
+    int parts = 1;
+    norm.count = scale.count = gram.count = poly.count = step[0].count = step[1].count = count;
+    for (int i = 0; i < count; ++i) {
+        const int m = t[i].rows < t[i].cols ? t[i].rows : t[i].cols, n = t[i].rows < t[i].cols ? t[i].cols : t[i].rows;
+        at[i] = muon_float_layout(m, n, bytes);
+        bytes = at[i].end;
+        norm.t[i] = scale.t[i] = t[i];
+        norm.parts[i] = scale.parts[i] = muon_parts(t[i]);
+        if (norm.parts[i] > parts) parts = norm.parts[i];
+        scale.first[i] = (int)blocks;
+        blocks += at[i].mp / 32 * (at[i].np / 32);
+    }
+    void* ws;
+    const int rc = workspace(bytes, &ws);
+    if (rc) return rc;
+    char* base = static_cast<char*>(ws);
+    norm.sums = scale.sums = static_cast<double*>(ws);
+    for (int i = 0; i < count; ++i) {
+        float *x[2] = {(float*)(base + at[i].x[0]), (float*)(base + at[i].x[1])}, *a = (float*)(base + at[i].a), *b = (float*)(base + at[i].b);
+        const int mp = (int)at[i].mp, np = (int)at[i].np;
+        scale.x[i] = x[0];
+        FloatProduct p = {};
+        p.rows = t[i].rows, p.cols = t[i].cols, p.theta = t[i].theta, p.out = t[i].out, p.gain = t[i].gain;
+        poly.p[i] = p;
+        poly.p[i].P = poly.p[i].Q = poly.p[i].R = a, poly.p[i].D = b, poly.p[i].M = poly.p[i].N = poly.p[i].K = mp;
+        for (int s = 0; s < 2; ++s) {
+            p.P = b, p.Q = p.R = x[s], p.D = x[1 - s], p.M = p.K = mp, p.N = np;
+            step[s].p[i] = p;
+        }
+    }
+    hipStream_t st = ctx().stream;
+    hipLaunchKernelGGL(muon_momentum, dim3(parts, count), dim3(256), 0, st, norm, mu, nesterov);
+    AETH_LAUNCH_CHECK();
+    hipLaunchKernelGGL(muon_scale, dim3((unsigned)blocks), dim3(256), 0, st, scale, mu, nesterov);
+    AETH_LAUNCH_CHECK();
+    const float unit = 1.f / kFloatScale;
+    gram.count = count;
+    for (int s = 0; s < steps; ++s) {
+        for (int i = 0; i < count; ++i) {
+            FloatProduct& p = gram.p[i];
+            p.P = p.Q = step[s & 1].p[i].Q, p.D = (float*)(base + at[i].a);
+            p.M = p.N = (int)at[i].mp, p.K = (int)at[i].np;
+        }
+        int e = muon_float_product<true, false>(gram, 0.f, unit, 0.f, nullptr, 0.f);
+        if (e == AETH_OK) e = muon_float_product<true, false>(poly, kNsB, kNsC * unit, 0.f, nullptr, 0.f);     // (A is symmetric)
+        if (e == AETH_OK)
+            e = s + 1 < steps ? muon_float_product<false, false>(step[s & 1], kNsA, unit, 0.f, nullptr, 0.f)
+                              : muon_float_product<false, true>(step[s & 1], kNsA, unit, lr, state, wd);
+        if (e) return e;
+    }
+    return AETH_OK;
+}
+
+// ---- the products on float16 halves ------------------------------------------------------------------------------------
 // One launch for one product of every matrix, in tiles of BM x BN.
 template <int BM, int BN, int WM, int WN, int NBUF, int BLOCK, int USE>
 static int muon_launch(SplitTable tb, float lr, const double* state, float wd) {
@@ -509,9 +637,8 @@ static int muon_group(const MuonMatrix* t, int count, float lr, const double* st
         const int m = t[i].rows < t[i].cols ? t[i].rows : t[i].cols, n = t[i].rows < t[i].cols ? t[i].cols : t[i].rows;
         at[i] = muon_layout(m, n, bytes);
         bytes = at[i].end;
-        const int64_t size = (int64_t)m * n;
         tb.t[i] = t[i];
-        tb.parts[i] = size > 4096 * (int64_t)kMuonParts ? kMuonParts : cdiv(size, 4096);
+        tb.parts[i] = muon_parts(t[i]);
         if (tb.parts[i] > parts) parts = tb.parts[i];
         tb.first[i] = (int)blocks;
         blocks += cdiv(at[i].mp / 32 * (at[i].np / 32), 4);
@@ -609,7 +736,34 @@ static int muon_small(const MuonMatrix* t, int count, int row_blocks, int blocks
 // Matrices whose buffers together pass this go out in several groups, one after the other.
 constexpr int64_t kMuonWorkspace = (int64_t)4 << 30;
 
+// The matrices that two halves do not carry through the steps, on float32 products.
+static int muon_float(const MuonMatrix* t, int count, float lr, const double* state, float mu, int nesterov, float wd, int steps) {
+    for (int i = 0; i < count;) {
+        int64_t bytes = 0;
+        int k = 0;
+        while (i + k < count) {
+            const MuonMatrix& x = t[i + k];
+            const int64_t more = muon_float_layout(std::min(x.rows, x.cols), std::max(x.rows, x.cols), 0).end;
+            if (k > 0 && bytes + more > kMuonWorkspace) break;
+            bytes += more;
+            ++k;
+        }
+        const int rc = muon_float_group(t + i, k, lr, state, mu, nesterov, wd, steps);
+        if (rc) return rc;
+        i += k;
+    }
+    return AETH_OK;
+}
+
 static int muon_run(MuonMatrix* t, int count, float lr, const double* state, float mu, int nesterov, float wd, int steps) {
+    const int halves = (int)(std::stable_partition(t, t + count, [&](const MuonMatrix& x) {
+                                 return muon_in_halves(std::max(x.rows, x.cols), steps);
+                             }) - t);
+    if (halves < count) {
+        const int rc = muon_float(t + halves, count - halves, lr, state, mu, nesterov, wd, steps);
+        if (rc) return rc;
+    }
+    count = halves;
     if (count == 0) return AETH_OK;
     int row_blocks;
     const int blocks = muon_whole_blocks(t, count, &row_blocks);

@@ -1,8 +1,8 @@
 // How a call's matrices are laid out and cut into tiles for the Newton-Schulz products.  Free of HIP calls, so that the host
 // can check it without a GPU.
 //
-// A matrix is held as two float16 halves (split_gemm.h) in slabs of 32 columns.  Rows and columns are padded to multiples of 32 with
-// zeros; zeros stay zeros through all products.
+// A matrix is held as two float16 halves (split_gemm.h) in slabs of 32 columns, or for many steps as float32 (muon_f32.h).  Rows and
+// columns are padded with zeros to multiples of 32, or 64; zeros stay zeros through all products.
 #pragma once
 
 #include <stdint.h>
@@ -20,6 +20,37 @@ constexpr int kMuonLongest = 1 << 21;                    // rows or columns: a 2
 constexpr int kMuonParts = 1024;                          // partial sums of a matrix's norm
 
 MUON_HD int64_t muon_pad(int64_t n) { return (n + 31) / 32 * 32; }
+
+// Whether two float16 halves carry a matrix of n columns (the longer side) through so many steps.  The halves end 2^-40 below |u|:
+// a row, a column or a block of the matrix that is much weaker than the rest is held with that error, which every step multiplies
+// by up to 3.4445 until the part has grown to full size.  An element's share of that is worth sqrt(n) in a row, so the result is off
+// by 2^-40 3.4445^steps sqrt(n) of its norm in the worst case (a part that reaches full size with the last step).  The limit is 2^-20,
+// what float32 products cost on the same matrices (64 x 96, 8 steps: 1.1e-6 against 2.3e-6; 64 x 2048: 2.2e-6 and 3.7e-6; above the
+// limit, 12 steps: 1.2e-5 and 7e-6; 8.8e-5 and 6.8e-6).  It allows 9 steps up to 236 columns, 8 up to 2800, 7 up to 33222, 5 up to 2^21.
+static inline bool muon_in_halves(int64_t n, int steps) {
+    double off = 1.0 / ((int64_t)1 << 40);               // squared: the square root is not needed
+    off = off * off * (double)n;
+    const double limit = 1.0 / ((int64_t)1 << 40);
+    for (int s = 0; s < steps && off <= limit; ++s) off *= 3.4445 * 3.4445;
+    return off <= limit;
+}
+
+// The buffers of a matrix held as float32 (byte offsets): X and the next X [mp][np], A and B [mp][mp].
+struct MuonFloatLayout {
+    int64_t mp, np;
+    int64_t x[2], a, b, end;
+};
+MUON_HD MuonFloatLayout muon_float_layout(int64_t m, int64_t n, int64_t begin) {
+    MuonFloatLayout l;
+    l.mp = (m + 63) / 64 * 64;
+    l.np = (n + 63) / 64 * 64;
+    l.x[0] = begin;
+    l.x[1] = l.x[0] + 4 * l.mp * l.np;
+    l.a = l.x[1] + 4 * l.mp * l.np;
+    l.b = l.a + 4 * l.mp * l.mp;
+    l.end = l.b + 4 * l.mp * l.mp;
+    return l;
+}
 
 // Byte offsets of one matrix's buffers in the workspace (m x n with m <= n; X is [m][n], Xt its transpose).
 struct MuonLayout {

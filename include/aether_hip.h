@@ -339,8 +339,12 @@ int aeth_adam_multi_dev_f32(int count, float* const* host_theta, const float* co
  * aeth_newton_schulz_f32 is its orthogonalisation alone: o = X after `steps` (1..100) rounds of
  *     X = g / |g| (Frobenius);  X <- a X + (b A + c A^2) X,  A = X X^T   (a, b, c) = (3.4445, -4.7750, 2.0315),
  * which takes every singular value s of g / |g| to p(...p(s)), p(s) = a s + b s^3 + c s^5, and keeps the singular vectors.
- * Any positive multiple of g gives the same o (there is no epsilon); g = 0 gives 0; a NaN or an infinity makes all of o NaN.
- * g and o are [rows, cols], sides of at most 2^21, and may not overlap; products and sums hold 22 bits or more of every factor.
+ * Any positive multiple of g gives the same o up to roundings (a power of two the same bits, as long as no element becomes
+ * subnormal; there is no epsilon); g = 0 gives 0; a NaN or an infinity makes all of o NaN.  g and o are [rows, cols], sides of at
+ * most 2^21, and may not overlap.  Precision, sums being float32: while 3.4445^steps sqrt(longer side) <= 2^20 (5 steps at any
+ * size, 7 up to 33222, 8 up to 2800, 9 up to 236) the factors of a product hold 22 bits of an element, or 2^-40 of |g| (A, B: of 1)
+ * where that is more: rows far below the rest come out with that error of their own.  With more steps, which bring such rows to
+ * full size, products are float32 and much slower.
  * aeth_muon_multi_f32 updates `count` (1..32) matrices in one call:
  *     m <- momentum m + grad;  u = grad + momentum m (nesterov != 0) or m;  O = newton_schulz(u);
  *     theta <- theta (1 - lr weight_decay) - lr sqrt(max(1, cols / rows)) O.

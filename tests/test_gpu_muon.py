@@ -470,3 +470,110 @@ def test_parameter_files_with_a_layer_norm(tmp_path):
     other.load_parameters(path)
     assert all(np.array_equal(a, b) for a, b in zip(_host(model), _host(other)))
     assert np.array_equal(model.predict(x), other.predict(x))
+
+
+# ---- many steps ------------------------------------------------------------------------------------------------------
+def _weak(r, c, scale, kind, seed=0):
+    """A matrix of which a part is `scale` below the rest."""
+    g = np.random.RandomState(seed + r + 3 * c).randn(r, c)
+    if kind == "block":
+        g[:r // 2, c // 2:] = 0
+        g[r // 2:, :c // 2] = 0
+        g[r // 2:] *= scale
+    elif kind == "rows":
+        g[r // 2:] *= scale
+    elif kind == "columns":
+        g[:, c // 2:] *= scale
+    else:
+        g *= np.logspace(0, np.log10(scale), r)[:, None]
+    return g.astype(np.float32)
+
+
+# on both sides of the steps that the halves carry (9 up to 236 columns, 8 up to 2800, 7 beyond), with one workgroup and with many
+@pytest.mark.parametrize("r,c,steps", [(64, 96, 5), (64, 96, 9), (64, 96, 10), (64, 96, 12), (96, 64, 16), (64, 96, 25), (64, 96, 100),
+                                       (150, 90, 9), (150, 90, 14), (90, 150, 20), (64, 700, 8), (700, 64, 9), (40, 2900, 7),
+                                       (40, 2900, 8), (2900, 40, 14), (300, 260, 8), (300, 260, 20), (2, 3, 30)])
+def test_steps_on_matrices_with_weak_parts(r, c, steps):
+    """Every step brings a weak part nearer to full size: what was lost of it shows in the end."""
+    for kind in ("block", "rows", "columns", "graded"):
+        for scale in (1e-4, 1e-8, 1e-9, 1e-10, 1e-12, 1e-20, 1e-30):
+            g = _weak(r, c, scale, kind)
+            tol, exact = R.tolerance(g, steps)
+            off = np.linalg.norm(_ortho(g, steps) - exact)
+            assert off <= tol, (kind, scale, off / np.linalg.norm(exact), tol / np.linalg.norm(exact))
+
+
+@pytest.mark.parametrize("r,c,steps", [(64, 96, 12), (96, 64, 20), (300, 260, 30), (40, 2900, 14), (64, 128, 100)])
+def test_weak_rows_alone_after_many_steps(r, c, steps):
+    """Row by row (of the shorter side): a float32 sum of products with a weak row is as exact for the row as for a strong one, so
+    the worst row is off by what the worst row of a float32 evaluation is, and a factor of 8 for the other order of the sums."""
+    for kind in ("block", "rows", "graded"):
+        for scale in (1e-6, 1e-9, 1e-12):
+            g = _weak(min(r, c), max(r, c), scale, kind, seed=1)
+            exact, simple = R.newton_schulz(g, steps), R.newton_schulz(g, steps, np.float32)
+            size = np.linalg.norm(exact, axis=1)
+            worst = np.max(np.linalg.norm(simple - exact, axis=1) / size)
+            o = _ortho(g, steps) if r <= c else _ortho(np.ascontiguousarray(g.T), steps).T
+            off = np.max(np.linalg.norm(o - exact, axis=1) / size)
+            assert off <= 8 * worst + 2.0 ** -17, (kind, scale, off, worst)
+
+
+@pytest.mark.parametrize("steps", [9, 30])
+def test_update_of_matrices_on_both_kinds_of_products(steps):
+    """One call whose matrices need float32 products, or not, by their sizes."""
+    shapes = [(20, 30), (5, 3000), (300, 500), (2000, 33), (64, 64), (1, 1), (129, 70), (230, 236), (230, 237)]
+    tensors = [_triple(r, c, seed=10 * i) for i, (r, c) in enumerate(shapes)]
+    got = _multi(tensors, steps=steps)
+    for t, g in zip(tensors, got):
+        want, m, bound = R.update(*t, 0.02, 0.95, 1, 0.01, steps)
+        assert np.all(np.abs(g[1] - m) <= R.momentum_bound(t[1], t[2], 0.95))
+        assert np.linalg.norm(g[0] - want) <= bound
+    assert all(np.array_equal(p[0], q[0]) and np.array_equal(p[1], q[1]) for p, q in zip(got, _multi(tensors, steps=steps)))
+
+
+@pytest.mark.parametrize("r,c", [(4, 6), (150, 90), (1, 500)])
+def test_values_at_the_edge_with_many_steps(r, c):
+    assert np.all(_ortho(np.zeros((r, c), np.float32), 20) == 0)
+    for bad in (np.nan, np.inf):
+        g = _gradient(r, c, seed=4)
+        g[r - 1, 1] = bad
+        assert np.all(np.isnan(_ortho(g, 20)))
+    g = _gradient(r, c, seed=2)
+    o = _ortho(g, 20)
+    for k in (-60, 90):
+        assert np.array_equal(_ortho(g * np.float32(2.0) ** k, 20), o)
+    if min(r, c) > 1:
+        g[r // 2] = 0
+        o = _ortho(g, 20)
+        _check(g, 20, o)
+        assert np.all(o[r // 2] == 0)
+
+
+def test_many_steps_of_a_long_row():
+    """2^21 columns: the norm of a single row goes to p(p(...p(1))), every element its part of it."""
+    g = np.tile(_gradient(1, 4096, seed=7), (1, 512))
+    exact = R.newton_schulz(g, 6)
+    # a sum of squares in float32, 2^9 pairs in line and 2^11 totals: off by at most e = (2^9 + 2^11) 2^-24 of itself.  A step's result
+    # moves by |b A + 2 c A^2| s e, at most 1.1 e on [0.68, 1.2], and the slope of p along this orbit (1, 0.70, 1.11, 0.70, ...) is at
+    # most 1.5 over two steps, 3.4 over six: at most 6 * 1.1 * 3.4 = 22 e
+    assert np.linalg.norm(_ortho(g, 6) - exact) <= 22 * (2 ** 9 + 2 ** 11) * 2.0 ** -24 * np.linalg.norm(exact)
+
+
+def test_more_steps_in_the_middle_of_recorded_training():
+    """The float32 products need a workspace of their own, which has to be there before a step is recorded with them."""
+    import aether
+    steps = _batches(9)
+    runs = []
+    for record in (False, True):
+        model = _network(aether.Optimizer_Muon(), norm=False)
+        model.record_steps(record)
+        for k, (x, y) in enumerate(steps):
+            if k == 3:
+                model.train_step(x[:6], y[:6])               # (a second shape, recorded only after the change)
+                model.optimizer.ns_steps = 30
+            model.train_step(x, y)
+            if k == 5:
+                model.train_step(x[:6], y[:6])
+        runs.append(_host(model))
+        model.record_steps(False)
+    assert all(np.array_equal(a, b) for a, b in zip(*runs))

@@ -138,3 +138,35 @@ def test_tiles_runs_and_buffers_cover_every_product(tmp_path):
     r = subprocess.run([exe], capture_output=True, text=True)
     assert r.returncode == 0, r.stdout + r.stderr
     assert [line.split()[1] for line in r.stdout.splitlines()] == ["triangles", "choices", "layouts"]
+
+
+def test_the_limit_of_the_halves(tmp_path):
+    """aether-ml_amd/csrc/muon_plan.h: which matrices go through the steps as two float16 halves."""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    exe = str(tmp_path / "muon_halves_check")
+    subprocess.run(["g++", "-std=c++17", "-O2", "-Wall", "-Werror", "-I", os.path.join(root, "aether-ml_amd", "csrc"),
+                    os.path.join(root, "tests", "cpu", "muon_halves_check.cpp"), "-o", exe], check=True)
+    r = subprocess.run([exe], capture_output=True, text=True)
+    assert r.returncode == 0 and r.stdout == "ok halves\n", r.stdout + r.stderr
+
+
+@pytest.mark.parametrize("steps,scale", [(16, 1e-9), (25, 1e-12)])
+def test_the_tolerance_refuses_halves_beyond_their_limit(steps, scale):
+    """Two float16 halves under one power of two, for more steps than they carry (planted in the reference's own arithmetic)."""
+    rng = np.random.RandomState(steps)
+    g = rng.randn(64, 96)
+    g[:32, 48:] = 0
+    g[32:, :48] = 0
+    g[32:] *= scale
+    tol, exact = R.tolerance(g.astype(np.float32), steps)
+
+    def halves(x, s):
+        y = (x * s).astype(np.float32)
+        hi = y.astype(np.float16)
+        return (hi.astype(np.float64) + (y - hi).astype(np.float16)) / s
+
+    x = halves(g / np.linalg.norm(g), 32768.0)
+    for _ in range(steps):
+        a = halves(x @ x.T, 32768.0)
+        x = halves(halves(R.COEF[0] * np.eye(64) + R.COEF[1] * a + R.COEF[2] * a @ a, 16384.0) @ x, 32768.0)
+    assert np.linalg.norm(x - exact) > tol
