@@ -7,7 +7,8 @@
 //   dx = invstd_r (g - sum_c g / C - xhat sum_c g xhat / C)
 //   dgamma_c = sum_r dy xhat,  dbeta_c = sum_r dy
 //
-// All sums are float32 in a fixed order: results do not depend on timing.
+// All sums are in a fixed order: results do not depend on timing.  They are float32 where no lane adds more than a few dozen numbers in
+// line (a row in registers); a row of any length is summed in 64 bits.
 #include "common.h"
 
 namespace aeth {
@@ -120,6 +121,40 @@ struct LnTeam {
     }
 };
 
+// A thread's columns of a row of any length, every kLnLong'th: f(column, terms) of four columns by pairs in float32, the rest in 64 bits.
+template <int N, typename F>
+__device__ __forceinline__ void ln_long_sum(int C, double* s, F f) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) s[i] = 0.0;
+    int64_t c = threadIdx.x;
+    for (; c + 3 * kLnLong < C; c += 4 * kLnLong) {
+        float v[4][N];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) f(c + k * kLnLong, v[k]);
+#pragma unroll
+        for (int i = 0; i < N; ++i) s[i] += (double)((v[0][i] + v[1][i]) + (v[2][i] + v[3][i]));
+    }
+    for (; c < C; c += kLnLong) {
+        float v[N];
+        f(c, v);
+#pragma unroll
+        for (int i = 0; i < N; ++i) s[i] += (double)v[i];
+    }
+}
+
+// Sums over the workgroup in 64 bits, one at a time; red: one slot, so there is a barrier in front of it.
+__device__ __forceinline__ double ln_block_sum(double v, double* red) {
+    const int waves = blockDim.x >> 6;
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+    __syncthreads();                                     // (the last sum has been read)
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = red[0];
+    for (int w = 1; w < waves; ++w) v += red[w];
+    return v;
+}
+
 // ---- forward -----------------------------------------------------------------------------------------------------------
 // Bound: HBM, 8 bytes an element (10 with the bfloat16 copy): 16384 x 8192 201 us = 5.3 TB/s, the rate of a copy; rows that no
 // power of two divides 4.2-5.2 TB/s.  A row is read once and stays in registers: the mean, then the sum of
@@ -223,24 +258,18 @@ __global__ __launch_bounds__(T) void ln_fwd_block(const LnFwdArgs p) {
     }
 }
 
-// Rows of any length: three passes over the row.
+// Rows of any length: three passes over the row.  The sums are 64-bit (float32, a thread adding its columns in line, gave a row of 2^20
+// times 1000.3 the mean 1000.3087).
 __global__ __launch_bounds__(kLnLong) void ln_fwd_rows(const LnFwdArgs p) {
-    __shared__ float red[2][2][16];
-    LnTeam team(red);
+    __shared__ double red[kLnLong / 64];
     const int C = p.C;
     for (int64_t r = blockIdx.x; r < p.rows; r += gridDim.x) {
         const float* xr = p.x + (size_t)r * C;
-        float s = 0.f;
-        for (int64_t c = threadIdx.x; c < C; c += kLnLong) s += xr[c];
-        team.sum<1>(&s);
-        const float mean = s * p.inv_c;
-        float q = 0.f;
-        for (int64_t c = threadIdx.x; c < C; c += kLnLong) {
-            const float d = xr[c] - mean;
-            q += d * d;
-        }
-        team.sum<1>(&q);
-        const float invstd = 1.0f / sqrtf(q * p.inv_c + p.eps);
+        double s[1], q[1];
+        ln_long_sum<1>(C, s, [&](int64_t c, float* v) { v[0] = xr[c]; });
+        const float mean = (float)(ln_block_sum(s[0], red) / C);
+        ln_long_sum<1>(C, q, [&](int64_t c, float* v) { v[0] = (xr[c] - mean) * (xr[c] - mean); });
+        const float invstd = 1.0f / sqrtf((float)(ln_block_sum(q[0], red) / C) + p.eps);
         if (threadIdx.x == 0 && p.mean != nullptr) {
             p.mean[r] = mean;
             p.invstd[r] = invstd;
@@ -448,22 +477,19 @@ __global__ __launch_bounds__(T) void ln_bwd_block(const LnBwdArgs p) {
     }
 }
 
-// Rows of any length: the gradient of the rows in two passes over each, the column sums in a kernel of their own.
+// Rows of any length: the gradient of the rows in two passes over each (sums in 64 bits), the column sums in a kernel of their own.
 __global__ __launch_bounds__(kLnLong) void ln_bwd_rows(const LnBwdArgs p) {
-    __shared__ float red[2][2][16];
-    LnTeam team(red);
+    __shared__ double red[kLnLong / 64];
     const int C = p.C;
     for (int64_t r = blockIdx.x; r < p.rows; r += gridDim.x) {
         const size_t at = (size_t)r * C;
         const float m = p.mean[r], is = p.invstd[r];
-        float s[2] = {0.f, 0.f};
-        for (int64_t c = threadIdx.x; c < C; c += kLnLong) {
-            const float g = p.dy[at + c] * p.gamma[c];
-            s[0] += g;
-            s[1] += g * ((p.x[at + c] - m) * is);
-        }
-        team.sum<2>(s);
-        const float c1 = s[0] * p.inv_c, c2 = s[1] * p.inv_c;
+        double s[2];
+        ln_long_sum<2>(C, s, [&](int64_t c, float* v) {
+            v[0] = p.dy[at + c] * p.gamma[c];
+            v[1] = v[0] * ((p.x[at + c] - m) * is);
+        });
+        const float c1 = (float)(ln_block_sum(s[0], red) / C), c2 = (float)(ln_block_sum(s[1], red) / C);
         for (int64_t c = threadIdx.x; c < C; c += kLnLong) {
             const float v = is * (p.dy[at + c] * p.gamma[c] - c1 - (p.x[at + c] - m) * is * c2);
             p.dx[at + c] = v;

@@ -335,3 +335,65 @@ def test_recorded_and_replayed(rows):
         other.forward(r.randn(900 * (k + 1), 700).astype(np.float32), True)
         other.backward(r.randn(900 * (k + 1), 700).astype(np.float32))
     check(lib.aeth_graph_destroy(graph))
+
+
+# ---- long sums -------------------------------------------------------------------------------------------------------
+U = R.U
+
+
+@pytest.mark.parametrize("c", [32769, 200704, (1 << 20) + 37, 1 << 22])
+def test_long_constant_rows_give_beta(c):
+    """A sum of equal numbers in 64 bits is exact (24 bits times fewer than 2^29 of them), and so is its mean: what is left is 0."""
+    beta = np.random.RandomState(c).randn(c).astype(np.float32)
+    x = np.empty((3, c), np.float32)
+    x[0], x[1], x[2] = 1000.3, -0.1, 3e7
+    y, mean, inv, _ = _forward(x, np.ones(c, np.float32), beta)
+    assert np.array_equal(mean, x[:, 0])
+    assert all(np.array_equal(row, beta) for row in y)
+
+
+def _long_forward(x, gamma, beta, eps):
+    """R.forward with the bounds of sums in 64 bits: four terms by pairs in float32 (two roundings), the result (one); a square has
+    one more."""
+    (y, mean, inv), _ = R.forward(x, gamma, beta, eps)
+    d = x.astype(np.float64) - mean[:, None]
+    var = (d * d).mean(-1)
+    e_mean = 3 * U * np.abs(x.astype(np.float64)).mean(-1)
+    e_d = e_mean[:, None] + U * np.abs(d)
+    e_var = 6 * U * var + e_mean ** 2 + 2 * U * float(np.float32(eps))
+    e_inv = inv * (0.5 * e_var * inv ** 2 + 3 * U)
+    xhat = d * inv[:, None]
+    e_y = np.abs(gamma) * (e_d * inv[:, None] + np.abs(d) * e_inv[:, None] + 2 * U * np.abs(xhat)) + U * (np.abs(y) + np.abs(xhat * gamma))
+    return (y, mean, inv), (e_y, e_mean, e_inv)
+
+
+def _long_backward(x, dy, gamma, mean, invstd):
+    """The same of R.backward."""
+    want, (_, e_dgamma, e_dbeta) = R.backward(x, dy, gamma, mean, invstd)
+    x, dy, gamma = (np.asarray(a, np.float64) for a in (x, dy, gamma))
+    invstd = invstd.astype(np.float64)[:, None]
+    xhat = (x - mean.astype(np.float64)[:, None]) * invstd
+    g = dy * gamma
+    mean_of = lambda a: a.mean(-1, keepdims=True)  # noqa: E731
+    c1, c2 = mean_of(g), mean_of(g * xhat)
+    e_c1 = 4 * U * mean_of(np.abs(g))                                    # the product, two sums, the result
+    e_c2 = 7 * U * mean_of(np.abs(g * xhat))                             # xhat 2, g 1, the product 1, two sums, the result
+    size = np.abs(g) + np.abs(c1) + np.abs(xhat * c2)
+    e_dx = invstd * (e_c1 + np.abs(xhat) * e_c2 + 2 * U * np.abs(c2 * xhat) + 5 * U * size)
+    return want, (e_dx, e_dgamma, e_dbeta)
+
+
+@pytest.mark.parametrize("rows,c", [(3, 32769), (30, 23000), (3, 200704), (2, (1 << 20) + 37), (1, 1 << 24)])
+def test_long_rows_of_like_numbers(rows, c):
+    """Numbers far from zero and of one sign, whose sums grow with every term: the bounds are those of 64-bit sums."""
+    r = np.random.RandomState(rows + c)
+    x = (300 + 200 * r.rand(rows, c)).astype(np.float32)
+    dy = (1 + 0.1 * r.randn(rows, c)).astype(np.float32)
+    gamma, beta = (1 + 0.1 * r.randn(c)).astype(np.float32), r.randn(c).astype(np.float32)
+    got = _forward(x, gamma, beta)
+    if c > 32768:
+        for g, w, b in zip(got, *_long_forward(x, gamma, beta, 1e-5)):
+            assert R.worst(g, w, b) <= 1
+    back = _backward(x, dy, gamma, got[1], got[2])
+    for g, w, b, name in zip(back, *_long_backward(x, dy, gamma, got[1], got[2]), ("dx", "dgamma", "dbeta")):
+        assert R.worst(g, w, b) <= 1, name
