@@ -8,12 +8,16 @@
 //   dgamma_c = sum_r dy xhat,  dbeta_c = sum_r dy
 //
 // All sums are in a fixed order: results do not depend on timing.  They are float32 where no lane adds more than a few dozen numbers in
-// line (a row in registers); a row of any length is summed in 64 bits.
+// line (a row in registers), and a few hundred over the rows (kLnRun); a row of any length is summed in 64 bits.
 #include "common.h"
 
 namespace aeth {
 
 constexpr int kLnLong = 1024;                            // threads of the kernels for rows of any length
+
+// Rows that a lane adds in line to its columns' sums, at most: a float32 sum of n like terms in line is off by up to n 2^-24 of itself
+// (0.1 added 65536 times: 6e-4 of the sum).
+constexpr int kLnRun = 256;
 
 // Outputs of this size and more are stored with the non-temporal hint: the next kernel will not find them in a cache anyway.
 constexpr int64_t kLnStreamBytes = 64 << 20;
@@ -286,7 +290,8 @@ __global__ __launch_bounds__(kLnLong) void ln_fwd_rows(const LnFwdArgs p) {
 // Bound: HBM, 12 bytes an element (14 with the bfloat16 copy): 65536 x 1024 152 us = 5.3 TB/s, 802816 x 64 115 us = 5.4 TB/s, ragged
 // rows 4.6-5.2 TB/s; a short call (5003 x 1537, 92 MB, 22 us) pays for two launches.  x and dy are read once: the same lanes hold the row
 // while its two sums are taken, and the lane that owns a column adds its dy xhat and dy over all rows it sees.  A workgroup walks many
-// rows and leaves one partial row of dgamma and one of dbeta, part[block][2][C]; ln_bwd_finish adds those in block order.
+// rows and leaves a partial row of dgamma and one of dbeta for every kLnRun rows of a lane, part[piece][block][2][C]; ln_bwd_finish adds
+// those in order.
 // Few rows: one launch (part == NULL), in which workgroups of their own read the columns a second time and write dgamma and dbeta.
 struct LnBwdArgs {
     const float *x, *dy, *gamma, *mean, *invstd;
@@ -297,6 +302,7 @@ struct LnBwdArgs {
     float* part;
     bool stream;
     int groups;                                          // workgroups of rows; those behind them have 32 columns each
+    int pieces;                                          // partial rows a workgroup leaves, one for every kLnRun rows a lane
     float *dgamma, *dbeta;
 };
 
@@ -400,40 +406,45 @@ __global__ __launch_bounds__(T) void ln_bwd_wave(const LnBwdArgs p) {
     int64_t r = (int64_t)blockIdx.x * (T / L) + threadIdx.x / L;
     LnBwdRow<V> next;
     if (kAhead && r < p.rows) next.load(p, r, u);
-    while (r < p.rows) {
-        LnBwdRow<V> w;
-        if (kAhead) w = next;
-        else w.load(p, r, u);
-        const int64_t now = r;
-        r += step;
-        if (kAhead) next.load(p, r < p.rows ? r : now, u);
-        ln_bwd_row(p, now, u, w, gm, dg, db, [](float* a) {
-            a[0] = ln_group_sum<L>(a[0]);
-            a[1] = ln_group_sum<L>(a[1]);
-        });
-    }
-    if (p.part == nullptr) return;
-    // the rows of a wave, then the waves in order
-    float* out = p.part + (size_t)blockIdx.x * 2 * C;
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-#pragma unroll
-        for (int j = 0; j < V; ++j)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                float v = k == 0 ? dg[j][e] : db[j][e];
-#pragma unroll
-                for (int o = L; o < 64; o <<= 1) v += __shfl_xor(v, o, 64);
-                if ((threadIdx.x & 63) < L && u.own(j, e)) red[threadIdx.x >> 6][u.at(j) + e] = v;
-            }
-        __syncthreads();
-        for (int c = threadIdx.x; c < C; c += T) {
-            float v = red[0][c];
-#pragma unroll
-            for (int w = 1; w < T / 64; ++w) v += red[w][c];
-            out[(size_t)k * C + c] = v;
+    for (int piece = 0; piece < p.pieces; ++piece) {
+        const int64_t end = min((int64_t)p.rows, (int64_t)(piece + 1) * kLnRun * step);
+        while (r < end) {
+            LnBwdRow<V> w;
+            if (kAhead) w = next;
+            else w.load(p, r, u);
+            const int64_t now = r;
+            r += step;
+            if (kAhead) next.load(p, r < p.rows ? r : now, u);
+            ln_bwd_row(p, now, u, w, gm, dg, db, [](float* a) {
+                a[0] = ln_group_sum<L>(a[0]);
+                a[1] = ln_group_sum<L>(a[1]);
+            });
         }
-        __syncthreads();
+        if (p.part == nullptr) return;
+        // the rows of a wave, then the waves in order
+        float* out = p.part + ((size_t)piece * p.groups + blockIdx.x) * 2 * C;
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+#pragma unroll
+            for (int j = 0; j < V; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    float& sum = k == 0 ? dg[j][e] : db[j][e];
+                    float v = sum;
+                    sum = 0.f;
+#pragma unroll
+                    for (int o = L; o < 64; o <<= 1) v += __shfl_xor(v, o, 64);
+                    if ((threadIdx.x & 63) < L && u.own(j, e)) red[threadIdx.x >> 6][u.at(j) + e] = v;
+                }
+            __syncthreads();
+            for (int c = threadIdx.x; c < C; c += T) {
+                float v = red[0][c];
+#pragma unroll
+                for (int w = 1; w < T / 64; ++w) v += red[w][c];
+                out[(size_t)k * C + c] = v;
+            }
+            __syncthreads();
+        }
     }
 }
 
@@ -455,25 +466,30 @@ __global__ __launch_bounds__(T) void ln_bwd_block(const LnBwdArgs p) {
     int64_t r = blockIdx.x;
     LnBwdRow<V> next;
     if (kAhead && r < p.rows) next.load(p, r, u);
-    while (r < p.rows) {
-        LnBwdRow<V> w;
-        if (kAhead) {
-            w = next;
-        } else {
-            w.load(p, r, u);
-            ln_gains(p, u, gm);
+    for (int piece = 0; piece < p.pieces; ++piece) {
+        const int64_t end = min((int64_t)p.rows, (int64_t)(piece + 1) * kLnRun * p.groups);
+        while (r < end) {
+            LnBwdRow<V> w;
+            if (kAhead) {
+                w = next;
+            } else {
+                w.load(p, r, u);
+                ln_gains(p, u, gm);
+            }
+            const int64_t now = r;
+            r += p.groups;
+            if (kAhead) next.load(p, r < p.rows ? r : now, u);
+            ln_bwd_row(p, now, u, w, gm, dg, db, [&](float* a) { team.sum<2>(a); });
         }
-        const int64_t now = r;
-        r += p.groups;
-        if (kAhead) next.load(p, r < p.rows ? r : now, u);
-        ln_bwd_row(p, now, u, w, gm, dg, db, [&](float* a) { team.sum<2>(a); });
-    }
-    if (p.part == nullptr) return;
-    float* out = p.part + (size_t)blockIdx.x * 2 * C;
+        if (p.part == nullptr) return;
+        float* out = p.part + ((size_t)piece * p.groups + blockIdx.x) * 2 * C;
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-        u.store(out, j, dg[j], false);
-        u.store(out + C, j, db[j], false);
+        for (int j = 0; j < V; ++j) {
+            u.store(out, j, dg[j], false);
+            u.store(out + C, j, db[j], false);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) dg[j][e] = db[j][e] = 0.f;
+        }
     }
 }
 
@@ -736,23 +752,24 @@ static int ln_bwd_impl(const float* x, const float* dy, const float* gamma, cons
         // One launch for few rows: 128 x 256 3.1 us instead of 5.6, 512 x 256 4.1 and 5.6, 512 x 2048 5.4 and 9.3, 128 x 8192 6.0 and 12.4,
         // 256 x 20000 27 and 36; but a column's rows are one workgroup's: 1024 x 256 6.3 and 5.8, 512 x 8192 18 and 17
         if (s.lanes >= 0 && rows <= (s.lanes > 0 ? 512 : 256)) {
-            const LnBwdArgs p{x, dy, gamma, mean, invstd, dx, dx16, rows, C, 1.0f / (float)C, nullptr, 4 * n >= kLnStreamBytes, turns, dgamma,
+            const LnBwdArgs p{x, dy, gamma, mean, invstd, dx, dx16, rows, C, 1.0f / (float)C, nullptr, 4 * n >= kLnStreamBytes, turns, 1, dgamma,
                               dbeta};
             hipLaunchKernelGGL(ln_bwd_kernel(s), dim3(turns + cdiv(C, 32)), dim3(threads), 0, st, p);
             AETH_LAUNCH_CHECK();
             return AETH_OK;
         }
         // as many workgroups as are needed for each to take no more rows than with `cap` of them
-        const int run = cdiv(turns, cap);
-        blocks = cdiv(turns, run);
+        const int run = cdiv(turns, cap), groups = cdiv(turns, run), pieces = s.lanes < 0 ? 1 : cdiv(run, kLnRun);
+        blocks = groups * pieces;
         const int rc = workspace((int64_t)2 * blocks * C * sizeof(float), &ws);
         if (rc) return rc;
-        const LnBwdArgs p{x, dy, gamma, mean, invstd, dx, dx16, rows, C, 1.0f / (float)C, (float*)ws, 4 * n >= kLnStreamBytes, blocks, nullptr, nullptr};
-        hipLaunchKernelGGL(ln_bwd_kernel(s), dim3(s.lanes < 0 ? (rows < 4096 ? rows : 4096) : blocks), dim3(threads), 0, st, p);
+        const LnBwdArgs p{x, dy, gamma, mean, invstd, dx, dx16, rows, C, 1.0f / (float)C, (float*)ws, 4 * n >= kLnStreamBytes, groups, pieces,
+                          nullptr, nullptr};
+        hipLaunchKernelGGL(ln_bwd_kernel(s), dim3(s.lanes < 0 ? (rows < 4096 ? rows : 4096) : groups), dim3(threads), 0, st, p);
         AETH_LAUNCH_CHECK();
         if (s.lanes < 0) {
-            const int groups = cdiv(C, 64);
-            hipLaunchKernelGGL(ln_bwd_columns, dim3(groups < kLnMostGroups ? groups : kLnMostGroups, blocks), dim3(256), 0, st, p, run);
+            const int columns = cdiv(C, 64);
+            hipLaunchKernelGGL(ln_bwd_columns, dim3(columns < kLnMostGroups ? columns : kLnMostGroups, blocks), dim3(256), 0, st, p, run);
             AETH_LAUNCH_CHECK();
         }
     }

@@ -397,3 +397,40 @@ def test_long_rows_of_like_numbers(rows, c):
     back = _backward(x, dy, gamma, got[1], got[2])
     for g, w, b, name in zip(back, *_long_backward(x, dy, gamma, got[1], got[2]), ("dx", "dgamma", "dbeta")):
         assert R.worst(g, w, b) <= 1, name
+
+
+# blocks: partial rows, of 256 workgroups and for every 256 rows that a lane has
+@pytest.mark.parametrize("rows,c,blocks", [(1 << 27, 8, 4096), (1 << 25, 3, 1024), (3000000, 250, 1536), (400000, 2500, 1792)])
+def test_column_sums_of_like_rows(rows, c, blocks):
+    """Copies of a tile of rows whose terms are all of one sign in a column, up to 2^30 elements: the sums are the tile's, in 64 bits,
+    times the copies.  At most 256 terms are added in line by a lane, then by 6 + 7 levels of lanes and waves; of the partial rows that
+    leaves, 128 lanes take their share each and 7 levels the rest."""
+    from aether import DeviceTensor
+    lib, check = _lib()
+    tile = 4000
+    rows = rows // tile * tile
+    r = np.random.RandomState(c)
+    x = (np.arange(c) - (c + 3) / 2 + 0.01 * r.randn(tile, c)).astype(np.float32)
+    dy = np.full((tile, c), 0.1, np.float32)
+    gamma = np.ones(c, np.float32)
+    small = _forward(x, gamma, gamma)
+
+    def repeated(a):
+        t = DeviceTensor((rows,) + a.shape[1:])
+        check(lib.aeth_memcpy_d2d(t.ptr, _dev(a).ptr, a.nbytes))
+        done = tile
+        while done < rows:
+            n = min(done, rows - done)
+            check(lib.aeth_memcpy_d2d(t[done:done + n].ptr, t.ptr, n * (a.nbytes // tile)))
+            done += n
+        return t
+
+    xd, dyd, md, sd, gd = repeated(x), repeated(dy), repeated(small[1]), repeated(small[2]), _dev(gamma)
+    dx, dg, db = DeviceTensor((rows, c)), _nan(c), _nan(c)
+    check(lib.aeth_ln_bwd_f32(xd.ptr, dyd.ptr, gd.ptr, md.ptr, sd.ptr, dx.ptr, dg.ptr, db.ptr, rows, c))
+    (_, dgamma, dbeta), _ = R.backward(x, dy, gamma, small[1], small[2])
+    depth = 256 + 13 + blocks / 128 + 7
+    n = rows // tile
+    size = (np.abs(dy * (x - small[1][:, None]).astype(np.float64) * small[2][:, None])).sum(0)
+    assert R.worst(db.get(), n * dbeta, depth * U * n * np.abs(dbeta)) <= 1
+    assert R.worst(dg.get(), n * dgamma, (depth + 3) * U * n * size) <= 1
