@@ -11,6 +11,8 @@
 // line (a row in registers), and a few hundred over the rows (kLnRun); a row of any length is summed in 64 bits.
 #include "common.h"
 
+#include <algorithm>
+
 namespace aeth {
 
 constexpr int kLnLong = 1024;                            // threads of the kernels for rows of any length
@@ -514,7 +516,8 @@ __global__ __launch_bounds__(kLnLong) void ln_bwd_rows(const LnBwdArgs p) {
     }
 }
 
-// Partial sums of dy xhat and dy over a run of rows: 64 columns x 4 row lanes per workgroup, part[run][2][C].
+// Sums of dy xhat and dy over a run of rows: 64 columns x 4 row lanes per workgroup, to part[run][2][C], or to dgamma and dbeta where one
+// run has all rows (part == NULL).
 __global__ __launch_bounds__(256) void ln_bwd_columns(const LnBwdArgs p, int run) {
     __shared__ float red[2][4][64];
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, C = p.C;
@@ -532,9 +535,10 @@ __global__ __launch_bounds__(256) void ln_bwd_columns(const LnBwdArgs p, int run
         red[0][w][lane] = a;
         red[1][w][lane] = b;
         __syncthreads();
-        if (w < 2 && c < C)
-            p.part[((size_t)blockIdx.y * 2 + w) * C + c] =
-                (red[w][0][lane] + red[w][1][lane]) + (red[w][2][lane] + red[w][3][lane]);
+        if (w < 2 && c < C) {
+            float* out = p.part != nullptr ? p.part + ((size_t)blockIdx.y * 2 + w) * C : w == 0 ? p.dgamma : p.dbeta;
+            out[c] = (red[w][0][lane] + red[w][1][lane]) + (red[w][2][lane] + red[w][3][lane]);
+        }
     }
 }
 
@@ -682,7 +686,7 @@ static LnBwd ln_bwd_kernel(const LnShape& s) {
             if (s.threads > 512) return s.v == 6 ? ln_bwd_block<768, 6> : ln_bwd_block<768, 7>;
             return s.v <= 4 ? ahead[s.v - 2] : block[s.v - 6];
     }
-    return ln_bwd_rows;
+    return nullptr;                                      // (rows of any length: ln_bwd_rows and ln_bwd_columns)
 }
 
 // Backward: with the next row on its way where that fits 512 threads, else without; then 768 threads, whose 168 registers take up to
@@ -739,15 +743,15 @@ static int ln_bwd_impl(const float* x, const float* dy, const float* gamma, cons
     void* ws = nullptr;
     if (rows > 0) {
         const LnShape s = ln_bwd_shape(C);
-        int threads = s.threads, turns = rows, cap;
+        int threads = s.threads, turns = rows, cap = 0;
         if (s.lanes > 0) {
             threads = kLnBwdWaveThreads;
             turns = cdiv(rows, threads / s.lanes);
             cap = 256;                                   // (pixels x64 with twin: 512 workgroups 143 us, 256 129)
-        } else {
+        } else if (s.lanes == 0) {
             // whole workgroups a CU, 512 threads of them (16384 x 5000: 182 us with 512 threads a CU, 193 with 640 and 768, 197 with
             // 1024; 4096 x 16384: 171, 171, 170, 183); more leave more partial rows, a part of one leaves CUs idle
-            cap = s.lanes < 0 ? 64 : 256 * (threads < 512 ? 512 / threads : 1);
+            cap = 256 * (threads < 512 ? 512 / threads : 1);
         }
         // One launch for few rows: 128 x 256 3.1 us instead of 5.6, 512 x 256 4.1 and 5.6, 512 x 2048 5.4 and 9.3, 128 x 8192 6.0 and 12.4,
         // 256 x 20000 27 and 36; but a column's rows are one workgroup's: 1024 x 256 6.3 and 5.8, 512 x 8192 18 and 17
@@ -758,18 +762,30 @@ static int ln_bwd_impl(const float* x, const float* dy, const float* gamma, cons
             AETH_LAUNCH_CHECK();
             return AETH_OK;
         }
-        // as many workgroups as are needed for each to take no more rows than with `cap` of them
-        const int run = cdiv(turns, cap), groups = cdiv(turns, run), pieces = s.lanes < 0 ? 1 : cdiv(run, kLnRun);
-        blocks = groups * pieces;
-        const int rc = workspace((int64_t)2 * blocks * C * sizeof(float), &ws);
-        if (rc) return rc;
-        const LnBwdArgs p{x, dy, gamma, mean, invstd, dx, dx16, rows, C, 1.0f / (float)C, (float*)ws, 4 * n >= kLnStreamBytes, groups, pieces,
-                          nullptr, nullptr};
-        hipLaunchKernelGGL(ln_bwd_kernel(s), dim3(s.lanes < 0 ? (rows < 4096 ? rows : 4096) : groups), dim3(threads), 0, st, p);
-        AETH_LAUNCH_CHECK();
         if (s.lanes < 0) {
-            const int columns = cdiv(C, 64);
+            // runs for eight workgroups a CU, as far as the columns leave too few, of 16 rows at least (a partial row each: an eighth of
+            // the tensor's bytes at most) and 512 at most (128 a lane)
+            const int columns = cdiv(C, 64), run = std::min(std::max(cdiv(rows, cdiv(2048, columns)), 16), 512);
+            blocks = cdiv(rows, run);
+            if (blocks > 1) {
+                const int rc = workspace((int64_t)2 * blocks * C * sizeof(float), &ws);
+                if (rc) return rc;
+            }
+            const LnBwdArgs p{x, dy, gamma, mean, invstd, dx, dx16, rows, C, 1.0f / (float)C, (float*)ws, false, 0, 0, dgamma, dbeta};
+            hipLaunchKernelGGL(ln_bwd_rows, dim3(rows < 4096 ? rows : 4096), dim3(threads), 0, st, p);
+            AETH_LAUNCH_CHECK();
             hipLaunchKernelGGL(ln_bwd_columns, dim3(columns < kLnMostGroups ? columns : kLnMostGroups, blocks), dim3(256), 0, st, p, run);
+            AETH_LAUNCH_CHECK();
+            if (blocks == 1) return AETH_OK;
+        } else {
+            // as many workgroups as are needed for each to take no more rows than with `cap` of them
+            const int run = cdiv(turns, cap), groups = cdiv(turns, run), pieces = cdiv(run, kLnRun);
+            blocks = groups * pieces;
+            const int rc = workspace((int64_t)2 * blocks * C * sizeof(float), &ws);
+            if (rc) return rc;
+            const LnBwdArgs p{x, dy, gamma, mean, invstd, dx, dx16, rows, C, 1.0f / (float)C, (float*)ws, 4 * n >= kLnStreamBytes, groups,
+                              pieces, nullptr, nullptr};
+            hipLaunchKernelGGL(ln_bwd_kernel(s), dim3(groups), dim3(threads), 0, st, p);
             AETH_LAUNCH_CHECK();
         }
     }

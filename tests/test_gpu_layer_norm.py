@@ -434,3 +434,46 @@ def test_column_sums_of_like_rows(rows, c, blocks):
     size = (np.abs(dy * (x - small[1][:, None]).astype(np.float64) * small[2][:, None])).sum(0)
     assert R.worst(db.get(), n * dbeta, depth * U * n * np.abs(dbeta)) <= 1
     assert R.worst(dg.get(), n * dgamma, (depth + 3) * U * n * size) <= 1
+
+
+# one run of rows (16 and 17 of them, 64 with columns enough), several, the longest
+@pytest.mark.parametrize("rows,c", [(1, 21505), (15, 21600), (16, 21505), (17, 21505), (64, 100000), (100, 40000), (513, 22001), (4100, 21507)])
+def test_runs_of_long_rows(rows, c):
+    x, gamma, beta, dy = _inputs(rows, c, seed=6)
+    _, mean, inv, _ = _forward(x, gamma, beta)
+    back = _backward(x, dy, gamma, mean, inv)
+    for g, w, b, name in zip(back, *_long_backward(x, dy, gamma, mean, inv), ("dx", "dgamma", "dbeta")):
+        assert R.worst(g, w, b) <= 1, name
+    assert all(np.array_equal(a, b) for a, b in zip(back[:3], _backward(x, dy, gamma, mean, inv)[:3]))
+
+
+def test_the_scratch_of_long_rows_stays_below_their_tensor():
+    """64 rows of 2^23 (2 GiB): where they were given a run each, the partial rows took twice that.  A recording refuses a workspace
+    that grows, so the calls go through one, after everything else that has grown it is gone (a process of its own)."""
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    code = """
+import ctypes as C, sys
+sys.path[:0] = [%r, %r]
+import numpy as np
+from aether import DeviceTensor, _lib
+lib, check = _lib.lib(), _lib.check
+rows, c = 64, 1 << 23
+x, dy, dx = DeviceTensor.full((rows, c), 1.0), DeviceTensor.full((rows, c), 0.5), DeviceTensor((rows, c))
+g, dg, db = DeviceTensor.full(c, 1.0), DeviceTensor(c), DeviceTensor(c)
+m, s = DeviceTensor.zeros(rows), DeviceTensor.full(rows, 1.0)
+check(lib.aeth_graph_begin())
+rc = lib.aeth_ln_bwd_f32(x.ptr, dy.ptr, g.ptr, m.ptr, s.ptr, dx.ptr, dg.ptr, db.ptr, rows, c)
+graph = C.c_void_p()
+check(lib.aeth_graph_end(C.byref(graph)))
+check(rc)
+for _ in range(2):
+    check(lib.aeth_graph_launch(graph))
+    assert np.all(dg.get() == 32) and np.all(db.get() == 32)
+check(lib.aeth_graph_destroy(graph))
+print("done")
+""" % (root, os.path.join(root, "aether-ml_amd"))
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=100)
+    assert r.returncode == 0 and r.stdout.endswith("done\n"), r.stderr[-2000:]
