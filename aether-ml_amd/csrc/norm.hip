@@ -325,8 +325,8 @@ struct LnBwdRow {
     }
 };
 
-// gamma of a lane's units, 0 in the places that a unit does not own: their g is 0 in the sums (or NaN, in a row that has one), their
-// dx is not written, their column sums are dropped.
+// gamma of a lane's units, 0 in the places that a unit does not own: used here, it has arrived before the rows' loop (a wait for it
+// inside the loop is one for the next row's loads too: 2^27 rows of one float 3.7 ms instead of 2.6).
 template <int V, bool kTiny>
 __device__ __forceinline__ void ln_gains(const LnBwdArgs& p, const LnLane<V, kTiny>& u, float (*gm)[4]) {
 #pragma unroll
@@ -338,7 +338,9 @@ __device__ __forceinline__ void ln_gains(const LnBwdArgs& p, const LnLane<V, kTi
     }
 }
 
-// One row: its part of the column sums, and its dx.  `sum(float*)`: two sums over the row's lanes.
+// One row: its part of the column sums, and its dx.  Places that a unit does not own count 0 times in the row's sums, whatever they hold
+// (an infinity times a gain of 0 would be NaN); their dx is not written, their column sums are dropped.  `sum(float*)`: two sums over the
+// row's lanes.
 template <int V, bool kTiny, typename Sum>
 __device__ __forceinline__ void ln_bwd_row(const LnBwdArgs& p, int64_t r, const LnLane<V, kTiny>& u, LnBwdRow<V>& w,
                                            const float (*gm)[4], float (*dg)[4], float (*db)[4], Sum sum) {
@@ -347,7 +349,8 @@ __device__ __forceinline__ void ln_bwd_row(const LnBwdArgs& p, int64_t r, const 
     for (int j = 0; j < V; ++j)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            const float xh = (w.x[j][e] - w.mean) * w.invstd, d = w.dy[j][e], g = d * gm[j][e];
+            const bool own = kTiny || u.own(j, e);       // (of a tiny row other places hold 0)
+            const float d = w.dy[j][e], xh = own ? (w.x[j][e] - w.mean) * w.invstd : 0.f, g = own ? d * gm[j][e] : 0.f;
             dg[j][e] = fmaf(d, xh, dg[j][e]);
             db[j][e] += d;
             s[0] += g;

@@ -477,3 +477,30 @@ print("done")
 """ % (root, os.path.join(root, "aether-ml_amd"))
     r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=100)
     assert r.returncode == 0 and r.stdout.endswith("done\n"), r.stderr[-2000:]
+
+
+@pytest.mark.parametrize("rows,c", [(4, 1), (4, 3), (4, 5), (4, 6), (4, 7), (4, 64), (4, 101), (4, 255), (4, 1537), (4, 2050), (3, 4099),
+                                    (3, 20001), (3, 30001), (600, 7), (600, 101), (300, 2050)])
+def test_infinite_gradients(rows, c):
+    """An infinity in dy, wherever it stands in its row, gives that row the formula's infinities and NaN, its column's dgamma and dbeta
+    an infinity, and nothing else."""
+    x, gamma, beta, dy = _inputs(rows, c, seed=8)
+    fwd = _forward(x, gamma, beta)
+    clean = _backward(x, dy, gamma, fwd[1], fwd[2])
+    places = sorted({0, c // 2, c - 1, max(0, c - 2), max(0, c - 3), max(0, c - 4), max(0, c - 5)})
+    for col in places:
+        for value in (np.inf, -np.inf):
+            bad = dy.copy()
+            bad[1, col] = value
+            got = _backward(x, bad, gamma, fwd[1], fwd[2])
+            with np.errstate(invalid="ignore"):              # (a single column has xhat = 0: its dgamma is NaN)
+                xhat = (x[1].astype(np.float64) - fwd[1][1]) * fwd[2][1]
+                g = bad[1].astype(np.float64) * gamma
+                dx = fwd[2][1] * (g - g.mean() - xhat * (g * xhat).mean())
+                dgamma = value * np.sign(xhat[col])
+            assert np.array_equal(got[0][1].astype(np.float64), dx, equal_nan=True), (col, value)
+            others = [r for r in range(rows) if r != 1]
+            assert np.array_equal(got[0][others], clean[0][others])
+            rest = [k for k in range(c) if k != col]
+            assert np.array_equal(got[1][rest], clean[1][rest]) and np.array_equal(got[2][rest], clean[2][rest])
+            assert got[2][col] == value and np.array_equal(got[1][col], dgamma, equal_nan=True)
