@@ -967,21 +967,21 @@ class Optimizer_Adam:
     # -- recorded steps: the step number lives on the device -----------------------------
     def device_state(self):
         """{iterations, beta_1^iterations, beta_2^iterations, lr} as 4 doubles on the device,
-        brought in line with ``self.iterations`` whenever eager steps moved it."""
+        brought in line with ``self.iterations`` and the betas whenever they are others than the recorded steps left."""
         if getattr(self, "_state", None) is None:
             self._state = DeviceTensor(4, np.float64)
-            self._state_iterations = None
-        if self._state_iterations != self.iterations:
+            self._state_holds = None
+        if self._state_holds != (self.iterations, self.beta_1, self.beta_2):
             b1, b2 = float(np.float32(self.beta_1)), float(np.float32(self.beta_2))   # what the kernels receive
             self._state.set(np.array([self.iterations, b1 ** self.iterations, b2 ** self.iterations,
                                       self.current_learning_rate], dtype=np.float64))
-            self._state_iterations = self.iterations
+            self._state_holds = (self.iterations, self.beta_1, self.beta_2)
         return self._state
 
     def recorded_settings(self, layers):
         """What a recorded update holds besides its tensors: with other values it has to be recorded anew, after a normal
         step with them."""
-        return self._base_rate(), self.decay, self.epsilon
+        return self._base_rate(), self.decay, self.epsilon, self.beta_1, self.beta_2
 
     def _base_rate(self):
         """What a step without decay would take (pre_update_parameters leaves the current rate alone then)."""
@@ -1015,7 +1015,7 @@ class Optimizer_Adam:
         if self.decay:
             self.current_learning_rate = self.learning_rate * (1. / (1. + self.decay * self.iterations))
         self.iterations += 1
-        self._state_iterations = self.iterations
+        self._state_holds = (self.iterations, self.beta_1, self.beta_2)
         for t in getattr(self, "_recorded_params", ()):
             t.touched()
 

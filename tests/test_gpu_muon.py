@@ -577,3 +577,36 @@ def test_more_steps_in_the_middle_of_recorded_training():
         runs.append(_host(model))
         model.record_steps(False)
     assert all(np.array_equal(a, b) for a, b in zip(*runs))
+
+
+@pytest.mark.parametrize("muon", [False, True])
+@pytest.mark.parametrize("change", [dict(beta_1=.5), dict(beta_2=.9), dict(epsilon=1e-3), dict(beta_1=.7, beta_2=.99)])
+def test_other_betas_make_a_recording_stale(muon, change):
+    """The betas are in a recording twice: in its kernels and, to the power of the step number, in the state on the device."""
+    import aether
+    steps = _batches(7)
+    runs = []
+    for record in (False, True):
+        model = _network(aether.Optimizer_Muon() if muon else aether.Optimizer_Adam(), norm=False)
+        model.record_steps(record)
+        for k, (x, y) in enumerate(steps):
+            if k == 4:
+                for name, value in change.items():
+                    setattr(model.optimizer.adam if muon else model.optimizer, name, value)
+            model.train_step(x, y)
+        if record:
+            assert any(rec["graph"] for rec in model._recordings.values())
+        runs.append(_host(model))
+        model.record_steps(False)
+    assert all(np.array_equal(a, b) for a, b in zip(*runs))
+
+
+def test_the_state_on_the_device_follows_the_betas():
+    """Between two replays, without a step that would move the step number."""
+    import aether
+    opt = aether.Optimizer_Adam()
+    opt.iterations = 3
+    for b1, b2 in ((.9, .999), (.5, .999), (.5, .75)):
+        opt.beta_1, opt.beta_2 = b1, b2
+        want = [3, float(np.float32(b1)) ** 3, float(np.float32(b2)) ** 3, opt.current_learning_rate]
+        assert np.array_equal(opt.device_state().get(), np.array(want))
