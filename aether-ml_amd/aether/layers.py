@@ -945,6 +945,10 @@ class Optimizer_Adam:
         """Whether an update of this layer has created its moments."""
         return hasattr(layer, "weight_cache")
 
+    def state_tensors(self, layer):
+        """The moments that an update of this layer reads and writes."""
+        return layer.weight_momentums, layer.weight_cache, layer.bias_momentums, layer.bias_cache
+
     def _flush(self):
         import ctypes as C
         while self._pending:
@@ -1087,6 +1091,11 @@ class Optimizer_Muon:
         if not self.takes(layer):
             return self.adam.has_state(layer)
         return hasattr(layer, "muon_momentums") and hasattr(layer, "bias_cache")
+
+    def state_tensors(self, layer):
+        if not self.takes(layer):
+            return self.adam.state_tensors(layer)
+        return layer.muon_momentums, layer.bias_momentums, layer.bias_cache
 
     def _matrices(self, batch):
         """The host arrays of one call: pointers of weights, gradients, momentums; rows; columns."""

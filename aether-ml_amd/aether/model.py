@@ -244,9 +244,10 @@ class Model:
                 _lib.check(lib.aeth_graph_destroy(rec["graph"]))
             recs[key] = {"graph": None, "optimizer": self.optimizer, "settings": settings}
             return None
-        # a recording reads and writes the parameter buffers it was made with: parameters set anew since then
-        # (set_parameters, load_parameters) make it stale
-        params = [(id(l), l.weights.ptr, l.biases.ptr) for l in self.trainable_layers]
+        # a recording reads and writes the buffers it was made with: parameters set anew since then (set_parameters,
+        # load_parameters) or moments made anew (their old memory is somebody else's) make it stale
+        params = [(id(l),) + tuple(t.ptr for t in (l.weights, l.biases) + self.optimizer.state_tensors(l))
+                  for l in self.trainable_layers]
         if rec["graph"] is not None and rec.get("params") != params:
             _lib.check(lib.aeth_graph_destroy(rec["graph"]))
             recs[key] = rec = {"graph": None, "optimizer": self.optimizer, "settings": settings}

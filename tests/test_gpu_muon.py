@@ -610,3 +610,32 @@ def test_the_state_on_the_device_follows_the_betas():
         opt.beta_1, opt.beta_2 = b1, b2
         want = [3, float(np.float32(b1)) ** 3, float(np.float32(b2)) ** 3, opt.current_learning_rate]
         assert np.array_equal(opt.device_state().get(), np.array(want))
+
+
+@pytest.mark.parametrize("muon", [False, True])
+def test_moments_made_anew_make_every_recording_stale(muon):
+    """Two batch shapes are recorded, then training starts over with fresh moments: the step that makes them runs normally, and the
+    other shape's recording, which knows the old ones, may not be replayed."""
+    import aether
+    steps = _batches(8)
+    runs = []
+    for record in (False, True):
+        model = _network(aether.Optimizer_Muon() if muon else aether.Optimizer_Adam(), norm=False)
+        model.record_steps(record)
+        for k, (x, y) in enumerate(steps):
+            if k == 4:
+                if record:
+                    assert len([rec for rec in model._recordings.values() if rec["graph"]]) == 2
+                for layer in model.trainable_layers:
+                    for name in ("weight_momentums", "weight_cache", "bias_momentums", "bias_cache", "muon_momentums"):
+                        if hasattr(layer, name):
+                            delattr(layer, name)
+            model.train_step(x, y)
+            model.train_step(x[:7], y[:7])
+            if k == 5:                                   # other moments in place of those that are there
+                for layer in model.trainable_layers:
+                    layer.bias_cache = aether.DeviceTensor.full(layer.biases.shape, 1e-3)
+        runs.append((_host(model), [layer.bias_momentums.get() for layer in model.trainable_layers]))
+        model.record_steps(False)
+    for a, b in zip(*runs):
+        assert all(np.array_equal(p, q) for p, q in zip(a, b))
