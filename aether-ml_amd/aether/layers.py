@@ -14,6 +14,7 @@ Departures from the reference, each deliberate:
   * ``Pooling(padding="same")`` raises ValueError (the reference reads ``H_out``
     before assigning it, :226-228).
 """
+import contextlib
 import os
 
 import numpy as np
@@ -907,6 +908,17 @@ class Activation_Softmax_Loss_CategoricalCrossEntropy():
         _ck(fn(dvalues.ptr, labels.ptr, ls, self.dinputs.ptr, rows, K))
 
 
+@contextlib.contextmanager
+def _or_drop(optimizer):
+    """A refused step leaves no updates queued: the next step queues the same tensors again, and one launch that updates a
+    tensor from two places at once races."""
+    try:
+        yield
+    except BaseException:
+        optimizer._drop()
+        raise
+
+
 # ----------------------------------------------------------------------------------
 # Optimizer_Adam  (CNN_classes_cupy.py:685-736)
 # ----------------------------------------------------------------------------------
@@ -922,10 +934,19 @@ class Optimizer_Adam:
         self._pending = []
 
     def pre_update_parameters(self):
+        with _or_drop(self):
+            self._flush()                                    # (nothing, unless the last step was broken off)
         if self.decay:
             self.current_learning_rate = self.learning_rate * (1. / (1. + self.decay * self.iterations))
 
     def update_parameters(self, layer):
+        with _or_drop(self):
+            self._update(layer)
+
+    def _drop(self):
+        self._pending = []
+
+    def _update(self, layer):
         if not hasattr(layer, "weight_cache"):
             layer.weight_momentums = DeviceTensor.zeros(layer.weights.shape)
             layer.weight_cache = DeviceTensor.zeros(layer.weights.shape)
@@ -965,7 +986,8 @@ class Optimizer_Adam:
                 t[0].touched()                               # the parameters changed in place
 
     def post_update_parameters(self):
-        self._flush()
+        with _or_drop(self):
+            self._flush()
         self.iterations += 1
 
     # -- recorded steps: the step number lives on the device -----------------------------
@@ -1068,11 +1090,21 @@ class Optimizer_Muon:
         return bool(wanted) and len(shape) >= 2 and shape[-1] > 1 and layer.weights.size > shape[-1]
 
     def pre_update_parameters(self):
+        with _or_drop(self):
+            self._flush()                                    # (as Adam's)
+            self.adam.pre_update_parameters()
         if self.decay:
             self.current_learning_rate = self.learning_rate * (1. / (1. + self.decay * self.iterations))
-        self.adam.pre_update_parameters()
 
     def update_parameters(self, layer):
+        with _or_drop(self):
+            self._update(layer)
+
+    def _drop(self):
+        self._pending = []
+        self.adam._drop()
+
+    def _update(self, layer):
         if not self.takes(layer):
             self.adam.update_parameters(layer)
             return
@@ -1118,8 +1150,9 @@ class Optimizer_Muon:
                 t[0].touched()                               # the parameters changed in place
 
     def post_update_parameters(self):
-        self._flush()
-        self.adam.post_update_parameters()
+        with _or_drop(self):
+            self._flush()
+            self.adam.post_update_parameters()
         self.iterations += 1
 
     # -- recorded steps: step number and learning rates live on the device ----------------
