@@ -950,6 +950,7 @@ class Optimizer_Adam:
         if not hasattr(layer, "weight_cache"):
             layer.weight_momentums = DeviceTensor.zeros(layer.weights.shape)
             layer.weight_cache = DeviceTensor.zeros(layer.weights.shape)
+        if not hasattr(layer, "bias_cache"):                 # (a layer that Optimizer_Muon let go has these)
             layer.bias_momentums = DeviceTensor.zeros(layer.biases.shape)
             layer.bias_cache = DeviceTensor.zeros(layer.biases.shape)
         # The updates of all layers of a step go out as one launch: they are queued
@@ -964,7 +965,7 @@ class Optimizer_Adam:
 
     def has_state(self, layer):
         """Whether an update of this layer has created its moments."""
-        return hasattr(layer, "weight_cache")
+        return hasattr(layer, "weight_cache") and hasattr(layer, "bias_cache")
 
     def state_tensors(self, layer):
         """The moments that an update of this layer reads and writes."""

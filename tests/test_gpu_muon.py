@@ -639,3 +639,22 @@ def test_moments_made_anew_make_every_recording_stale(muon):
         model.record_steps(False)
     for a, b in zip(*runs):
         assert all(np.array_equal(p, q) for p, q in zip(a, b))
+
+
+def test_a_layer_taken_out_of_muon_goes_on_with_its_bias():
+    """The step after it moves the bias by Adam's formula from the moments that it had."""
+    import aether
+    from tests import step_checks
+    opt = aether.Optimizer_Muon(adam_learning_rate=2e-3)
+    model = _network(opt, norm=False)
+    steps = _batches(4)
+    for x, y in steps[:3]:
+        model.train_step(x, y)
+    layer = model.trainable_layers[1]
+    layer.muon = False
+    before = [t.get() for t in (layer.biases, layer.bias_momentums, layer.bias_cache)]
+    assert np.any(before[2] != 0)
+    model.train_step(*steps[3])
+    e = step_checks.update_errors(before[0], layer.dbiases.get(), before[1], before[2], layer.biases.get(),
+                                  layer.bias_momentums.get(), layer.bias_cache.get(), 2e-3, 3)
+    assert max(e) <= 1

@@ -115,3 +115,19 @@ def test_a_step_broken_off_is_not_mixed_into_the_next(library, make):
     _step(opt, layers)
     assert _updated(library) == sorted(_all(layers) + _all(layers[:1]))
     assert all(len(set(tensors)) == len(tensors) for _, tensors in library.calls)
+
+
+def test_a_layer_taken_out_of_muon_keeps_its_bias_moments(library):
+    opt, layers = aether.Optimizer_Muon(), [_layer() for _ in range(2)]
+    for _ in range(2):
+        _step(opt, layers)
+    held = layers[0].bias_momentums, layers[0].bias_cache
+    layers[0].muon = False
+    assert not opt.has_state(layers[0])
+    _step(opt, layers)
+    assert (layers[0].bias_momentums, layers[0].bias_cache) == held and opt.has_state(layers[0])
+    assert layers[0].weight_momentums.shape == layers[0].weight_cache.shape == layers[0].weights.shape
+    matrix = layers[0].muon_momentums
+    layers[0].muon = True
+    _step(opt, layers)
+    assert (layers[0].muon_momentums, layers[0].bias_momentums, layers[0].bias_cache) == (matrix,) + held
