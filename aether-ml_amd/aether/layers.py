@@ -1070,14 +1070,29 @@ class Optimizer_Muon:
             raise ValueError(f"Expected weight_decay >= 0, got {weight_decay}.")
         self.learning_rate = learning_rate
         self.current_learning_rate = learning_rate
-        self.decay = decay
-        self.iterations = 0
         self.momentum = momentum
         self.nesterov = nesterov
         self.ns_steps = ns_steps
         self.weight_decay = weight_decay
         self.adam = Optimizer_Adam(adam_learning_rate, decay, epsilon, beta_1, beta_2)
         self._pending = []
+
+    # the decay and the step number are Adam's: a change of either (a resumed run) is one for both kinds of parameters
+    @property
+    def decay(self):
+        return self.adam.decay
+
+    @decay.setter
+    def decay(self, value):
+        self.adam.decay = value
+
+    @property
+    def iterations(self):
+        return self.adam.iterations
+
+    @iterations.setter
+    def iterations(self, value):
+        self.adam.iterations = value
 
     @staticmethod
     def takes(layer):
@@ -1153,8 +1168,7 @@ class Optimizer_Muon:
     def post_update_parameters(self):
         with _or_drop(self):
             self._flush()
-            self.adam.post_update_parameters()
-        self.iterations += 1
+            self.adam.post_update_parameters()               # (counts the step)
 
     # -- recorded steps: step number and learning rates live on the device ----------------
     def device_state(self):
@@ -1195,8 +1209,7 @@ class Optimizer_Muon:
         """Host bookkeeping after a recorded step has run once more."""
         if self.decay:
             self.current_learning_rate = self.learning_rate * (1. / (1. + self.decay * self.iterations))
-        self.iterations += 1
+        self.adam.replayed()                                 # (counts the step)
         self._state_iterations = self.iterations
         for t in getattr(self, "_recorded_params", ()):
             t.touched()
-        self.adam.replayed()

@@ -658,3 +658,24 @@ def test_a_layer_taken_out_of_muon_goes_on_with_its_bias():
     e = step_checks.update_errors(before[0], layer.dbiases.get(), before[1], before[2], layer.biases.get(),
                                   layer.bias_momentums.get(), layer.bias_cache.get(), 2e-3, 3)
     assert max(e) <= 1
+
+
+def test_a_resumed_run_in_recorded_training():
+    """The step number and the decay set in the middle: replays and eager steps go on alike, both learning rates lowered."""
+    import aether
+    steps = _batches(8)
+    runs = []
+    for record in (False, True):
+        model = _network(aether.Optimizer_Muon(), norm=False)
+        model.record_steps(record)
+        for k, (x, y) in enumerate(steps):
+            if k == 3:
+                model.optimizer.iterations = 50
+            if k == 5:
+                model.optimizer.decay = .1
+            model.train_step(x, y)
+        assert model.optimizer.iterations == model.optimizer.adam.iterations == 55
+        assert np.isclose(model.optimizer.adam.current_learning_rate, 1e-3 / (1 + .1 * 54))
+        runs.append(_host(model))
+        model.record_steps(False)
+    assert all(np.array_equal(a, b) for a, b in zip(*runs))

@@ -131,3 +131,23 @@ def test_a_layer_taken_out_of_muon_keeps_its_bias_moments(library):
     layers[0].muon = True
     _step(opt, layers)
     assert (layers[0].muon_momentums, layers[0].bias_momentums, layers[0].bias_cache) == (matrix,) + held
+
+
+def test_decay_and_step_number_of_muon_are_adams_too(library):
+    """A resumed run sets them on the optimizer; both learning rates follow, in eager steps and in what a recording is checked by."""
+    opt, layers = aether.Optimizer_Muon(learning_rate=.1, adam_learning_rate=.01), [_layer()]
+    _step(opt, layers)
+    assert opt.iterations == opt.adam.iterations == 1 and opt.decay == 0
+    before = opt.recorded_settings(layers)
+    opt.decay, opt.iterations = .5, 4
+    opt.pre_update_parameters()
+    assert opt.current_learning_rate == .1 * (1 / 3) and opt.adam.current_learning_rate == .01 * (1 / 3)    # (the formula's roundings)
+    after = opt.recorded_settings(layers)
+    assert after != before and after[6] != before[6]
+    opt.update_parameters(layers[0])
+    opt.post_update_parameters()
+    assert opt.iterations == opt.adam.iterations == 5
+    opt.replayed()
+    assert opt.iterations == opt.adam.iterations == 6 and np.isclose(opt.current_learning_rate, .1 / 3.5)
+    assert np.isclose(opt.adam.current_learning_rate, .01 / 3.5)
+    assert aether.Optimizer_Muon(decay=.25).decay == .25
