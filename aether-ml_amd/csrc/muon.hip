@@ -506,7 +506,8 @@ static int muon_float_product(FloatTable tb, float alpha, float beta, float lr, 
     return AETH_OK;
 }
 
-static int muon_float_group(const MuonMatrix* t, int count, float lr, const double* state, float mu, int nesterov, float wd, int steps) {
+static int muon_float_group(const MuonMatrix* t, int count, float lr, const double* state, float mu, int nesterov, float wd, int steps,
+                            int64_t* need) {
     MuonTable norm = {};
     MuonScaleTable scale = {};
     FloatTable gram = {}, poly = {}, step[2] = {};
@@ -523,6 +524,10 @@ static int muon_float_group(const MuonMatrix* t, int count, float lr, const doub
         if (norm.parts[i] > parts) parts = norm.parts[i];
         scale.first[i] = (int)blocks;
         blocks += at[i].mp / 32 * (at[i].np / 32);
+    }
+    if (need != nullptr) {
+        *need = std::max(*need, bytes);
+        return AETH_OK;
     }
     void* ws;
     const int rc = workspace(bytes, &ws);
@@ -625,8 +630,9 @@ static int muon_gram_runs(SplitTable tb, int tile) {
     return AETH_OK;
 }
 
-// The whole update of at most kMuonMax matrices that share the workspace.
-static int muon_group(const MuonMatrix* t, int count, float lr, const double* state, float mu, int nesterov, float wd, int steps) {
+// The whole update of at most kMuonMax matrices that share the workspace.  With `need`: only the bytes of it, if they are more.
+static int muon_group(const MuonMatrix* t, int count, float lr, const double* state, float mu, int nesterov, float wd, int steps,
+                      int64_t* need) {
     MuonTable tb = {};
     SplitTable gram = {}, poly = {}, step[2] = {}, apply = {};
     MuonLayout at[kMuonMax];
@@ -649,6 +655,10 @@ static int muon_group(const MuonMatrix* t, int count, float lr, const double* st
     const bool in_runs = muon_choose_runs(shapes, count, &runs);
     const int64_t partial = bytes;                       // (after the matrices: a multiple of 4096 bytes from their begin)
     if (in_runs) bytes += runs.bytes;
+    if (need != nullptr) {
+        *need = std::max(*need, bytes);
+        return AETH_OK;
+    }
     void* ws;
     const int rc = workspace(bytes, &ws);
     if (rc) return rc;
@@ -736,19 +746,14 @@ static int muon_small(const MuonMatrix* t, int count, int row_blocks, int blocks
 // Matrices whose buffers together pass this go out in several groups, one after the other.
 constexpr int64_t kMuonWorkspace = (int64_t)4 << 30;
 
-// The matrices that two halves do not carry through the steps, on float32 products.
-static int muon_float(const MuonMatrix* t, int count, float lr, const double* state, float mu, int nesterov, float wd, int steps) {
+// group(first, how many) for every group; bytes(matrix): of its buffers.
+template <typename Bytes, typename Group>
+static int muon_in_groups(const MuonMatrix* t, int count, Bytes bytes, Group group) {
     for (int i = 0; i < count;) {
-        int64_t bytes = 0;
-        int k = 0;
-        while (i + k < count) {
-            const MuonMatrix& x = t[i + k];
-            const int64_t more = muon_float_layout(std::min(x.rows, x.cols), std::max(x.rows, x.cols), 0).end;
-            if (k > 0 && bytes + more > kMuonWorkspace) break;
-            bytes += more;
-            ++k;
-        }
-        const int rc = muon_float_group(t + i, k, lr, state, mu, nesterov, wd, steps);
+        int64_t sum = bytes(t[i]);
+        int k = 1;
+        while (i + k < count && sum + bytes(t[i + k]) <= kMuonWorkspace) sum += bytes(t[i + k++]);
+        const int rc = group(t + i, k);
         if (rc) return rc;
         i += k;
     }
@@ -756,38 +761,45 @@ static int muon_float(const MuonMatrix* t, int count, float lr, const double* st
 }
 
 static int muon_run(MuonMatrix* t, int count, float lr, const double* state, float mu, int nesterov, float wd, int steps) {
-    const int halves = (int)(std::stable_partition(t, t + count, [&](const MuonMatrix& x) {
-                                 return muon_in_halves(std::max(x.rows, x.cols), steps);
-                             }) - t);
-    if (halves < count) {
-        const int rc = muon_float(t + halves, count - halves, lr, state, mu, nesterov, wd, steps);
-        if (rc) return rc;
-    }
-    count = halves;
-    if (count == 0) return AETH_OK;
-    int row_blocks;
-    const int blocks = muon_whole_blocks(t, count, &row_blocks);
-    if (blocks > 0) return muon_small(t, count, row_blocks, blocks, lr, state, mu, nesterov, wd, steps);
+    // those that two halves do not carry through the steps come last
+    MuonMatrix* const rest = std::stable_partition(
+        t, t + count, [&](const MuonMatrix& x) { return muon_in_halves(std::max(x.rows, x.cols), steps); });
+    const int halves = (int)(rest - t), floats = count - halves;
+    int row_blocks = 0;
+    const int blocks = halves > 0 ? muon_whole_blocks(t, halves, &row_blocks) : 0;
     // the longest tiles first: what is left at a launch's end is short
-    std::stable_sort(t, t + count, [](const MuonMatrix& a, const MuonMatrix& b) {
-        const int n = a.rows > a.cols ? a.rows : a.cols, p = b.rows > b.cols ? b.rows : b.cols;
-        return n != p ? n > p : (a.rows < a.cols ? a.rows : a.cols) > (b.rows < b.cols ? b.rows : b.cols);
+    std::stable_sort(t, rest, [](const MuonMatrix& a, const MuonMatrix& b) {
+        const int n = std::max(a.rows, a.cols), p = std::max(b.rows, b.cols);
+        return n != p ? n > p : std::min(a.rows, a.cols) > std::min(b.rows, b.cols);
     });
-    for (int i = 0; i < count;) {
-        int64_t bytes = 0;
-        int k = 0;
-        while (i + k < count) {
-            const MuonMatrix& x = t[i + k];
-            const int64_t more = muon_layout(x.rows < x.cols ? x.rows : x.cols, x.rows < x.cols ? x.cols : x.rows, 0).end;
-            if (k > 0 && bytes + more > kMuonWorkspace) break;
-            bytes += more;
-            ++k;
-        }
-        const int rc = muon_group(t + i, k, lr, state, mu, nesterov, wd, steps);
+    const auto all = [&](auto on_floats, auto on_halves) {
+        const int rc = muon_in_groups(
+            rest, floats, [](const MuonMatrix& x) { return muon_float_layout(std::min(x.rows, x.cols), std::max(x.rows, x.cols), 0).end; }, on_floats);
+        if (rc || blocks > 0) return rc;
+        return muon_in_groups(
+            t, halves, [](const MuonMatrix& x) { return muon_layout(std::min(x.rows, x.cols), std::max(x.rows, x.cols), 0).end; }, on_halves);
+    };
+    const auto update = [&](int64_t* need) {
+        return all([&](const MuonMatrix* g, int k) { return muon_float_group(g, k, lr, state, mu, nesterov, wd, steps, need); },
+                   [&](const MuonMatrix* g, int k) { return muon_group(g, k, lr, state, mu, nesterov, wd, steps, need); });
+    };
+    int groups = 0;
+    const auto one = [&](const MuonMatrix*, int) {
+        ++groups;
+        return AETH_OK;
+    };
+    all(one, one);
+    if (groups > 1) {
+        // the scratch of all groups before the first one's launches: a call that cannot have it changes nothing
+        int64_t need = 0;
+        void* ws;
+        update(&need);
+        const int rc = workspace(need, &ws);
         if (rc) return rc;
-        i += k;
     }
-    return AETH_OK;
+    const int rc = update(nullptr);
+    if (rc || blocks == 0) return rc;
+    return muon_small(t, halves, row_blocks, blocks, lr, state, mu, nesterov, wd, steps);
 }
 
 static bool muon_size(int rows, int cols) {

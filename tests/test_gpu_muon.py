@@ -679,3 +679,44 @@ def test_a_resumed_run_in_recorded_training():
         runs.append(_host(model))
         model.record_steps(False)
     assert all(np.array_equal(a, b) for a, b in zip(*runs))
+
+
+@pytest.mark.parametrize("steps", [5, 9])
+def test_a_call_that_cannot_have_its_scratch_changes_nothing(steps):
+    """Two matrices that go out one after the other, with a workspace for the first: a recording refuses one that grows, and what it
+    recorded of the call must be nothing.  (9 steps: both on float32 products.)  In a process of its own, whose workspace is small."""
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    code = """
+import ctypes as C, sys
+sys.path[:0] = [%r, %r]
+import numpy as np
+from aether import DeviceTensor, _lib
+lib, check = _lib.lib(), _lib.check
+steps = %d
+shapes = [(64, 1 << 20), (16000, 16000)]
+t = [[DeviceTensor.full(s, 0.5 + k) for k in range(3)] for s in shapes]
+
+def call(n):
+    table = [(C.c_void_p * n)(*[m[k].ptr for m in t[:n]]) for k in range(3)]
+    return lib.aeth_muon_multi_f32(n, *table, (C.c_int * n)(*[s[0] for s in shapes[:n]]), (C.c_int * n)(*[s[1] for s in shapes[:n]]),
+                                   0.02, 0.95, 1, 0.01, steps)
+
+check(call(1))
+before = [m[k][:4].get() for m in t for k in range(3)]
+check(lib.aeth_graph_begin())
+rc = call(2)
+graph = C.c_void_p()
+check(lib.aeth_graph_end(C.byref(graph)))
+assert rc == -4 and "grow" in lib.aeth_last_error().decode(), rc
+check(lib.aeth_graph_launch(graph))
+assert all(np.array_equal(a, b) for a, b in zip(before, [m[k][:4].get() for m in t for k in range(3)]))
+check(lib.aeth_graph_destroy(graph))
+check(call(2))
+assert not np.array_equal(before[0], t[0][0][:4].get())
+print("done")
+""" % (root, os.path.join(root, "aether-ml_amd"), steps)
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=100)
+    assert r.returncode == 0 and r.stdout.endswith("done\n"), r.stderr[-2000:]
