@@ -196,7 +196,8 @@ class Model:
         learning rate live on the device.  Dropout masks are still drawn on the host, in
         the layers' order from the reference's random stream, and copied into the buffers
         the recorded kernels read before every replay.  Regularisers are recorded: their
-        sums and their gradient terms are kernels like the rest.  Falls back to normal
+        sums and their gradient terms are kernels like the rest.  Other settings of the optimizer
+        (a learning rate set by hand, say) take one normal step before they are recorded.  Falls back to normal
         steps for models the recording cannot express (anything but Adam or Muon with the
         fused softmax / cross-entropy output)."""
         self._record = bool(enabled)

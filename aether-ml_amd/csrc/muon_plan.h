@@ -16,7 +16,7 @@
 namespace aeth {
 
 constexpr int kMuonMax = 32;                             // matrices of a call
-constexpr int kMuonLongest = 1 << 21;                    // rows or columns: a 256-row tile's bytes stay below 2^31
+constexpr int kMuonLongest = 1 << 21;                    // rows or columns: a sum of more float32 products in line would be worth little
 constexpr int kMuonParts = 1024;                          // partial sums of a matrix's norm
 
 MUON_HD int64_t muon_pad(int64_t n) { return (n + 31) / 32 * 32; }
@@ -92,7 +92,8 @@ static inline int64_t muon_tiles(int64_t rows, int64_t cols, int bm, int bn, boo
 // matrix units may draw).  CUs with one tile more than others hold the launch up by `slack` of that tile (several small tiles are
 // on a CU at once).  Fitted to square and wide products of 64 to 4096 rows; the tile with the least cost is taken: 3000 x 3000
 // gram 94 us in tiles of 160 x 160 (120 in 96, 121 in 192, 132 in 64), step 136 in 192 x 192 (169 in 96); 4096 x 4096 gram 180 in
-// 192 x 192 (240 in 160), step 330 in 256 x 128 (373 in 192 x 192).
+// 192 x 192 (240 in 160), step 330 in 256 x 128 (373 in 192 x 192).  (Products alone, repeated; within an update, after one another,
+// the large ones take 2-3 % more.)
 struct MuonTile {
     int bm, bn;
     bool symmetric, general, runs;     // offered for symmetric results, for others, for gram products in runs

@@ -1,10 +1,11 @@
 // Products of matrices whose elements are held as two float16 halves.
 //
-// x = hi + lo with hi = float16(x) and lo = float16(x - hi): 22 bits of x where neither half leaves float16's normal range, for
-// which every matrix is scaled by a power of two (kScale*).  hi.hi + hi.lo + lo.hi is x y up to 2^-22 of |x y| (the product of
-// the low halves is left out), each of the three a float16 MFMA with float32 accumulation.  Three float16 products take 0.19 of the
-// time of one float32 MFMA product of the same size at their peaks (2.5 PFLOP/s and 157 TFLOP/s), and are closer to it than
-// float32 sums of this length are to each other.
+// x = hi + lo with hi = float16(x) and lo = float16(x - hi): 22 bits of x where neither half leaves float16's normal range.  Every
+// matrix is scaled by one power of two (kScale*); the low half is subnormal below 2^-18 of what the scale stands for (1, and |u| = 1
+// for X), where x is held to 2^-40 (B, at half the scale, 2^-39).  hi.hi + hi.lo + lo.hi is x y up to 2^-22 of |x y| (the product of the low halves is left out),
+// each of the three a float16 MFMA with float32 accumulation.  Three float16 products take 0.19 of the time of one float32 MFMA
+// product of the same size at their peaks (2.5 PFLOP/s and 157 TFLOP/s).  muon_in_halves says how many steps of the update that
+// bears: five steps on evenly scaled matrices are off by 2e-6 of the result, with float32 products by 3-4e-6.
 #pragma once
 
 #include "conv_common.h"
@@ -239,7 +240,8 @@ __device__ __forceinline__ f4 split_mfma(const half8& a, const half8& b, const f
 // of 48 x 48, 44 with three of 96 x 32; 4096 x 4096 in 192 x 192: 190 us, with 32 x 32 blocks 198; before the results went through
 // LDS).
 // Bound: with a tile on every CU, the power the matrix units draw (4096 x 4096: 1.15-1.25 PFLOP/s of float16, what a library's
-// float16 product of that size reaches); below that what a CU can have in flight from the L2 caches, 85 GB/s.
+// float16 product of that size reaches); below that, with one wave a SIMD, a slab's barrier, LDS reads and MFMAs one after the other
+// and a tile's first loads and epilogue (more slabs in flight change nothing).
 template <int BM, int BN, int WM, int WN, int NBUF, int BLOCK, int USE>
 __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN)) void split_product(const SplitTable tb, float lr,
                                                                            const double* __restrict__ state, float wd) {

@@ -342,9 +342,9 @@ int aeth_adam_multi_dev_f32(int count, float* const* host_theta, const float* co
  * Any positive multiple of g gives the same o up to roundings (a power of two the same bits, as long as no element becomes
  * subnormal; there is no epsilon); g = 0 gives 0; a NaN or an infinity makes all of o NaN.  g and o are [rows, cols], sides of at
  * most 2^21, and may not overlap.  Precision, sums being float32: while 3.4445^steps sqrt(longer side) <= 2^20 (5 steps at any
- * size, 7 up to 33222, 8 up to 2800, 9 up to 236) the factors of a product hold 22 bits of an element, or 2^-40 of |g| (A, B: of 1)
- * where that is more: rows far below the rest come out with that error of their own.  With more steps, which bring such rows to
- * full size, products are float32 and much slower.
+ * size, 7 up to 33222, 8 up to 2800, 9 up to 236) the factors of a product hold 22 bits of an element, or 2^-40 of |g| (in A
+ * 2^-40, in its polynomial 2^-39) where that is more: rows far below the rest come out with that error of their own.  With more
+ * steps, which bring such rows to full size, products are float32, and slower.
  * aeth_muon_multi_f32 updates `count` (1..32) matrices in one call:
  *     m <- momentum m + grad;  u = grad + momentum m (nesterov != 0) or m;  O = newton_schulz(u);
  *     theta <- theta (1 - lr weight_decay) - lr sqrt(max(1, cols / rows)) O.
