@@ -995,6 +995,8 @@ class Optimizer_Adam:
     def device_state(self):
         """{iterations, beta_1^iterations, beta_2^iterations, lr} as 4 doubles on the device,
         brought in line with ``self.iterations`` and the betas whenever they are others than the recorded steps left."""
+        with _or_drop(self):
+            self._flush()                                    # (as pre_update_parameters: this comes before a recorded step)
         if getattr(self, "_state", None) is None:
             self._state = DeviceTensor(4, np.float64)
             self._state_holds = None
@@ -1175,7 +1177,9 @@ class Optimizer_Muon:
     # -- recorded steps: step number and learning rates live on the device ----------------
     def device_state(self):
         """Adam's state, and for the matrices {iterations, -, -, lr} in the same form."""
-        self.adam.device_state()
+        with _or_drop(self):
+            self._flush()
+            self.adam.device_state()
         if getattr(self, "_state", None) is None:
             self._state = DeviceTensor(4, np.float64)
             self._state_iterations = None

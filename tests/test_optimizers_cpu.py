@@ -12,14 +12,17 @@ class Tensor:
     """Stands for a DeviceTensor: a shape and an address of its own."""
     made = 0
 
-    def __init__(self, shape):
+    def __init__(self, shape, dtype=np.float32):
         Tensor.made += 1
         self.ptr = Tensor.made << 20
-        self.shape = tuple(shape)
+        self.shape = tuple(np.atleast_1d(shape))
         self.size = int(np.prod(self.shape))
 
     def touched(self):
         pass
+
+    def set(self, values):
+        self.values = values
 
     @staticmethod
     def zeros(shape):
@@ -151,3 +154,18 @@ def test_decay_and_step_number_of_muon_are_adams_too(library):
     assert opt.iterations == opt.adam.iterations == 6 and np.isclose(opt.current_learning_rate, .1 / 3.5)
     assert np.isclose(opt.adam.current_learning_rate, .01 / 3.5)
     assert aether.Optimizer_Muon(decay=.25).decay == .25
+
+
+@pytest.mark.parametrize("make", [aether.Optimizer_Adam, aether.Optimizer_Muon])
+def test_a_step_broken_off_goes_out_before_a_replayed_one(library, make):
+    """Not with the next eager step, which may come much later."""
+    opt, layers = make(), [_layer() for _ in range(3)]
+    opt.pre_update_parameters()
+    opt.update_parameters(layers[0])
+    assert not library.calls
+    opt.device_state()                                   # (what a recorded step asks for before its launch)
+    assert _updated(library) == _all(layers[:1])
+    opt.replayed()
+    del library.calls[:]
+    _step(opt, layers)
+    assert _updated(library) == _all(layers)
